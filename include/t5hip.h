@@ -263,6 +263,71 @@ int t5h_embeddings_from_packed(int32_t hip_device, const uint8_t* buf, const siz
                                int32_t cols, float* out, size_t out_cap_rows, int32_t* row_offsets,
                                double* gpu_ms);
 
+/* ---- 8-bit floating point, next to the encoder's f16 and int8 products ----
+ * No counterpart in the reference.  The linears of a layer on OCP e4m3 operands (1-4-3, bias 7,
+ * largest value 448, no infinities, codes 0x7f / 0xff NaN) with a scale per block of 128 values
+ * along the summed axis (the last block of a row may be shorter):
+ *   t5h_fp8_rmsnorm -> t5h_fp8_matmul (q, k, v);  t5h_fp8_quantize -> t5h_fp8_matmul (o);
+ *   t5h_fp8_rmsnorm -> t5h_fp8_gated_gelu -> t5h_fp8_matmul (feed-forward).
+ * Activations: codes [M][K]; one scale per row and block, the power of two 2^(byte - 127), stored
+ * block-major as bytes scales[ceil(K / 128)][M16], M16 = M rounded up to 16 (entries past M are
+ * neither used nor, by the device forms, written).  Weights: codes [N][K]; one scale per 128 x 128
+ * block, scales[ceil(N / 128)][ceil(K / 128)], bytes (T5H_SCALE_E8M0) or f32 (T5H_SCALE_F32).
+ * The scale of a block is the smallest power of two s >= 2^-126 with max|x| <= 448 s, or
+ * max(max|x| / 448, 2^-126) in f32; codes are e4m3(x / s), nearest with ties to even (for f32
+ * scales e4m3(x r), r = 448 / max|x| rounded to f32).  Values that are not finite get a NaN code
+ * and do not count towards the maximum.
+ * Row lengths K, D (and N of the gated product) are multiples of 16; any M, N >= 0 (0: nothing to
+ * do).  Rows are contiguous.  Buffers of the device forms start on 16 bytes (weight scales on their
+ * own size), lie on the current device, and do not overlap outputs except where said; calls are
+ * enqueued on `stream` (a hipStream_t; NULL = the default stream) and return without waiting.  They
+ * allocate nothing and keep no state, so they may be captured into a graph and run concurrently.
+ * The host forms are synchronous, on HIP device hip_device. */
+#define T5H_TYPE_F32 0
+#define T5H_TYPE_F16 1
+#define T5H_TYPE_BF16 2
+#define T5H_SCALE_E8M0 0
+#define T5H_SCALE_F32 1
+
+/* Activations x[M][K] of `type` -> codes[M][K], scales[ceil(K / 128)][M16]. */
+int t5h_fp8_quantize(int32_t hip_device, const void* x, int32_t type, int32_t M, int32_t K, uint8_t* codes,
+                     uint8_t* scales);
+int t5h_fp8_quantize_device(const void* d_x, int32_t type, int32_t M, int32_t K, uint8_t* d_codes,
+                            uint8_t* d_scales, void* stream);
+/* Weights w[N][K] of `type` -> codes[N][K], scales[ceil(N / 128)][ceil(K / 128)] of `scale_type`. */
+int t5h_fp8_quantize_weights(int32_t hip_device, const void* w, int32_t type, int32_t N, int32_t K,
+                             int32_t scale_type, uint8_t* codes, void* scales);
+int t5h_fp8_quantize_weights_device(const void* d_w, int32_t type, int32_t N, int32_t K, int32_t scale_type,
+                                    uint8_t* d_codes, void* d_scales, void* stream);
+/* The residual's addition, T5LayerNorm (src/quantized_t5.rs:163-172) and the activation codes:
+ * h = x + delta rounded to x_type, y = h / sqrt(mean(h^2) + eps) * gamma in f32, codes and scales of
+ * y.  delta may be NULL (h = x).  sum[M][D] of x_type receives h; it may be NULL, x itself, or delta
+ * itself where the two types have one size; it needs a delta. */
+int t5h_fp8_rmsnorm(int32_t hip_device, const void* x, int32_t x_type, const void* delta, int32_t delta_type,
+                    int32_t M, int32_t D, const float* gamma, float eps, void* sum, uint8_t* codes,
+                    uint8_t* scales);
+int t5h_fp8_rmsnorm_device(const void* d_x, int32_t x_type, const void* d_delta, int32_t delta_type, int32_t M,
+                           int32_t D, const float* d_gamma, float eps, void* d_sum, uint8_t* d_codes,
+                           uint8_t* d_scales, void* stream);
+/* c[M][N] = a . w^T over the values that codes and scales stand for, rounded once to c_type.  F32
+ * results are f32 sums of exact products.  For F16 and BF16 results the fp8 matrix instructions
+ * align each group of 8 to 16 products to the group's largest with about 14 bits, 1e-5 of the
+ * result's norm on ordinary data and below those types' rounding; sums of groups are f32. */
+int t5h_fp8_matmul(int32_t hip_device, const uint8_t* a, const uint8_t* a_scales, int32_t M, const uint8_t* w,
+                   const void* w_scales, int32_t N, int32_t K, int32_t scale_type, void* c, int32_t c_type);
+int t5h_fp8_matmul_device(const uint8_t* d_a, const uint8_t* d_a_scales, int32_t M, const uint8_t* d_w,
+                          const void* d_w_scales, int32_t N, int32_t K, int32_t scale_type, void* d_c,
+                          int32_t c_type, void* stream);
+/* The gated feed-forward's first half (src/quantized_t5.rs:231-249): y = gelu(a . w0^T) * (a . w1^T)
+ * with the tanh gelu, as the codes [M][N] and scales [ceil(N / 128)][M16] of the next product's
+ * activations.  w0 and w1 share a scale type.  Products as for F16 results. */
+int t5h_fp8_gated_gelu(int32_t hip_device, const uint8_t* a, const uint8_t* a_scales, int32_t M, const uint8_t* w0,
+                       const void* w0_scales, const uint8_t* w1, const void* w1_scales, int32_t N, int32_t K,
+                       int32_t scale_type, uint8_t* codes, uint8_t* scales);
+int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int32_t M, const uint8_t* d_w0,
+                              const void* d_w0_scales, const uint8_t* d_w1, const void* d_w1_scales, int32_t N,
+                              int32_t K, int32_t scale_type, uint8_t* d_codes, uint8_t* d_scales, void* stream);
+
 /* One T5Block (src/quantized_t5.rs:598-627) on packed sequences: x_in/x_out are
  * host [T, d_model] f32. */
 int t5h_layer_forward(t5h_model* model, int32_t layer, const float* x_in,

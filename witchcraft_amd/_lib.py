@@ -23,6 +23,12 @@ T5H_NUMERICS_DEFAULT = 0
 T5H_NUMERICS_HYBRID = 1
 T5H_NUMERICS_HYBRID_BF16 = 2
 
+T5H_TYPE_F32 = 0
+T5H_TYPE_F16 = 1
+T5H_TYPE_BF16 = 2
+T5H_SCALE_E8M0 = 0
+T5H_SCALE_F32 = 1
+
 
 class T5HConfig(C.Structure):
     _fields_ = [
@@ -84,6 +90,22 @@ SIGNATURES = {
     "t5h_embeddings_from_packed": (C.c_int, [C.c_int32, _u8p, np.ctypeslib.ndpointer(np.uint64, flags="C_CONTIGUOUS"),
                                              C.c_int32, C.c_int32, _f32p, C.c_size_t, _i32p,
                                              C.POINTER(C.c_double)]),
+    "t5h_fp8_quantize": (C.c_int, [C.c_int32, _vp, C.c_int32, C.c_int32, C.c_int32, _vp, _vp]),
+    "t5h_fp8_quantize_device": (C.c_int, [_vp, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp]),
+    "t5h_fp8_quantize_weights": (C.c_int, [C.c_int32, _vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp]),
+    "t5h_fp8_quantize_weights_device": (C.c_int, [_vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp]),
+    "t5h_fp8_rmsnorm": (C.c_int, [C.c_int32, _vp, C.c_int32, _vp, C.c_int32, C.c_int32, C.c_int32, _vp, C.c_float, _vp,
+                                  _vp, _vp]),
+    "t5h_fp8_rmsnorm_device": (C.c_int, [_vp, C.c_int32, _vp, C.c_int32, C.c_int32, C.c_int32, _vp, C.c_float, _vp, _vp,
+                                         _vp, _vp]),
+    "t5h_fp8_matmul": (C.c_int, [C.c_int32, _vp, _vp, C.c_int32, _vp, _vp, C.c_int32, C.c_int32, C.c_int32, _vp,
+                                 C.c_int32]),
+    "t5h_fp8_matmul_device": (C.c_int, [_vp, _vp, C.c_int32, _vp, _vp, C.c_int32, C.c_int32, C.c_int32, _vp, C.c_int32,
+                                        _vp]),
+    "t5h_fp8_gated_gelu": (C.c_int, [C.c_int32, _vp, _vp, C.c_int32, _vp, _vp, _vp, _vp, C.c_int32, C.c_int32, C.c_int32,
+                                     _vp, _vp]),
+    "t5h_fp8_gated_gelu_device": (C.c_int, [_vp, _vp, C.c_int32, _vp, _vp, _vp, _vp, C.c_int32, C.c_int32, C.c_int32, _vp,
+                                            _vp, _vp]),
     "t5h_layer_forward": (C.c_int, [_vp, C.c_int32, _f32p, _i32p, C.c_int32, _f32p]),
     "t5h_ffn_block": (C.c_int, [_vp, C.c_int32, _f32p, C.c_int32, _f32p, C.c_int32]),
     "t5h_set_profiling": (C.c_int, [_vp, C.c_int32]),
