@@ -18,6 +18,8 @@
 // v_mfma_f32_16x16x32_f16, at half the rate, from codes widened to f16 (every e4m3 value is one).
 #include "fp8.hpp"
 
+#include <atomic>
+
 namespace {
 using namespace t5k;
 
@@ -34,19 +36,32 @@ __device__ __forceinline__ h8 widen8(int lo, int hi) {
             (_Float16)c[0], (_Float16)c[1], (_Float16)d[0], (_Float16)d[1]};
 }
 
+struct Wide {
+  h8 v[4];
+};
+__device__ __forceinline__ Wide widen(const i8v& x) {
+  Wide r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) r.v[i] = widen8(x[2 * i], x[2 * i + 1]);
+  return r;
+}
+
 // acc += one K block of a 16 x 16 tile.  sa: the scale byte of the lane's row (l % 16); swb / swf: the
 // weights' byte or float.
+template <int ST>
+__device__ __forceinline__ void wide_product(const Wide& w, const Wide& a, uint32_t sa, uint32_t swb, float swf, f4& acc) {
+  f4 t = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; i++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], a.v[i], t, 0, 0, 0);
+  const float f = e8m0_value(sa) * (ST == FP8_E8M0 ? e8m0_value(swb) : swf);
+#pragma unroll
+  for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(t[e], f, acc[e]);
+}
 template <bool EXACT, int ST>
 __device__ __forceinline__ void block_product(const i8v& w, const i8v& a, uint32_t sa, uint32_t swb, float swf, f4& acc) {
   const f4 zero = f4{0.f, 0.f, 0.f, 0.f};
   if constexpr (EXACT) {
-    f4 t = zero;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      t = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(w[2 * i], w[2 * i + 1]), widen8(a[2 * i], a[2 * i + 1]), t, 0, 0, 0);
-    const float f = e8m0_value(sa) * (ST == FP8_E8M0 ? e8m0_value(swb) : swf);
-#pragma unroll
-    for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(t[e], f, acc[e]);
+    wide_product<ST>(widen(w), widen(a), sa, swb, swf, acc);
   } else if constexpr (ST == FP8_E8M0) {
     acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, (int)swb, 0, (int)sa);
   } else {
@@ -240,6 +255,351 @@ __global__ __launch_bounds__(512 * KS) void fp8_small_gated_kernel(Fp8GemmArgs p
   }
 }
 
+// ---- tiles: BM rows x BN weight rows per workgroup, K blocks through a double buffer in LDS --------
+// WM x WN waves, each MT x NT tiles of 16 x 16.  Both operands go global -> LDS without registers, a
+// K block (128 bytes of every row) per step; a row's eight 16-byte chunks are stored rotated (xor) by a
+// function of the row, so that the 16 rows that a wave reads at once spread over all banks.
+//  * A wave's activation rows are dealt out as row = MT (l % 16) + i for tile i, so that a lane's
+//    scale bytes of one K block are MT consecutive ones: a dword holds four tiles' scales, and the
+//    instruction picks its byte.
+//  * Weight scales, one per K block and wave, sit in a register of the lane kb % 64.
+//  * Step kb + 1's data has been requested one step ahead; the wait for it, and the barrier after which
+//    step kb's buffer is refilled, come before the last row of MFMAs of step kb, whose operands are
+//    in registers by then, so the first operands of step kb + 1 are read behind those MFMAs.
+// Out-of-range rows and K chunks past K read as zero through the buffer descriptors' range.
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+// Raw buffer of `bytes` bytes at a wave-uniform base; reads past it give zero.
+__device__ __forceinline__ i4v buffer_at(const void* base, uint32_t bytes) {
+  const uint64_t b = (uint64_t)(uintptr_t)base;
+  return i4v{__builtin_amdgcn_readfirstlane((int)(uint32_t)b), __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff),
+             __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+// Global -> LDS copies as inline asm, so that the compiler adds no waits for them at LDS reads: the
+// kernel's own vmcnt waits and barriers order them.  Lane l's bytes land at m0 + 16 l (4 l).
+__device__ __forceinline__ void lds_copy16(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
+               "s"(m0)
+               : "memory");
+}
+__device__ __forceinline__ void lds_copy4(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
+               "s"(m0)
+               : "memory");
+}
+constexpr uint32_t kOutside = 0x7fffffffu;  // past every descriptor's range
+constexpr int kTileMaxK = 1 << 21;          // 256 rows' bytes fit a descriptor and a lane's offset
+
+template <int SEL, int ST>
+__device__ __forceinline__ void tile_product_sel(const i8v& w, const i8v& a, uint32_t sa4, uint32_t swb, float swf, f4& acc) {
+  const f4 zero = f4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (ST == FP8_E8M0) {
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, (int)swb, SEL, (int)sa4);
+  } else {
+    const f4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, zero, 0, 0, 0, 127, SEL, (int)sa4);
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(t[e], swf, acc[e]);
+  }
+}
+template <int ST>
+__device__ __forceinline__ void tile_product(const i8v& w, const i8v& a, uint32_t sa4, int sel, uint32_t swb, float swf, f4& acc) {
+  switch (sel) {  // a constant once the loops are unrolled
+    case 0: tile_product_sel<0, ST>(w, a, sa4, swb, swf, acc); break;
+    case 1: tile_product_sel<1, ST>(w, a, sa4, swb, swf, acc); break;
+    case 2: tile_product_sel<2, ST>(w, a, sa4, swb, swf, acc); break;
+    default: tile_product_sel<3, ST>(w, a, sa4, swb, swf, acc); break;
+  }
+}
+
+// Tile of the launch's index: bands of 8 row tiles, walked column by column, a contiguous stretch of
+// them per XCD (workgroups are dealt to the 8 XCDs in turn), so that what runs at one time on an XCD
+// is a patch of 8 row tiles by a few column tiles and its L2 serves both operands.
+__device__ __forceinline__ void tile_place(uint32_t tiles, int tiles_m, int tiles_n, uint32_t i, int& tm, int& tn) {
+  const uint32_t x = i % 8, rest = tiles % 8;
+  const uint32_t t = x * (tiles / 8) + min(x, rest) + i / 8;
+  const uint32_t wide = 8u * (uint32_t)tiles_n, band = t / wide, in = t - band * wide;
+  const uint32_t h = min(8u, (uint32_t)tiles_m - band * 8);
+  tm = (int)(band * 8 + in % h);
+  tn = (int)(in / h);
+}
+
+// The values of one 16-row stripe of a wave's tile (row l % 16 of each lane, columns 16 j + 4 (l / 16)),
+// stored as whole 16-byte pieces of its rows through the wave's own LDS (16 rows of 16 NT columns of a
+// 2-byte type, half of them of a 4-byte one), rotated like the operands.  mrow(i): the row of C of the
+// stripe's row i.  N that does not divide into such pieces is stored by single values.
+template <int OUT, int NT, typename Row>
+__device__ __forceinline__ void store_stripe(const Fp8GemmArgs& p, uint8_t* stage, int lane, int n0, const f4 (&v)[NT],
+                                             Row mrow) {
+  constexpr int SZ = OUT == FP8_IO_F32 ? 4 : 2, PASSES = SZ / 2, TJ = NT / PASSES, ROWB = TJ * 16 * SZ, CH = ROWB / 16;
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int h = 0; h < PASSES; h++) {
+#pragma unroll
+    for (int j = 0; j < TJ; j++) {
+      const int b = (16 * j + 4 * g) * SZ;  // byte within the row
+      uint8_t* at = stage + r * ROWB + (((b >> 4) ^ (r & 7)) << 4) + (b & 15);
+      if constexpr (OUT == FP8_IO_F32) *reinterpret_cast<f4*>(at) = v[h * TJ + j];
+      else if constexpr (OUT == FP8_IO_F16) *reinterpret_cast<h4*>(at) = __builtin_convertvector(v[h * TJ + j], h4);
+      else *reinterpret_cast<b4*>(at) = __builtin_convertvector(v[h * TJ + j], b4);
+    }
+    const int nh = n0 + h * TJ * 16;
+    if (p.N % (16 / SZ) == 0) {
+#pragma unroll
+      for (int q = 0; q < 16 * CH / 64; q++) {
+        const int row = (q * 64 + lane) / CH, c = (q * 64 + lane) % CH, m = mrow(row), n = nh + c * (16 / SZ);
+        if (m < p.M && n < p.N)
+          *reinterpret_cast<uint4*>((uint8_t*)p.out + ((size_t)m * p.N + n) * SZ) =
+              *reinterpret_cast<const uint4*>(stage + row * ROWB + ((c ^ (row & 7)) << 4));
+      }
+    } else {
+      for (int q = lane; q < 16 * TJ * 16; q += 64) {
+        const int row = q / (TJ * 16), c = q % (TJ * 16), m = mrow(row), n = nh + c, b = c * SZ;
+        const uint8_t* at = stage + row * ROWB + (((b >> 4) ^ (row & 7)) << 4) + (b & 15);
+        if (m < p.M && n < p.N) {
+          if constexpr (SZ == 4) ((float*)p.out)[(size_t)m * p.N + n] = *reinterpret_cast<const float*>(at);
+          else ((uint16_t*)p.out)[(size_t)m * p.N + n] = *reinterpret_cast<const uint16_t*>(at);
+        }
+      }
+    }
+  }
+}
+
+// OUT: the result's type; F32 results take the f16 matrix instructions (see the top of the file).
+// GATED: BN / 2 = 128 columns of both matrices, the result is codes.
+template <int OUT, int ST, bool GATED, int BM, int BN, int WM, int WN, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+  constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
+  constexpr int NW = WM * WN, MT = BM / 16 / WM, NT = BN / 16 / WN, STAGE = (BM + BN) * 128, ND = (BM + BN) / 8 / NW;
+  constexpr int COLS = GATED ? BN / 2 : BN, SCALES = 2 * STAGE, TOPS = SCALES + 512;
+  constexpr int OUTS = TOPS + (GATED ? WN * BM * 4 : 0), GI = 4;  // GI: stripes whose codes are staged at once
+  constexpr int LDS = OUTS + (GATED ? WM * 16 * GI * 128 : NW * 16 * 16 * NT * 2);
+  static_assert((BM + BN) % (8 * NW) == 0 && MT % 4 == 0 && BM <= 256 && (!GATED || COLS == FP8_BLOCK), "whole copies");
+  static_assert(GATED || 16 * NT <= FP8_BLOCK, "one weight scale per wave and K block");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
+  const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK, m16 = (int)fp8_scale_rows(p.M);
+  const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
+
+  // ---- the stream of copies: K block after K block, tile after tile, two steps ahead of the products.
+  // Copies of 8 rows of 128 bytes each: lane l brings chunk (l % 8) ^ f(row) of row l / 8 to place l % 8.
+  // A copy whose rows are all past the matrix brings the tile's first ones, which nothing uses.  The
+  // scalar offset stays below one row, and so within every descriptor.
+  i4v rs[ND], rsc;
+  uint32_t fx[ND];
+  const uint32_t rowk = (uint32_t)(lane >> 3) * (uint32_t)p.K;
+#pragma unroll
+  for (int j = 0; j < ND; j++) {
+    const int q = wave * ND + j;
+    fx[j] = 16u * ((lane & 7) ^ ((8 * q < BM ? (8 * q + (lane >> 3)) / MT : lane >> 3) & 7));
+  }
+  uint32_t ctile = blockIdx.x;
+  int ckb = 0, climit = p.K;  // climit 0: past the last tile, zeros
+  auto aim = [&]() {          // the descriptors of tile ctile
+    int tm, tn;
+    tile_place(tiles, tiles_m, tiles_n, ctile, tm, tn);
+    const int m0 = tm * BM, n0 = tn * COLS;
+#pragma unroll
+    for (int j = 0; j < ND; j++) {
+      const int q = wave * ND + j;
+      const bool is_a = 8 * q < BM, up = GATED && 8 * q - BM >= COLS;
+      int row = is_a ? 8 * q : (up ? 8 * q - BM - COLS : 8 * q - BM);
+      const int first = is_a ? m0 : n0, end = is_a ? p.M : p.N;
+      if (first + row >= end) row = 0;
+      rs[j] = buffer_at((is_a ? p.a : (up ? p.w1 : p.w)) + (size_t)(first + row) * p.K,
+                        (uint32_t)min(8, end - first - row) * (uint32_t)p.K);
+    }
+    // the rows' scale bytes of a K block: BM of them (whole dwords: m16 and m0 are multiples of 16)
+    rsc = buffer_at(p.a_scales + m0, (uint32_t)((size_t)kbs * m16 - m0));
+  };
+  const uint32_t lds0 = lds_offset(lds), vsc = lane < BM / 4 ? 4u * lane : kOutside;
+  auto copy = [&](uint32_t slot) {
+    const uint32_t at = lds0 + slot * STAGE + wave * ND * 1024;
+#pragma unroll
+    for (int j = 0; j < ND; j++)
+      lds_copy16(rs[j], ckb * 128 + (int)fx[j] < climit ? rowk + fx[j] : kOutside, ckb * 128, at + 1024 * j);
+    lds_copy4(rsc, vsc, ckb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
+    ckb++;
+  };
+  auto next_tile = [&]() {
+    ckb = 0;
+    ctile += gridDim.x;
+    if (ctile < tiles) aim();
+    else climit = 0;
+  };
+
+  // ---- weight scales: lane k holds those of K block kb + k of this wave's column block
+  uint32_t ws[GATED ? 2 : 1], wsn[GATED ? 2 : 1];
+  auto weight_scales = [&](int n0, int kb, uint32_t (&to)[GATED ? 2 : 1]) {
+    const int nb = min(n0 + (GATED ? 0 : wn * 16 * NT), p.N - 1) / FP8_BLOCK;
+    const size_t at = (size_t)nb * kbs + min(kb + lane, kbs - 1);
+#pragma unroll
+    for (int j = 0; j < (GATED ? 2 : 1); j++) {
+      const void* s = j ? p.w1_scales : p.w_scales;
+      to[j] = ST == FP8_E8M0 ? ((const uint8_t*)s)[at] : __float_as_uint(((const float*)s)[at]);
+    }
+  };
+
+  f4 acc[MT][NT];
+  i8v a[2], w[NT];
+  Wide ww[EXACT ? NT : 1];
+  uint32_t sa[MT / 4];
+  // lane's chunks g and g + 4 of its row: places (g ^ f) and (g ^ f) ^ 4
+  const int arow = wm * 16 * MT + r * MT, wrow = (GATED ? wn * 8 * NT : wn * 16 * NT) + r;
+  const uint32_t place = 16 * (g ^ (r & 7));
+  uint32_t alo = arow * 128 + place, ahi = arow * 128 + (place ^ 64);  // in the current step's buffer
+  uint32_t wlo = (BM + wrow) * 128 + place, whi = (BM + wrow) * 128 + (place ^ 64), sat = SCALES + arow;
+  auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
+    const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
+    v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  };
+  auto read_w = [&](int j) {
+    const int o = (GATED ? (j < NT / 2 ? 16 * j : COLS + 16 * (j - NT / 2)) : 16 * j) * 128;
+    read(wlo + o, whi + o, w[j]);
+  };
+  auto read_scales = [&]() {
+#pragma unroll
+    for (int c = 0; c < MT / 4; c++) sa[c] = *reinterpret_cast<const uint32_t*>(lds + sat + 4 * c);
+  };
+
+  int tm, tn;
+  tile_place(tiles, tiles_m, tiles_n, ctile, tm, tn);
+  aim();
+  copy(0);
+  weight_scales(tn * COLS, 0, ws);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("s_barrier" ::: "memory");
+  if (ckb == kbs) next_tile();
+  copy(1);
+  read_scales();
+#pragma unroll
+  for (int j = 0; j < NT; j++) read_w(j);
+  read(alo, ahi, a[0]);
+  uint32_t slot = 0;
+
+  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int m0 = tm * BM, n0 = tn * COLS;
+    if (tile + gridDim.x < tiles) tile_place(tiles, tiles_m, tiles_n, tile + gridDim.x, tm, tn);
+    weight_scales(tn * COLS, 0, wsn);  // of the next tile: complete after the first step's wait
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+    int kb = 0;
+    do {
+      if (kb && (kb & 63) == 0) {
+        weight_scales(n0, kb, ws);
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+      }
+      if (ckb == kbs) next_tile();
+      uint32_t swb[GATED ? 2 : 1];
+#pragma unroll
+      for (int j = 0; j < (GATED ? 2 : 1); j++) swb[j] = __builtin_amdgcn_readlane(ws[j], kb & 63);
+      if constexpr (EXACT) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) ww[j] = widen(w[j]);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        const uint32_t sc = sa[i / 4];
+        if (i < MT - 1) {
+          read(alo + (i + 1) * 128, ahi + (i + 1) * 128, a[(i + 1) & 1]);
+        } else {
+          // the next step's data has landed and this step's operands are all in registers
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_waitcnt(0x0f70);
+          asm volatile("s_barrier" ::: "memory");
+          copy(slot);
+          slot ^= 1;
+          const uint32_t step = slot ? STAGE : -STAGE;
+          alo += step, ahi += step, wlo += step, whi += step, sat += slot ? 256 : -256;
+          read_scales();
+          read(alo, ahi, a[0]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        Wide wa;
+        if constexpr (EXACT) wa = widen(a[i & 1]);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const uint32_t s = swb[GATED && j >= NT / 2 ? 1 : 0];
+          if constexpr (EXACT) wide_product<ST>(ww[j], wa, (sc >> (8 * (i % 4))) & 255, s, __uint_as_float(s), acc[i][j]);
+          else tile_product<ST>(w[j], a[i & 1], sc, i % 4, s, __uint_as_float(s), acc[i][j]);
+          if (i == MT - 1) {  // each weight operand is replaced as soon as it has been used
+            __builtin_amdgcn_sched_barrier(0);
+            read_w(j);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      kb++;
+    } while (kb < kbs);
+
+    if constexpr (!GATED) {
+      uint8_t* stage = lds + OUTS + wave * (16 * 16 * NT * 2);
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        const int row0 = m0 + wm * 16 * MT + i;
+        store_stripe<OUT, NT>(p, stage, lane, n0 + wn * NT * 16, acc[i], [&](int q) { return row0 + q * MT; });
+      }
+    } else {
+      // rows' maxima over the 128 columns, from WN waves; then the codes through LDS, in whole rows
+      float* tops = reinterpret_cast<float*>(lds + TOPS);  // [WN][BM]
+      uint8_t* stage = lds + OUTS;                         // [GI][WM * 16][128], 16-byte chunks rotated
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < NT / 2; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float y = gelu_tanh_dev(acc[i][j][e]) * acc[i][j + NT / 2][e];
+            acc[i][j][e] = y;
+            if (n0 + (wn * NT / 2 + j) * 16 < p.N) top = fmaxf(top, finite_abs(y));
+          }
+        top = max_xor32(max_xor16(top));
+        if (g == 0) tops[wn * BM + arow + i] = top;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+      for (int i0 = 0; i0 < MT; i0 += GI) {
+#pragma unroll
+        for (int i = i0; i < i0 + GI; i++) {
+          const int row = arow + i;
+          float top = tops[row];
+#pragma unroll
+          for (int c = 1; c < WN; c++) top = fmaxf(top, tops[c * BM + row]);
+          const uint32_t byte = e8m0_of(top);
+          const float inv = e8m0_inverse(byte);
+#pragma unroll
+          for (int j = 0; j < NT / 2; j++) {
+            const int c = wn * NT / 2 + j;  // 16-byte chunk of the row
+            *reinterpret_cast<uint32_t*>(stage + ((i - i0) * WM * 16 + wm * 16 + r) * 128 + 16 * (c ^ (r & 7)) + 4 * g) =
+                e4m3_pack4(acc[i][j][0] * inv, acc[i][j][1] * inv, acc[i][j][2] * inv, acc[i][j][3] * inv);
+          }
+          if (wn == 0 && g == 0 && m0 + row < p.M) p.out_scales[(size_t)(n0 / FP8_BLOCK) * m16 + m0 + row] = (uint8_t)byte;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < GI * WM * 16 * 8 / (64 * NW); q++) {
+          const int at = (q * 64 * NW + tid) >> 3, c = tid & 7, i = at / (WM * 16), rr = at % 16;
+          const int m = m0 + ((at / 16) % WM) * 16 * MT + rr * MT + i0 + i;
+          if (m < p.M && n0 + 16 * c < p.N)
+            *reinterpret_cast<uint4*>((uint8_t*)p.out + (size_t)m * p.N + n0 + 16 * c) =
+                *reinterpret_cast<const uint4*>(stage + at * 128 + 16 * (c ^ (rr & 7)));
+        }
+        // the stage is written again
+        if (i0 + GI < MT) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < (GATED ? 2 : 1); j++) ws[j] = wsn[j];
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
+}
+
 constexpr int64_t kMostGroups = 1 << 20;  // workgroups of a launch; the kernels walk what is left
 
 template <bool EXACT, int ST, int MB, int NB, int KS>
@@ -259,25 +619,69 @@ hipError_t launch_small_gated(const Fp8GemmArgs& p, hipStream_t s) {
              p, tiles_n, tiles);
   return hipGetLastError();
 }
+
+template <int OUT, int ST, bool GATED, int BM, int BN, int WM, int WN, int OCC>
+hipError_t launch_tile(const Fp8GemmArgs& p, int cus, hipStream_t s) {
+  constexpr int COLS = GATED ? BN / 2 : BN;
+  const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + COLS - 1) / COLS;
+  const int64_t tiles = (int64_t)tiles_m * tiles_n;
+  constexpr int per = OCC * 4 / (WM * WN) > 0 ? OCC * 4 / (WM * WN) : 1;  // workgroups per compute unit
+  if (p.K > kTileMaxK || tiles >> 30) return hipErrorInvalidValue;
+  T5K_LAUNCH((fp8_tile_kernel<OUT, ST, GATED, BM, BN, WM, WN, OCC>), dim3((unsigned)std::min<int64_t>(tiles, cus * per)),
+             dim3(64 * WM * WN), 0, s, p, tiles_m, tiles_n);
+  return hipGetLastError();
+}
+
+// Compute units of the current device, asked for once per device.
+int compute_units() {
+  static std::atomic<int> known[64];
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if ((cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+  known[dev].store(cus, std::memory_order_relaxed);
+  return cus;
+}
+
+template <int OUT, int ST>
+hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
+  if (p.M <= 64 || p.K > kTileMaxK) return launch_small<OUT == FP8_IO_F32, ST, 2, 2, 4>(p, s);
+  const int cus = compute_units();
+  if constexpr (OUT != FP8_IO_F32) {
+    if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= cus) return launch_tile<OUT, ST, false, 256, 256, 2, 4, 2>(p, cus, s);
+  }
+  return launch_tile<OUT, ST, false, 128, 128, 2, 2, 2>(p, cus, s);
+}
+
+template <int ST>
+hipError_t launch_gated(const Fp8GemmArgs& p, hipStream_t s) {
+  if (p.M <= 64 || p.K > kTileMaxK) return launch_small_gated<ST, 2, 1>(p, s);
+  const int cus = compute_units();
+  if ((int64_t)((p.M + 255) / 256) * ((p.N + 127) / 128) >= 2 * cus) return launch_tile<FP8_IO_NONE, ST, true, 256, 256, 2, 4, 2>(p, cus, s);
+  return launch_tile<FP8_IO_NONE, ST, true, 128, 256, 2, 4, 2>(p, cus, s);
+}
 }  // namespace
 
 namespace t5k {
 hipError_t launch_fp8_matmul(const Fp8GemmArgs& p, hipStream_t s) {
   if (p.M == 0 || p.N == 0) return hipSuccess;
   if (p.M < 0 || p.N < 0 || p.K <= 0 || p.K % 16) return hipErrorInvalidValue;
-  const bool exact = p.out_type == FP8_IO_F32;
-  if (p.scale_type == FP8_E8M0)
-    return exact ? launch_small<true, FP8_E8M0, 2, 2, 4>(p, s) : launch_small<false, FP8_E8M0, 2, 2, 4>(p, s);
-  if (p.scale_type == FP8_F32)
-    return exact ? launch_small<true, FP8_F32, 2, 2, 4>(p, s) : launch_small<false, FP8_F32, 2, 2, 4>(p, s);
+  switch (2 * p.out_type + p.scale_type) {
+    case 2 * FP8_IO_F32 + FP8_E8M0: return launch_product<FP8_IO_F32, FP8_E8M0>(p, s);
+    case 2 * FP8_IO_F32 + FP8_F32: return launch_product<FP8_IO_F32, FP8_F32>(p, s);
+    case 2 * FP8_IO_F16 + FP8_E8M0: return launch_product<FP8_IO_F16, FP8_E8M0>(p, s);
+    case 2 * FP8_IO_F16 + FP8_F32: return launch_product<FP8_IO_F16, FP8_F32>(p, s);
+    case 2 * FP8_IO_BF16 + FP8_E8M0: return launch_product<FP8_IO_BF16, FP8_E8M0>(p, s);
+    case 2 * FP8_IO_BF16 + FP8_F32: return launch_product<FP8_IO_BF16, FP8_F32>(p, s);
+  }
   return hipErrorInvalidValue;
 }
 
 hipError_t launch_fp8_gated_gelu(const Fp8GemmArgs& p, hipStream_t s) {
   if (p.M == 0 || p.N == 0) return hipSuccess;
   if (p.M < 0 || p.N < 0 || p.N % 16 || p.K <= 0 || p.K % 16) return hipErrorInvalidValue;
-  if (p.scale_type == FP8_E8M0) return launch_small_gated<FP8_E8M0, 2, 1>(p, s);
-  if (p.scale_type == FP8_F32) return launch_small_gated<FP8_F32, 2, 1>(p, s);
+  if (p.scale_type == FP8_E8M0) return launch_gated<FP8_E8M0>(p, s);
+  if (p.scale_type == FP8_F32) return launch_gated<FP8_F32>(p, s);
   return hipErrorInvalidValue;
 }
 }  // namespace t5k
