@@ -371,11 +371,14 @@ __device__ __forceinline__ void store_stripe(const Fp8GemmArgs& p, uint8_t* stag
 template <int OUT, int ST, bool GATED, int BM, int BN, int WM, int WN, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
   constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
-  constexpr int NW = WM * WN, MT = BM / 16 / WM, NT = BN / 16 / WN, STAGE = (BM + BN) * 128, ND = (BM + BN) / 8 / NW;
+  constexpr int NW = WM * WN, MT = BM / 16 / WM, NT = BN / 16 / WN, STAGE = (BM + BN) * 128;
+  constexpr int H = MT / 2;                                      // stripes of a half step
+  constexpr int CA = BM / 16 / NW, CW = BN / 8 / NW;             // copies per wave: of each half of the rows, of weights
   constexpr int COLS = GATED ? BN / 2 : BN, SCALES = 2 * STAGE, TOPS = SCALES + 512;
   constexpr int OUTS = TOPS + (GATED ? WN * BM * 4 : 0), GI = 4;  // GI: stripes whose codes are staged at once
   constexpr int LDS = OUTS + (GATED ? WM * 16 * GI * 128 : NW * 16 * 16 * NT * 2);
-  static_assert((BM + BN) % (8 * NW) == 0 && MT % 4 == 0 && BM <= 256 && (!GATED || COLS == FP8_BLOCK), "whole copies");
+  static_assert(BM % (16 * NW) == 0 && BN % (8 * NW) == 0 && MT % 4 == 0 && BM <= 256, "whole copies, whole scale dwords");
+  static_assert(!GATED || COLS == FP8_BLOCK, "a workgroup has all columns of a scale");
   static_assert(GATED || 16 * NT <= FP8_BLOCK, "one weight scale per wave and K block");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -383,51 +386,70 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
   const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK, m16 = (int)fp8_scale_rows(p.M);
   const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
 
-  // ---- the stream of copies: K block after K block, tile after tile, two steps ahead of the products.
-  // Copies of 8 rows of 128 bytes each: lane l brings chunk (l % 8) ^ f(row) of row l / 8 to place l % 8.
-  // A copy whose rows are all past the matrix brings the tile's first ones, which nothing uses.  The
-  // scalar offset stays below one row, and so within every descriptor.
-  i4v rs[ND], rsc;
-  uint32_t fx[ND];
-  const uint32_t rowk = (uint32_t)(lane >> 3) * (uint32_t)p.K;
+  // ---- copies.  One brings K block kb of 8 rows: lane l chunk (l % 8) ^ (l / 8) of its row l / 8, to place
+  // l % 8.  In LDS the activation rows are ordered by stripe, [MT][WM][16]; consecutive rows there lie MT
+  // apart in memory.  A copy whose rows are all past the matrix brings the tile's first ones, which
+  // nothing uses.  The scalar offset stays below one row, and so within every descriptor.
+  struct Cursor {
+    uint32_t tile;
+    int kb, limit;  // limit: K, or 0 past the last tile (zeros)
+  };
+  Cursor c1 = {blockIdx.x, 0, p.K}, c2 = c1;  // of weights and the first stripes, of the last stripes
+  i4v rw[CW], ra[2][CA], rsc;
+  auto row_buffer = [&](const uint8_t* base, int first, int row, int end, int rows) {
+    if (first + row >= end) row = 0;
+    return buffer_at(base + (size_t)(first + row) * p.K, (uint32_t)min(rows, end - first - row) * (uint32_t)p.K);
+  };
+  auto aim_rows = [&](int half, int m0) {
 #pragma unroll
-  for (int j = 0; j < ND; j++) {
-    const int q = wave * ND + j;
-    fx[j] = 16u * ((lane & 7) ^ ((8 * q < BM ? (8 * q + (lane >> 3)) / MT : lane >> 3) & 7));
-  }
-  uint32_t ctile = blockIdx.x;
-  int ckb = 0, climit = p.K;  // climit 0: past the last tile, zeros
-  auto aim = [&]() {          // the descriptors of tile ctile
+    for (int j = 0; j < CA; j++) {
+      const int q = 8 * ((half * NW + wave) * CA + j);  // LDS row: stripe q / (16 WM)
+      ra[half][j] = row_buffer(p.a, m0, (q / 16 % WM) * 16 * MT + (q & 8) * MT + q / (16 * WM), p.M, 7 * MT + 1);
+    }
+  };
+  auto aim1 = [&]() {
     int tm, tn;
-    tile_place(tiles, tiles_m, tiles_n, ctile, tm, tn);
+    tile_place(tiles, tiles_m, tiles_n, c1.tile, tm, tn);
     const int m0 = tm * BM, n0 = tn * COLS;
 #pragma unroll
-    for (int j = 0; j < ND; j++) {
-      const int q = wave * ND + j;
-      const bool is_a = 8 * q < BM, up = GATED && 8 * q - BM >= COLS;
-      int row = is_a ? 8 * q : (up ? 8 * q - BM - COLS : 8 * q - BM);
-      const int first = is_a ? m0 : n0, end = is_a ? p.M : p.N;
-      if (first + row >= end) row = 0;
-      rs[j] = buffer_at((is_a ? p.a : (up ? p.w1 : p.w)) + (size_t)(first + row) * p.K,
-                        (uint32_t)min(8, end - first - row) * (uint32_t)p.K);
+    for (int j = 0; j < CW; j++) {
+      const int q = 8 * (wave * CW + j);
+      const bool up = GATED && q >= COLS;
+      rw[j] = row_buffer(up ? p.w1 : p.w, n0, up ? q - COLS : q, p.N, 8);
     }
+    aim_rows(0, m0);
     // the rows' scale bytes of a K block: BM of them (whole dwords: m16 and m0 are multiples of 16)
     rsc = buffer_at(p.a_scales + m0, (uint32_t)((size_t)kbs * m16 - m0));
   };
-  const uint32_t lds0 = lds_offset(lds), vsc = lane < BM / 4 ? 4u * lane : kOutside;
-  auto copy = [&](uint32_t slot) {
-    const uint32_t at = lds0 + slot * STAGE + wave * ND * 1024;
-#pragma unroll
-    for (int j = 0; j < ND; j++)
-      lds_copy16(rs[j], ckb * 128 + (int)fx[j] < climit ? rowk + fx[j] : kOutside, ckb * 128, at + 1024 * j);
-    lds_copy4(rsc, vsc, ckb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
-    ckb++;
+  auto aim2 = [&]() {
+    int tm, tn;
+    tile_place(tiles, tiles_m, tiles_n, c2.tile, tm, tn);
+    aim_rows(1, tm * BM);
   };
-  auto next_tile = [&]() {
-    ckb = 0;
-    ctile += gridDim.x;
-    if (ctile < tiles) aim();
-    else climit = 0;
+  auto advance = [&](Cursor& c, auto aim) {
+    if (++c.kb < kbs) return;
+    c.kb = 0;
+    c.tile += gridDim.x;
+    if (c.tile < tiles) aim();
+    else c.limit = 0;
+  };
+  const uint32_t fx = 16u * ((lane & 7) ^ (lane >> 3)), vw = (lane >> 3) * (uint32_t)p.K + fx;
+  const uint32_t va = (lane >> 3) * (uint32_t)(MT * p.K) + fx, vsc = lane < BM / 4 ? 4u * lane : kOutside;
+  const uint32_t lds0 = lds_offset(lds);
+  // copy j of what cursor 1 brings: the first half of the rows, the scales, the weights
+  auto copy1 = [&](int j, uint32_t slot) {
+    const bool in = c1.kb * 128 + (int)fx < c1.limit;
+    if (j < CA) lds_copy16(ra[0][j], in ? va : kOutside, c1.kb * 128, lds0 + slot * STAGE + (wave * CA + j) * 1024);
+    else if (j == CA) lds_copy4(rsc, vsc, c1.kb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
+    else lds_copy16(rw[j - CA - 1], in ? vw : kOutside, c1.kb * 128, lds0 + slot * STAGE + BM * 128 + (wave * CW + j - CA - 1) * 1024);
+  };
+  auto copy2 = [&](int j, uint32_t slot) {
+    const bool in = c2.kb * 128 + (int)fx < c2.limit;
+    lds_copy16(ra[1][j], in ? va : kOutside, c2.kb * 128, lds0 + slot * STAGE + ((NW + wave) * CA + j) * 1024);
+  };
+  // All copies but the newest 2 CA + CW + 1 (one step's) have landed, and this wave's reads are complete.
+  auto arrive = [&]() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * CA + CW + 1) : "memory");
   };
 
   // ---- weight scales: lane k holds those of K block kb + k of this wave's column block
@@ -449,7 +471,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
   // lane's chunks g and g + 4 of its row: places (g ^ f) and (g ^ f) ^ 4
   const int arow = wm * 16 * MT + r * MT, wrow = (GATED ? wn * 8 * NT : wn * 16 * NT) + r;
   const uint32_t place = 16 * (g ^ (r & 7));
-  uint32_t alo = arow * 128 + place, ahi = arow * 128 + (place ^ 64);  // in the current step's buffer
+  uint32_t alo = (wm * 16 + r) * 128 + place, ahi = (wm * 16 + r) * 128 + (place ^ 64);  // in the current step's buffer
   uint32_t wlo = (BM + wrow) * 128 + place, whi = (BM + wrow) * 128 + (place ^ 64), sat = SCALES + arow;
   auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
     const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
@@ -465,14 +487,19 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
   };
 
   int tm, tn;
-  tile_place(tiles, tiles_m, tiles_n, ctile, tm, tn);
-  aim();
-  copy(0);
+  tile_place(tiles, tiles_m, tiles_n, blockIdx.x, tm, tn);
   weight_scales(tn * COLS, 0, ws);
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-  asm volatile("s_barrier" ::: "memory");
-  if (ckb == kbs) next_tile();
-  copy(1);
+  aim1();
+  aim2();
+#pragma unroll
+  for (int j = 0; j < CA + 1 + CW; j++) copy1(j, 0);
+#pragma unroll
+  for (int j = 0; j < CA; j++) copy2(j, 0);
+  advance(c1, aim1);
+#pragma unroll
+  for (int j = 0; j < CA + 1 + CW; j++) copy1(j, 1);
+  arrive();
   read_scales();
 #pragma unroll
   for (int j = 0; j < NT; j++) read_w(j);
@@ -482,7 +509,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int m0 = tm * BM, n0 = tn * COLS;
     if (tile + gridDim.x < tiles) tile_place(tiles, tiles_m, tiles_n, tile + gridDim.x, tm, tn);
-    weight_scales(tn * COLS, 0, wsn);  // of the next tile: complete after the first step's wait
+    weight_scales(tn * COLS, 0, wsn);  // of the next tile
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -493,7 +520,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
         weight_scales(n0, kb, ws);
         __builtin_amdgcn_s_waitcnt(0x0f70);
       }
-      if (ckb == kbs) next_tile();
+      advance(c1, aim1);
+      advance(c2, aim2);
       uint32_t swb[GATED ? 2 : 1];
 #pragma unroll
       for (int j = 0; j < (GATED ? 2 : 1); j++) swb[j] = __builtin_amdgcn_readlane(ws[j], kb & 63);
@@ -505,16 +533,14 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
       for (int i = 0; i < MT; i++) {
         const uint32_t sc = sa[i / 4];
         if (i < MT - 1) {
-          read(alo + (i + 1) * 128, ahi + (i + 1) * 128, a[(i + 1) & 1]);
+          // the second half's rows of this step have landed; the first half's, and the weights, are in registers
+          if (i == H - 1) arrive();
+          read(alo + (i + 1) * WM * 2048, ahi + (i + 1) * WM * 2048, a[(i + 1) & 1]);
         } else {
-          // the next step's data has landed and this step's operands are all in registers
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          __builtin_amdgcn_s_waitcnt(0x0f70);
-          asm volatile("s_barrier" ::: "memory");
-          copy(slot);
-          slot ^= 1;
-          const uint32_t step = slot ? STAGE : -STAGE;
-          alo += step, ahi += step, wlo += step, whi += step, sat += slot ? 256 : -256;
+          // the next step's first half and weights have landed; this step's operands are all in registers
+          arrive();
+          const uint32_t step = slot ? -STAGE : STAGE;
+          alo += step, ahi += step, wlo += step, whi += step, sat += slot ? -256 : 256;
           read_scales();
           read(alo, ahi, a[0]);
         }
@@ -526,14 +552,23 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
           const uint32_t s = swb[GATED && j >= NT / 2 ? 1 : 0];
           if constexpr (EXACT) wide_product<ST>(ww[j], wa, (sc >> (8 * (i % 4))) & 255, s, __uint_as_float(s), acc[i][j]);
           else tile_product<ST>(w[j], a[i & 1], sc, i % 4, s, __uint_as_float(s), acc[i][j]);
-          if (i == MT - 1) {  // each weight operand is replaced as soon as it has been used
-            __builtin_amdgcn_sched_barrier(0);
-            read_w(j);
-            __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (i == MT - 1) read_w(j);  // each weight operand is replaced as soon as it has been used
+          // this step's share of copies, behind the products: the next step's last stripes into its buffer,
+          // then, once this step's first half is read, the step after it into this one's
+          if (i < H - 1) {
+#pragma unroll
+            for (int c = (i * NT + j) * CA / ((H - 1) * NT); c < (i * NT + j + 1) * CA / ((H - 1) * NT); c++) copy2(c, slot ^ 1);
+          } else if (i < MT - 1) {
+            constexpr int C1 = CA + 1 + CW, SLOTS = (MT - H) * NT;
+            const int at = (i - H + 1) * NT + j;
+#pragma unroll
+            for (int c = at * C1 / SLOTS; c < (at + 1) * C1 / SLOTS; c++) copy1(c, slot);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      slot ^= 1;
       kb++;
     } while (kb < kbs);
 
