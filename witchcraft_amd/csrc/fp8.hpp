@@ -77,6 +77,15 @@ __device__ __forceinline__ uint32_t e4m3_pack4(float a, float b, float c, float 
   return (uint32_t)r;
 }
 
+// The same of v / s for a power of two s: one instruction divides and rounds two values.
+typedef short s2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t e4m3_pack4_scaled(f4 v, float s) {
+  s2v r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, v[0], v[1], s, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, v[2], v[3], s, true);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
 // v combined over the 16 lanes of a DPP row; every lane gets the same bits (each rotation step joins
 // two halves that both lanes see).
 template <int N>

@@ -81,29 +81,37 @@ __device__ __forceinline__ i8v load_row(const uint8_t* row, int kb, int g, int K
   return i8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
+// Four values as f16 or bf16.
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+template <int OUT>
+__device__ __forceinline__ u2v half4(f4 v) {
+  if constexpr (OUT == FP8_IO_F16) return __builtin_bit_cast(u2v, __builtin_convertvector(v, h4));
+  else return __builtin_bit_cast(u2v, __builtin_convertvector(v, b4));
+}
+
 // Four consecutive columns n .. n + 3 of row m of the product.
+template <int OUT>
 __device__ __forceinline__ void store_out(const Fp8GemmArgs& p, int m, int n, f4 v) {
   if (m >= p.M || n >= p.N) return;
   const size_t at = (size_t)m * p.N + n;
   if ((p.N & 3) == 0) {  // whole quads, aligned
-    if (p.out_type == FP8_IO_F32) *reinterpret_cast<f4*>((float*)p.out + at) = v;
-    else if (p.out_type == FP8_IO_F16) *reinterpret_cast<h4*>((_Float16*)p.out + at) = __builtin_convertvector(v, h4);
-    else *reinterpret_cast<b4*>((__bf16*)p.out + at) = __builtin_convertvector(v, b4);
+    if constexpr (OUT == FP8_IO_F32) *reinterpret_cast<f4*>((float*)p.out + at) = v;
+    else *reinterpret_cast<u2v*>((uint16_t*)p.out + at) = half4<OUT>(v);
     return;
   }
+  const u2v h = half4<OUT>(v);
 #pragma unroll
   for (int e = 0; e < 4; e++)
     if (n + e < p.N) {
-      if (p.out_type == FP8_IO_F32) ((float*)p.out)[at + e] = v[e];
-      else if (p.out_type == FP8_IO_F16) ((_Float16*)p.out)[at + e] = (_Float16)v[e];
-      else ((__bf16*)p.out)[at + e] = (__bf16)v[e];
+      if constexpr (OUT == FP8_IO_F32) ((float*)p.out)[at + e] = v[e];
+      else ((uint16_t*)p.out)[at + e] = (uint16_t)(h[e / 2] >> (16 * (e % 2)));
     }
 }
 
 // ---- few rows: 16 MB rows x 16 NB columns per workgroup, its waves on the K blocks in turn ---
 // Each operand goes from memory straight to the wave that multiplies it; the waves' partial sums
 // meet in LDS and are added in wave order.
-template <bool EXACT, int ST, int MB, int NB, int KS>
+template <int OUT, int ST, int MB, int NB, int KS>
 __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int tiles_n, int64_t tiles) {
   __shared__ f4 red[KS][MB * NB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -144,7 +152,7 @@ __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int t
 #pragma unroll
       for (int i = 0; i < MB; i++)
 #pragma unroll
-        for (int j = 0; j < NB; j++) block_product<EXACT, ST>(w[j], a[i], as[i], wb[j], wf[j], acc[i][j]);
+        for (int j = 0; j < NB; j++) block_product<OUT == FP8_IO_F32, ST>(w[j], a[i], as[i], wb[j], wf[j], acc[i][j]);
     }
 #pragma unroll
     for (int i = 0; i < MB; i++)
@@ -155,7 +163,7 @@ __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int t
       f4 v = red[0][t][lane];
 #pragma unroll
       for (int k = 1; k < KS; k++) v += red[k][t][lane];
-      store_out(p, m0 + 16 * (t / NB) + r, n0 + 16 * (t % NB) + 4 * g, v);
+      store_out<OUT>(p, m0 + 16 * (t / NB) + r, n0 + 16 * (t % NB) + 4 * g, v);
     }
     __syncthreads();  // red is written again for the next tile
   }
@@ -262,7 +270,7 @@ __global__ __launch_bounds__(512 * KS) void fp8_small_gated_kernel(Fp8GemmArgs p
 //  * A wave's activation rows are dealt out as row = MT (l % 16) + i for tile i, so that a lane's
 //    scale bytes of one K block are MT consecutive ones: a dword holds four tiles' scales, and the
 //    instruction picks its byte.
-//  * Weight scales, one per K block and wave, sit in a register of the lane kb % 64.
+//  * A step's scales come the same way, the rows' as dwords, the weights' one per block of 128 columns.
 //  * Step kb + 1's data has been requested one step ahead; the wait for it, and the barrier after which
 //    step kb's buffer is refilled, come before the last row of MFMAs of step kb, whose operands are
 //    in registers by then, so the first operands of step kb + 1 are read behind those MFMAs.
@@ -288,6 +296,15 @@ __device__ __forceinline__ void lds_copy4(i4v rsrc, uint32_t voff, uint32_t soff
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                "s"(m0)
                : "memory");
+}
+// One scale per lane, a byte or a dword of memory, a dword in LDS either way.
+template <int ST>
+__device__ __forceinline__ void lds_copy_scale(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
+  if constexpr (ST == FP8_F32) lds_copy4(rsrc, voff, soff, m0);
+  else
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_ubyte %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
+                 "s"(m0)
+                 : "memory");
 }
 constexpr uint32_t kOutside = 0x7fffffffu;  // past every descriptor's range
 constexpr int kTileMaxK = 1 << 21;          // 256 rows' bytes fit a descriptor and a lane's offset
@@ -325,61 +342,121 @@ __device__ __forceinline__ void tile_place(uint32_t tiles, int tiles_m, int tile
   tn = (int)(in / h);
 }
 
-// The values of one 16-row stripe of a wave's tile (row l % 16 of each lane, columns 16 j + 4 (l / 16)),
-// stored as whole 16-byte pieces of its rows through the wave's own LDS (16 rows of 16 NT columns of a
-// 2-byte type, half of them of a 4-byte one), rotated like the operands.  mrow(i): the row of C of the
-// stripe's row i.  N that does not divide into such pieces is stored by single values.
-template <int OUT, int NT, typename Row>
-__device__ __forceinline__ void store_stripe(const Fp8GemmArgs& p, uint8_t* stage, int lane, int n0, const f4 (&v)[NT],
-                                             Row mrow) {
-  constexpr int SZ = OUT == FP8_IO_F32 ? 4 : 2, PASSES = SZ / 2, TJ = NT / PASSES, ROWB = TJ * 16 * SZ, CH = ROWB / 16;
+// A wave's MT stripes of 16 rows and 16 NT columns: lane l has row MT (l % 16) + i of the wave's rows in
+// stripe i, columns 16 j + 4 (l / 16).  A stripe is laid out in the wave's LDS (16 rows of 128 bytes at a
+// time, 16-byte pieces rotated by the row) and stored in whole lines, past the caches: 64-byte pieces
+// straight from registers took 151 us instead of 114 for 74,640 x 2,048 (x 768) in bf16, whole lines
+// without the non-temporal hint 141.  Rows of C that do not keep 16-byte alignment go value by value.
+template <int OUT, int MT, int NT>
+__device__ __forceinline__ void store_stripes(const Fp8GemmArgs& p, uint8_t* stage, int lane, int m0, int n0,
+                                              const f4 (&v)[MT][NT]) {
+  constexpr int SZ = OUT == FP8_IO_F32 ? 4 : 2, TJ = 8 / SZ;  // TJ: columns / 16 of 128 bytes
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int h = 0; h < PASSES; h++) {
+  for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int j = 0; j < TJ; j++) {
-      const int b = (16 * j + 4 * g) * SZ;  // byte within the row
-      uint8_t* at = stage + r * ROWB + (((b >> 4) ^ (r & 7)) << 4) + (b & 15);
-      if constexpr (OUT == FP8_IO_F32) *reinterpret_cast<f4*>(at) = v[h * TJ + j];
-      else if constexpr (OUT == FP8_IO_F16) *reinterpret_cast<h4*>(at) = __builtin_convertvector(v[h * TJ + j], h4);
-      else *reinterpret_cast<b4*>(at) = __builtin_convertvector(v[h * TJ + j], b4);
-    }
-    const int nh = n0 + h * TJ * 16;
-    if (p.N % (16 / SZ) == 0) {
+    for (int h = 0; h < NT / TJ; h++) {
 #pragma unroll
-      for (int q = 0; q < 16 * CH / 64; q++) {
-        const int row = (q * 64 + lane) / CH, c = (q * 64 + lane) % CH, m = mrow(row), n = nh + c * (16 / SZ);
-        if (m < p.M && n < p.N)
-          *reinterpret_cast<uint4*>((uint8_t*)p.out + ((size_t)m * p.N + n) * SZ) =
-              *reinterpret_cast<const uint4*>(stage + row * ROWB + ((c ^ (row & 7)) << 4));
+      for (int j = 0; j < TJ; j++) {
+        const int b = (16 * j + 4 * g) * SZ;  // byte within the row
+        uint8_t* at = stage + r * 128 + (((b >> 4) ^ (r & 7)) << 4) + (b & 15);
+        if constexpr (SZ == 4) *reinterpret_cast<f4*>(at) = v[i][h * TJ + j];
+        else *reinterpret_cast<u2v*>(at) = half4<OUT>(v[i][h * TJ + j]);
       }
-    } else {
-      for (int q = lane; q < 16 * TJ * 16; q += 64) {
-        const int row = q / (TJ * 16), c = q % (TJ * 16), m = mrow(row), n = nh + c, b = c * SZ;
-        const uint8_t* at = stage + row * ROWB + (((b >> 4) ^ (row & 7)) << 4) + (b & 15);
-        if (m < p.M && n < p.N) {
-          if constexpr (SZ == 4) ((float*)p.out)[(size_t)m * p.N + n] = *reinterpret_cast<const float*>(at);
-          else ((uint16_t*)p.out)[(size_t)m * p.N + n] = *reinterpret_cast<const uint16_t*>(at);
+      const int nh = n0 + h * TJ * 16;
+      if (p.N % (16 / SZ) == 0) {
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          const int row = 8 * q + (lane >> 3), c = lane & 7, m = m0 + row * MT + i, n = nh + c * (16 / SZ);
+          if (m < p.M && n < p.N)
+            __builtin_nontemporal_store(*reinterpret_cast<const i4v*>(stage + row * 128 + ((c ^ (row & 7)) << 4)),
+                                        reinterpret_cast<i4v*>((uint8_t*)p.out + ((size_t)m * p.N + n) * SZ));
+        }
+      } else {
+#pragma unroll 8
+        for (int q = 0; q < 4 * TJ; q++) {
+          const int row = (q * 64 + lane) / (TJ * 16), c = lane % (TJ * 16), b = c * SZ, m = m0 + row * MT + i, n = nh + c;
+          const uint8_t* at = stage + row * 128 + (((b >> 4) ^ (row & 7)) << 4) + (b & 15);
+          if (m < p.M && n < p.N) {
+            if constexpr (SZ == 4) ((float*)p.out)[(size_t)m * p.N + n] = *reinterpret_cast<const float*>(at);
+            else ((uint16_t*)p.out)[(size_t)m * p.N + n] = *reinterpret_cast<const uint16_t*>(at);
+          }
         }
       }
     }
+}
+
+// The gated product's end: a wave has MT stripes of 16 rows, 32 gate columns and the same 32 up columns
+// (n0 + 32 wave ..) of the 128 whose scale four waves share.  The rows' maxima meet in tops [16 MT][4],
+// the codes in stage [MT][16][128], from where they are stored in whole lines.
+template <int MT>
+__device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, float* tops, uint8_t* stage, int lane, int wave, int m0,
+                                              int n0, int m16, f4 (&acc)[MT][4]) {
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+    if (n0 + wave * 32 + 16 * j >= p.N) {
+#pragma unroll
+      for (int i = 0; i < MT; i++) acc[i][j] = acc[i][j + 2] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        acc[i][j][e] = gelu_tanh_dev(acc[i][j][e]) * acc[i][j + 2][e];
+        top = fmaxf(top, fabsf(acc[i][j][e]));
+      }
+    if (top == INFINITY) {  // taken again over the finite values (fmaxf has left NaN out)
+      top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, finite_abs(acc[i][j][e]));
+    }
+    top = max_xor32(max_xor16(top));
+    if (g == 0) tops[(16 * i + r) * 4 + wave] = top;
   }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  uint8_t* scales = p.out_scales + (size_t)(n0 / FP8_BLOCK) * m16 + m0 + r * MT;
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    const f4 t4 = *reinterpret_cast<const f4*>(tops + (16 * i + r) * 4);
+    const uint32_t byte = e8m0_of(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+    const float s = __uint_as_float(byte << 23);
+#pragma unroll
+    for (int j = 0; j < 2; j++)  // 16-byte piece 2 wave + j of the row
+      *reinterpret_cast<uint32_t*>(stage + (16 * i + r) * 128 + 16 * ((2 * wave + j) ^ (r & 7)) + 4 * g) =
+          e4m3_pack4_scaled(acc[i][j], s);
+    if (wave == 0 && g == 0 && m0 + r * MT + i < p.M) scales[i] = (uint8_t)byte;
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  const int c = lane & 7, n = n0 + 16 * c;
+#pragma unroll
+  for (int q = 0; q < MT / 2; q++) {
+    const int i = 2 * q + wave / 2, rr = 8 * (wave & 1) + (lane >> 3), m = m0 + rr * MT + i;
+    if (m < p.M && n < p.N)  // N % 16 == 0: whole pieces
+      __builtin_nontemporal_store(*reinterpret_cast<const i4v*>(stage + (16 * i + rr) * 128 + 16 * (c ^ (rr & 7))),
+                                  reinterpret_cast<i4v*>((uint8_t*)p.out + (size_t)m * p.N + n));
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // stage is copied into again
 }
 
 // OUT: the result's type; F32 results take the f16 matrix instructions (see the top of the file).
-// GATED: BN / 2 = 128 columns of both matrices, the result is codes.
-template <int OUT, int ST, bool GATED, int BM, int BN, int WM, int WN, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
-  constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
+template <int OUT, int ST, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+  constexpr bool EXACT = OUT == FP8_IO_F32;
+  constexpr int WSZ = ST == FP8_F32 ? 4 : 1;  // bytes of a weight scale
   constexpr int NW = WM * WN, MT = BM / 16 / WM, NT = BN / 16 / WN, STAGE = (BM + BN) * 128;
   constexpr int H = MT / 2;                                      // stripes of a half step
   constexpr int CA = BM / 16 / NW, CW = BN / 8 / NW;             // copies per wave: of each half of the rows, of weights
-  constexpr int COLS = GATED ? BN / 2 : BN, SCALES = 2 * STAGE, TOPS = SCALES + 512;
-  constexpr int OUTS = TOPS + (GATED ? WN * BM * 4 : 0), GI = 4;  // GI: stripes whose codes are staged at once
-  constexpr int LDS = OUTS + (GATED ? WM * 16 * GI * 128 : NW * 16 * 16 * NT * 2);
+  constexpr int C1 = CA + 2 + CW;                                // with the scales': of cursor 1 together
+  constexpr int SC = 512, SCALES = 2 * STAGE, REST = SCALES + 2 * SC;  // SC: a step's scales, rows' and weights'
+  constexpr int LDS = REST + NW * 2048;
   static_assert(BM % (16 * NW) == 0 && BN % (8 * NW) == 0 && MT % 4 == 0 && BM <= 256, "whole copies, whole scale dwords");
-  static_assert(!GATED || COLS == FP8_BLOCK, "a workgroup has all columns of a scale");
-  static_assert(GATED || 16 * NT <= FP8_BLOCK, "one weight scale per wave and K block");
+  static_assert(BN <= FP8_BLOCK && FP8_BLOCK % BN == 0, "one weight scale per tile and K block");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
@@ -395,7 +472,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
     int kb, limit;  // limit: K, or 0 past the last tile (zeros)
   };
   Cursor c1 = {blockIdx.x, 0, p.K}, c2 = c1;  // of weights and the first stripes, of the last stripes
-  i4v rw[CW], ra[2][CA], rsc;
+  i4v rw[CW], ra[2][CA], rsa, rsw;
   auto row_buffer = [&](const uint8_t* base, int first, int row, int end, int rows) {
     if (first + row >= end) row = 0;
     return buffer_at(base + (size_t)(first + row) * p.K, (uint32_t)min(rows, end - first - row) * (uint32_t)p.K);
@@ -410,16 +487,15 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
   auto aim1 = [&]() {
     int tm, tn;
     tile_place(tiles, tiles_m, tiles_n, c1.tile, tm, tn);
-    const int m0 = tm * BM, n0 = tn * COLS;
+    const int m0 = tm * BM, n0 = tn * BN;
 #pragma unroll
     for (int j = 0; j < CW; j++) {
-      const int q = 8 * (wave * CW + j);
-      const bool up = GATED && q >= COLS;
-      rw[j] = row_buffer(up ? p.w1 : p.w, n0, up ? q - COLS : q, p.N, 8);
+      rw[j] = row_buffer(p.w, n0, 8 * (wave * CW + j), p.N, 8);
     }
     aim_rows(0, m0);
     // the rows' scale bytes of a K block: BM of them (whole dwords: m16 and m0 are multiples of 16)
-    rsc = buffer_at(p.a_scales + m0, (uint32_t)((size_t)kbs * m16 - m0));
+    rsa = buffer_at(p.a_scales + m0, (uint32_t)((size_t)kbs * m16 - m0));
+    rsw = buffer_at((const uint8_t*)p.w_scales + (size_t)(n0 / FP8_BLOCK) * kbs * WSZ, (uint32_t)(kbs * WSZ));
   };
   auto aim2 = [&]() {
     int tm, tn;
@@ -435,70 +511,54 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
   };
   const uint32_t fx = 16u * ((lane & 7) ^ (lane >> 3)), vw = (lane >> 3) * (uint32_t)p.K + fx;
   const uint32_t va = (lane >> 3) * (uint32_t)(MT * p.K) + fx, vsc = lane < BM / 4 ? 4u * lane : kOutside;
+  const uint32_t vws = lane == 0 ? 0 : kOutside;
   const uint32_t lds0 = lds_offset(lds);
   // copy j of what cursor 1 brings: the first half of the rows, the scales, the weights
   auto copy1 = [&](int j, uint32_t slot) {
     const bool in = c1.kb * 128 + (int)fx < c1.limit;
     if (j < CA) lds_copy16(ra[0][j], in ? va : kOutside, c1.kb * 128, lds0 + slot * STAGE + (wave * CA + j) * 1024);
-    else if (j == CA) lds_copy4(rsc, vsc, c1.kb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
-    else lds_copy16(rw[j - CA - 1], in ? vw : kOutside, c1.kb * 128, lds0 + slot * STAGE + BM * 128 + (wave * CW + j - CA - 1) * 1024);
+    else if (j == CA) lds_copy4(rsa, vsc, c1.kb * (uint32_t)m16, lds0 + SCALES + SC * slot);  // the same by every wave
+    else if (j == CA + 1) lds_copy_scale<ST>(rsw, vws, c1.kb * WSZ, lds0 + SCALES + SC * slot + 256);
+    else lds_copy16(rw[j - CA - 2], in ? vw : kOutside, c1.kb * 128, lds0 + slot * STAGE + BM * 128 + (wave * CW + j - CA - 2) * 1024);
   };
   auto copy2 = [&](int j, uint32_t slot) {
     const bool in = c2.kb * 128 + (int)fx < c2.limit;
     lds_copy16(ra[1][j], in ? va : kOutside, c2.kb * 128, lds0 + slot * STAGE + ((NW + wave) * CA + j) * 1024);
   };
-  // All copies but the newest 2 CA + CW + 1 (one step's) have landed, and this wave's reads are complete.
-  auto arrive = [&]() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * CA + CW + 1) : "memory");
-  };
-
-  // ---- weight scales: lane k holds those of K block kb + k of this wave's column block
-  uint32_t ws[GATED ? 2 : 1], wsn[GATED ? 2 : 1];
-  auto weight_scales = [&](int n0, int kb, uint32_t (&to)[GATED ? 2 : 1]) {
-    const int nb = min(n0 + (GATED ? 0 : wn * 16 * NT), p.N - 1) / FP8_BLOCK;
-    const size_t at = (size_t)nb * kbs + min(kb + lane, kbs - 1);
-#pragma unroll
-    for (int j = 0; j < (GATED ? 2 : 1); j++) {
-      const void* s = j ? p.w1_scales : p.w_scales;
-      to[j] = ST == FP8_E8M0 ? ((const uint8_t*)s)[at] : __float_as_uint(((const float*)s)[at]);
-    }
-  };
+  // All copies but the newest CA + C1 (one step's) have landed, and this wave's reads are complete.
+  auto arrive = [&]() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(CA + C1) : "memory"); };
 
   f4 acc[MT][NT];
   i8v a[2], w[NT];
   Wide ww[EXACT ? NT : 1];
-  uint32_t sa[MT / 4];
+  uint32_t sa[MT / 4], sw;  // scales: of the rows' stripes, of the weights
   // lane's chunks g and g + 4 of its row: places (g ^ f) and (g ^ f) ^ 4
-  const int arow = wm * 16 * MT + r * MT, wrow = (GATED ? wn * 8 * NT : wn * 16 * NT) + r;
+  const int arow = wm * 16 * MT + r * MT, wrow = wn * 16 * NT + r;
   const uint32_t place = 16 * (g ^ (r & 7));
   uint32_t alo = (wm * 16 + r) * 128 + place, ahi = (wm * 16 + r) * 128 + (place ^ 64);  // in the current step's buffer
-  uint32_t wlo = (BM + wrow) * 128 + place, whi = (BM + wrow) * 128 + (place ^ 64), sat = SCALES + arow;
+  uint32_t wlo = (BM + wrow) * 128 + place, whi = (BM + wrow) * 128 + (place ^ 64), sat = SCALES + arow, swat = SCALES + 256;
   auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
     const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
     v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   };
-  auto read_w = [&](int j) {
-    const int o = (GATED ? (j < NT / 2 ? 16 * j : COLS + 16 * (j - NT / 2)) : 16 * j) * 128;
-    read(wlo + o, whi + o, w[j]);
-  };
+  auto read_w = [&](int j) { read(wlo + 2048 * j, whi + 2048 * j, w[j]); };
   auto read_scales = [&]() {
 #pragma unroll
     for (int c = 0; c < MT / 4; c++) sa[c] = *reinterpret_cast<const uint32_t*>(lds + sat + 4 * c);
+    sw = *reinterpret_cast<const uint32_t*>(lds + swat);
   };
 
   int tm, tn;
   tile_place(tiles, tiles_m, tiles_n, blockIdx.x, tm, tn);
-  weight_scales(tn * COLS, 0, ws);
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   aim1();
   aim2();
 #pragma unroll
-  for (int j = 0; j < CA + 1 + CW; j++) copy1(j, 0);
+  for (int j = 0; j < C1; j++) copy1(j, 0);
 #pragma unroll
   for (int j = 0; j < CA; j++) copy2(j, 0);
   advance(c1, aim1);
 #pragma unroll
-  for (int j = 0; j < CA + 1 + CW; j++) copy1(j, 1);
+  for (int j = 0; j < C1; j++) copy1(j, 1);
   arrive();
   read_scales();
 #pragma unroll
@@ -507,24 +567,17 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
   uint32_t slot = 0;
 
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int m0 = tm * BM, n0 = tn * COLS;
+    const int m0 = tm * BM, n0 = tn * BN;
     if (tile + gridDim.x < tiles) tile_place(tiles, tiles_m, tiles_n, tile + gridDim.x, tm, tn);
-    weight_scales(tn * COLS, 0, wsn);  // of the next tile
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
       for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
     int kb = 0;
     do {
-      if (kb && (kb & 63) == 0) {
-        weight_scales(n0, kb, ws);
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-      }
       advance(c1, aim1);
       advance(c2, aim2);
-      uint32_t swb[GATED ? 2 : 1];
-#pragma unroll
-      for (int j = 0; j < (GATED ? 2 : 1); j++) swb[j] = __builtin_amdgcn_readlane(ws[j], kb & 63);
+      const uint32_t s = sw;
       if constexpr (EXACT) {
 #pragma unroll
         for (int j = 0; j < NT; j++) ww[j] = widen(w[j]);
@@ -540,7 +593,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
           // the next step's first half and weights have landed; this step's operands are all in registers
           arrive();
           const uint32_t step = slot ? -STAGE : STAGE;
-          alo += step, ahi += step, wlo += step, whi += step, sat += slot ? -256 : 256;
+          alo += step, ahi += step, wlo += step, whi += step, sat += slot ? -SC : SC, swat += slot ? -SC : SC;
           read_scales();
           read(alo, ahi, a[0]);
         }
@@ -549,7 +602,6 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
         if constexpr (EXACT) wa = widen(a[i & 1]);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          const uint32_t s = swb[GATED && j >= NT / 2 ? 1 : 0];
           if constexpr (EXACT) wide_product<ST>(ww[j], wa, (sc >> (8 * (i % 4))) & 255, s, __uint_as_float(s), acc[i][j]);
           else tile_product<ST>(w[j], a[i & 1], sc, i % 4, s, __uint_as_float(s), acc[i][j]);
           __builtin_amdgcn_sched_barrier(0);
@@ -560,7 +612,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
 #pragma unroll
             for (int c = (i * NT + j) * CA / ((H - 1) * NT); c < (i * NT + j + 1) * CA / ((H - 1) * NT); c++) copy2(c, slot ^ 1);
           } else if (i < MT - 1) {
-            constexpr int C1 = CA + 1 + CW, SLOTS = (MT - H) * NT;
+            constexpr int SLOTS = (MT - H) * NT;
             const int at = (i - H + 1) * NT + j;
 #pragma unroll
             for (int c = at * C1 / SLOTS; c < (at + 1) * C1 / SLOTS; c++) copy1(c, slot);
@@ -572,76 +624,196 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8GemmArgs
       kb++;
     } while (kb < kbs);
 
-    if constexpr (!GATED) {
-      uint8_t* stage = lds + OUTS + wave * (16 * 16 * NT * 2);
+    store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0 + wm * 16 * MT, n0 + wn * NT * 16, acc);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
+}
+
+// ---- strips: 16 MT rows x 64 NW weight rows per workgroup, two workgroups per compute unit ----------
+// Wave w has all rows and 64 weight rows of its own (gated: 32 gate rows and the 32 up rows of the same
+// columns).  Rows' codes are double-buffered in LDS; the weights have one buffer, a wave's own share:
+// their operands are in registers from a step's start, when the next step's are requested.  The two
+// workgroups run apart, so that one's results are formed and stored behind the other's products.
+template <int OUT, int ST, bool GATED, int MT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+  constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
+  constexpr int NT = 4, BM = 16 * MT, STAGE = BM * 128, NM = GATED ? 2 : 1;  // NM: matrices
+  constexpr int COLS = (GATED ? 32 : 64) * NW, CA = BM / 8 / NW;              // CA: copies of rows per wave and K block
+  constexpr int WEIGHTS = 2 * STAGE, SCALES = WEIGHTS + NW * 8192, REST = SCALES + 512;
+  constexpr int LDS = REST + (GATED ? NW * BM * 4 : NW * 2048);
+  static_assert(BM % (8 * NW) == 0 && MT % 4 == 0 && (!GATED || NW == 4), "whole copies; all columns of a scale");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK, m16 = (int)fp8_scale_rows(p.M);
+  const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
+
+  // ---- copies of the next step: K block ckb of tile ctile.  One brings 8 rows, lane l chunk (l % 8) ^ (l / 8)
+  // of its row l / 8 to place l % 8.  In LDS the activations are ordered by stripe, [MT][16]; consecutive
+  // ones lie MT apart in memory.  Descriptors end with the matrix; one whose rows are all past it has
+  // the tile's first rows, which nothing uses.
+  uint32_t ctile = blockIdx.x;
+  int ckb = 0, climit = p.K;  // climit 0: past the last tile, zeros
+  int tm, tn;                 // place of tile ctile
+  i4v ra[CA], rsa, rw[NM];
+  uint32_t ws[NM], wsn[NM];   // weight scales: lane k's are of K block k of a stretch of 64
+  auto weight_scales = [&](int n0, int kb, uint32_t (&to)[NM]) {
+    const size_t at = (size_t)(min(n0 + wave * (COLS / NW), p.N - 1) / FP8_BLOCK) * kbs + min(kb + lane, kbs - 1);
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
-        const int row0 = m0 + wm * 16 * MT + i;
-        store_stripe<OUT, NT>(p, stage, lane, n0 + wn * NT * 16, acc[i], [&](int q) { return row0 + q * MT; });
-      }
-    } else {
-      // rows' maxima over the 128 columns, from WN waves; then the codes through LDS, in whole rows
-      float* tops = reinterpret_cast<float*>(lds + TOPS);  // [WN][BM]
-      uint8_t* stage = lds + OUTS;                         // [GI][WM * 16][128], 16-byte chunks rotated
-#pragma unroll
-      for (int i = 0; i < MT; i++) {
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < NT / 2; j++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float y = gelu_tanh_dev(acc[i][j][e]) * acc[i][j + NT / 2][e];
-            acc[i][j][e] = y;
-            if (n0 + (wn * NT / 2 + j) * 16 < p.N) top = fmaxf(top, finite_abs(y));
-          }
-        top = max_xor32(max_xor16(top));
-        if (g == 0) tops[wn * BM + arow + i] = top;
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-      for (int i0 = 0; i0 < MT; i0 += GI) {
-#pragma unroll
-        for (int i = i0; i < i0 + GI; i++) {
-          const int row = arow + i;
-          float top = tops[row];
-#pragma unroll
-          for (int c = 1; c < WN; c++) top = fmaxf(top, tops[c * BM + row]);
-          const uint32_t byte = e8m0_of(top);
-          const float inv = e8m0_inverse(byte);
-#pragma unroll
-          for (int j = 0; j < NT / 2; j++) {
-            const int c = wn * NT / 2 + j;  // 16-byte chunk of the row
-            *reinterpret_cast<uint32_t*>(stage + ((i - i0) * WM * 16 + wm * 16 + r) * 128 + 16 * (c ^ (r & 7)) + 4 * g) =
-                e4m3_pack4(acc[i][j][0] * inv, acc[i][j][1] * inv, acc[i][j][2] * inv, acc[i][j][3] * inv);
-          }
-          if (wn == 0 && g == 0 && m0 + row < p.M) p.out_scales[(size_t)(n0 / FP8_BLOCK) * m16 + m0 + row] = (uint8_t)byte;
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-        for (int q = 0; q < GI * WM * 16 * 8 / (64 * NW); q++) {
-          const int at = (q * 64 * NW + tid) >> 3, c = tid & 7, i = at / (WM * 16), rr = at % 16;
-          const int m = m0 + ((at / 16) % WM) * 16 * MT + rr * MT + i0 + i;
-          if (m < p.M && n0 + 16 * c < p.N)
-            *reinterpret_cast<uint4*>((uint8_t*)p.out + (size_t)m * p.N + n0 + 16 * c) =
-                *reinterpret_cast<const uint4*>(stage + at * 128 + 16 * (c ^ (rr & 7)));
-        }
-        // the stage is written again
-        if (i0 + GI < MT) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      }
+    for (int j = 0; j < NM; j++) {
+      const void* s = j ? p.w1_scales : p.w_scales;
+      to[j] = ST == FP8_E8M0 ? ((const uint8_t*)s)[at] : __float_as_uint(((const float*)s)[at]);
     }
+  };
+  auto aim = [&]() {
+    tile_place(tiles, tiles_m, tiles_n, ctile, tm, tn);
+    const int m0 = tm * BM, n = tn * COLS + wave * (COLS / NW);
 #pragma unroll
-    for (int j = 0; j < (GATED ? 2 : 1); j++) ws[j] = wsn[j];
+    for (int j = 0; j < CA; j++) {
+      const int q = wave * CA + j;
+      int row = (q & 1) * 8 * MT + q / 2;
+      if (m0 + row >= p.M) row = 0;
+      ra[j] = buffer_at(p.a + (size_t)(m0 + row) * p.K, (uint32_t)min(7 * MT + 1, p.M - m0 - row) * (uint32_t)p.K);
+    }
+    rsa = buffer_at(p.a_scales + m0, (uint32_t)((size_t)kbs * m16 - m0));
+#pragma unroll
+    for (int j = 0; j < NM; j++)
+      rw[j] = buffer_at((j ? p.w1 : p.w) + (size_t)min(n, p.N - 1) * p.K, (uint32_t)max(1, min(COLS / NW, p.N - n)) * (uint32_t)p.K);
+  };
+  const uint32_t fx = 16u * ((lane & 7) ^ (lane >> 3)), va = (lane >> 3) * (uint32_t)(MT * p.K) + fx;
+  const uint32_t vsa = lane < BM / 4 ? 4u * lane : kOutside, vw = (lane >> 3) * (uint32_t)p.K + fx;
+  const uint32_t lds0 = lds_offset(lds);
+  uint32_t cva, cvw;  // this step's lane offsets; chunks past K lie outside
+  auto copy = [&](int j, uint32_t slot) {
+    if (j < 8)
+      lds_copy16(rw[GATED ? j / 4 : 0], cvw, ckb * 128u + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K,
+                 lds0 + WEIGHTS + wave * 8192 + j * 1024);
+    else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, ckb * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
+    else lds_copy4(rsa, vsa, ckb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
+  };
+  auto lane_offsets = [&]() {
+    const bool in = ckb * 128 + (int)fx < climit;
+    cva = in ? va : kOutside;
+    cvw = in ? vw : kOutside;
+  };
+
+  f4 acc[MT][NT];
+  i8v a[2], w[NT];
+  Wide ww[EXACT ? NT : 1];
+  uint32_t sa[MT / 4];
+  // lane's chunks g and g + 4 of its row
+  const uint32_t place = 16 * (g ^ (r & 7));
+  uint32_t alo = r * 128 + place, ahi = r * 128 + (place ^ 64), sat = SCALES + r * MT;  // in the current step's buffer
+  auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
+    const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
+    v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  };
+  const uint32_t wat = WEIGHTS + wave * 8192 + r * 128;
+  auto read_w = [&](int j) { read(wat + place + 2048 * j, wat + (place ^ 64) + 2048 * j, w[j]); };
+  auto read_scales = [&]() {
+#pragma unroll
+    for (int c = 0; c < MT / 4; c++) sa[c] = *reinterpret_cast<const uint32_t*>(lds + sat + 4 * c);
+  };
+
+  aim();
+  lane_offsets();
+#pragma unroll
+  for (int j = 0; j < 9 + CA; j++) copy(j, 0);
+  weight_scales(tn * COLS, 0, ws);
+  // through the builtin, so that the compiler knows its own loads to be complete
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  asm volatile("s_barrier" ::: "memory");
+  read_scales();
+#pragma unroll
+  for (int j = 0; j < NT; j++) read_w(j);
+  read(alo, ahi, a[0]);
+  uint32_t slot = 0;
+
+  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int m0 = tm * BM, n0 = tn * COLS;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+    int kb = 0;
+    do {
+      if (kb && (kb & 63) == 0) {
+        weight_scales(n0, kb, ws);
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+      }
+      if (++ckb == kbs) {  // the next step begins the next tile
+        ckb = 0;
+        ctile += gridDim.x;
+        if (ctile < tiles) aim();
+        else climit = 0;
+        weight_scales(tn * COLS, 0, wsn);
+      }
+      lane_offsets();
+      uint32_t swb[NM];
+#pragma unroll
+      for (int j = 0; j < NM; j++) swb[j] = __builtin_amdgcn_readlane(ws[j], kb & 63);
+      if constexpr (EXACT) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) ww[j] = widen(w[j]);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        const uint32_t sc = sa[i / 4];
+        if (i < MT - 1) {
+          read(alo + (i + 1) * 2048, ahi + (i + 1) * 2048, a[(i + 1) & 1]);
+        } else {
+          // all copies have landed; every wave has the next step's rows in LDS, and this step's in registers
+          __builtin_amdgcn_s_waitcnt(0x0070);
+          asm volatile("s_barrier" ::: "memory");
+          const uint32_t step = slot ? -STAGE : STAGE;
+          alo += step, ahi += step, sat += slot ? -256 : 256;
+          read_scales();
+          read(alo, ahi, a[0]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        Wide wa;
+        if constexpr (EXACT) wa = widen(a[i & 1]);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const uint32_t s = swb[GATED ? j / 2 : 0];
+          if constexpr (EXACT) wide_product<ST>(ww[j], wa, (sc >> (8 * (i % 4))) & 255, s, __uint_as_float(s), acc[i][j]);
+          else tile_product<ST>(w[j], a[i & 1], sc, i % 4, s, __uint_as_float(s), acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (i == MT - 1) read_w(j);  // each weight operand is replaced as soon as it has been used
+          // Behind the products: the next step's weights, whose buffer has been read, and rows.
+          constexpr int OPS = 9 + CA, SLOTS = (MT - 2) * NT;
+          const int at = i * NT + j;
+          if (at == 0) __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): w is in registers
+          if (at < SLOTS) {
+#pragma unroll
+            for (int c = at * OPS / SLOTS; c < (at + 1) * OPS / SLOTS; c++) copy(c, slot ^ 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      slot ^= 1;
+      kb++;
+    } while (kb < kbs);
+#pragma unroll
+    for (int j = 0; j < NM; j++) ws[j] = wsn[j];
+
+    if constexpr (!GATED) {
+      store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, acc);
+    } else {
+      // staged in the rows' buffer that the next step's copies go to
+      gated_stripes<MT>(p, reinterpret_cast<float*>(lds + REST), lds + (slot ^ 1) * STAGE, lane, wave, m0, n0, m16, acc);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
 }
 
 constexpr int64_t kMostGroups = 1 << 20;  // workgroups of a launch; the kernels walk what is left
 
-template <bool EXACT, int ST, int MB, int NB, int KS>
+template <int OUT, int ST, int MB, int NB, int KS>
 hipError_t launch_small(const Fp8GemmArgs& p, hipStream_t s) {
   const int tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
   const int64_t tiles = (int64_t)((p.M + 16 * MB - 1) / (16 * MB)) * tiles_n;
-  T5K_LAUNCH((fp8_small_kernel<EXACT, ST, MB, NB, KS>), dim3((unsigned)std::min(tiles, kMostGroups)), dim3(64 * KS), 0,
+  T5K_LAUNCH((fp8_small_kernel<OUT, ST, MB, NB, KS>), dim3((unsigned)std::min(tiles, kMostGroups)), dim3(64 * KS), 0,
              s, p, tiles_n, tiles);
   return hipGetLastError();
 }
@@ -655,15 +827,24 @@ hipError_t launch_small_gated(const Fp8GemmArgs& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int OUT, int ST, bool GATED, int BM, int BN, int WM, int WN, int OCC>
+template <int OUT, int ST, int BM, int BN, int WM, int WN>
 hipError_t launch_tile(const Fp8GemmArgs& p, int cus, hipStream_t s) {
-  constexpr int COLS = GATED ? BN / 2 : BN;
-  const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + COLS - 1) / COLS;
+  const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
-  constexpr int per = OCC * 4 / (WM * WN) > 0 ? OCC * 4 / (WM * WN) : 1;  // workgroups per compute unit
   if (p.K > kTileMaxK || tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_tile_kernel<OUT, ST, GATED, BM, BN, WM, WN, OCC>), dim3((unsigned)std::min<int64_t>(tiles, cus * per)),
+  T5K_LAUNCH((fp8_tile_kernel<OUT, ST, BM, BN, WM, WN>), dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / (WM * WN)))),
              dim3(64 * WM * WN), 0, s, p, tiles_m, tiles_n);
+  return hipGetLastError();
+}
+
+template <int OUT, int ST, bool GATED, int MT, int NW>
+hipError_t launch_strip(const Fp8GemmArgs& p, int cus, hipStream_t s) {
+  constexpr int COLS = (GATED ? 32 : 64) * NW;
+  const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + COLS - 1) / COLS;
+  const int64_t tiles = (int64_t)tiles_m * tiles_n;
+  if (p.K > kTileMaxK || tiles >> 30) return hipErrorInvalidValue;
+  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW>), dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / NW))), dim3(64 * NW), 0,
+             s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
@@ -680,20 +861,18 @@ int compute_units() {
 
 template <int OUT, int ST>
 hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
-  if (p.M <= 64 || p.K > kTileMaxK) return launch_small<OUT == FP8_IO_F32, ST, 2, 2, 4>(p, s);
+  if (p.M <= 64 || p.K > kTileMaxK) return launch_small<OUT, ST, 2, 2, 4>(p, s);
   const int cus = compute_units();
   if constexpr (OUT != FP8_IO_F32) {
-    if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= cus) return launch_tile<OUT, ST, false, 256, 256, 2, 4, 2>(p, cus, s);
+    if ((int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256) >= cus) return launch_strip<OUT, ST, false, 8, 4>(p, cus, s);
   }
-  return launch_tile<OUT, ST, false, 128, 128, 2, 2, 2>(p, cus, s);
+  return launch_tile<OUT, ST, 128, 128, 2, 2>(p, cus, s);
 }
 
 template <int ST>
 hipError_t launch_gated(const Fp8GemmArgs& p, hipStream_t s) {
   if (p.M <= 64 || p.K > kTileMaxK) return launch_small_gated<ST, 2, 1>(p, s);
-  const int cus = compute_units();
-  if ((int64_t)((p.M + 255) / 256) * ((p.N + 127) / 128) >= 2 * cus) return launch_tile<FP8_IO_NONE, ST, true, 256, 256, 2, 4, 2>(p, cus, s);
-  return launch_tile<FP8_IO_NONE, ST, true, 128, 256, 2, 4, 2>(p, cus, s);
+  return launch_strip<FP8_IO_NONE, ST, true, 8, 4>(p, compute_units(), s);
 }
 }  // namespace
 
