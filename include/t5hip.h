@@ -277,8 +277,8 @@ int t5h_embeddings_from_packed(int32_t hip_device, const uint8_t* buf, const siz
  * max(max|x| / 448, 2^-126) in f32; codes are e4m3(x / s), nearest with ties to even (for f32
  * scales e4m3(x r), r = 448 / max|x| rounded to f32).  Values that are not finite get a NaN code
  * and do not count towards the maximum.
- * Row lengths K, D (and N of the gated product) are multiples of 16; any M, N >= 0 (0: nothing to
- * do).  Rows are contiguous.  Buffers of the device forms start on 16 bytes (weight scales on their
+ * Row lengths K, D are multiples of 16 up to 2^21, N of the gated product is a multiple of 16; any M,
+ * N >= 0 up to 2^30 (0: nothing to do).  Rows are contiguous.  Buffers of the device forms start on 16 bytes (weight scales on their
  * own size), lie on the current device, and do not overlap outputs except where said; calls are
  * enqueued on `stream` (a hipStream_t; NULL = the default stream) and return without waiting.  They
  * allocate nothing and keep no state, so they may be captured into a graph and run concurrently.

@@ -27,7 +27,7 @@ static_assert(T5H_TYPE_F32 == t5k::FP8_IO_F32 && T5H_TYPE_F16 == t5k::FP8_IO_F16
               "the kernels take the ABI's type codes");
 static_assert(T5H_SCALE_E8M0 == t5k::FP8_E8M0 && T5H_SCALE_F32 == t5k::FP8_F32, "and its scale types");
 
-constexpr int32_t kMostDim = 1 << 30;
+constexpr int32_t kMostRows = 1 << 30;
 
 size_t type_bytes(int32_t t) { return t == T5H_TYPE_F32 ? 4 : 2; }
 bool known_type(int32_t t) { return t == T5H_TYPE_F32 || t == T5H_TYPE_F16 || t == T5H_TYPE_BF16; }
@@ -42,8 +42,8 @@ int bad(const char* what) { return fail(T5H_ERR_INVALID, std::string("fp8: ") + 
 
 // Rows and the summed length of a call; the kernels index blocks of 128 in 31 bits.
 int check_shape(int32_t rows, int32_t K) {
-  if (rows < 0 || rows > kMostDim) return bad("rows must lie in 0 .. 2^30");
-  if (K < 16 || K % 16 || K > kMostDim) return bad("row length must be a multiple of 16 in 16 .. 2^30");
+  if (rows < 0 || rows > kMostRows) return bad("rows must lie in 0 .. 2^30");
+  if (K < 16 || K % 16 || K > t5k::FP8_MAX_K) return bad("row length must be a multiple of 16 in 16 .. 2^21");
   if (((uint64_t)rows * blocks_of(K)) >> 31) return bad("2^31 blocks or more");
   return T5H_OK;
 }

@@ -18,6 +18,8 @@ namespace t5k {
 enum Fp8Type : int { FP8_IO_F32 = 0, FP8_IO_F16 = 1, FP8_IO_BF16 = 2, FP8_IO_NONE = 3 };
 enum Fp8Scale : int { FP8_E8M0 = 0, FP8_F32 = 1 };
 constexpr int FP8_BLOCK = 128;
+// Longest row: 64 weight rows, or 8 activation rows 8 apart, fit a buffer descriptor's 31-bit offsets.
+constexpr int FP8_MAX_K = 1 << 21;
 __host__ __device__ __forceinline__ size_t fp8_scale_rows(int M) { return ((size_t)M + 15) & ~(size_t)15; }
 
 hipError_t launch_fp8_quantize(const void* x, int type, int M, int K, uint8_t* codes, uint8_t* scales, hipStream_t s);

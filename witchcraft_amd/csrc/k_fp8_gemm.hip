@@ -169,100 +169,6 @@ __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int t
   }
 }
 
-// ---- gated, few rows: 16 MB rows x one block of 128 columns per workgroup --------------------
-// Eight waves side by side, 16 gate and the same 16 up columns each, KS such groups on the K blocks in
-// turn.  gelu(gate) * up stays in registers; the rows' maxima over the 128 columns meet in LDS.
-template <int ST, int MB, int KS>
-__global__ __launch_bounds__(512 * KS) void fp8_small_gated_kernel(Fp8GemmArgs p, int tiles_n, int64_t tiles) {
-  __shared__ f4 red[KS > 1 ? KS - 1 : 1][8][2 * MB][64];
-  __shared__ float tops[8][16 * MB];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int col = wave & 7, ks = wave >> 3;
-  const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK;
-  const size_t m16 = fp8_scale_rows(p.M);
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int m0 = (int)(tile / tiles_n) * 16 * MB, blk = (int)(tile % tiles_n), n0 = blk * FP8_BLOCK + 16 * col;
-    const bool live = n0 < p.N;  // N % 16 == 0: whole waves
-    f4 acc[2][MB];
-#pragma unroll
-    for (int i = 0; i < MB; i++) acc[0][i] = acc[1][i] = f4{0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const uint8_t* wrow[2] = {p.w + (size_t)(n0 + r) * p.K, p.w1 + (size_t)(n0 + r) * p.K};
-      const void* ws[2] = {p.w_scales, p.w1_scales};
-      const uint8_t *arow[MB], *sa[MB];
-#pragma unroll
-      for (int i = 0; i < MB; i++) {
-        const int m = min(m0 + 16 * i + r, p.M - 1);
-        arow[i] = p.a + (size_t)m * p.K;
-        sa[i] = p.a_scales + m;
-      }
-      for (int kb = ks; kb < kbs; kb += KS) {
-        i8v a[MB], w[2];
-        uint32_t as[MB], wb[2];
-        float wf[2];
-        const size_t at = (size_t)blk * kbs + kb;
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          w[j] = load_row(wrow[j], kb, g, p.K);
-          wb[j] = ST == FP8_E8M0 ? ((const uint8_t*)ws[j])[at] : 0;
-          wf[j] = ST == FP8_F32 ? ((const float*)ws[j])[at] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < MB; i++) {
-          a[i] = load_row(arow[i], kb, g, p.K);
-          as[i] = sa[i][kb * m16];
-        }
-#pragma unroll
-        for (int i = 0; i < MB; i++)
-#pragma unroll
-          for (int j = 0; j < 2; j++) block_product<false, ST>(w[j], a[i], as[i], wb[j], wf[j], acc[j][i]);
-      }
-    }
-    if constexpr (KS > 1) {
-      if (ks > 0)
-#pragma unroll
-        for (int i = 0; i < MB; i++) red[ks - 1][col][2 * i][lane] = acc[0][i], red[ks - 1][col][2 * i + 1][lane] = acc[1][i];
-      __syncthreads();
-      if (ks == 0)
-#pragma unroll
-        for (int k = 0; k < KS - 1; k++)
-#pragma unroll
-          for (int i = 0; i < MB; i++) acc[0][i] += red[k][col][2 * i][lane], acc[1][i] += red[k][col][2 * i + 1][lane];
-    }
-    f4 y[MB];
-    if (ks == 0) {
-#pragma unroll
-      for (int i = 0; i < MB; i++) {
-        float top = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          y[i][e] = gelu_tanh_dev(acc[0][i][e]) * acc[1][i][e];
-          top = fmaxf(top, finite_abs(y[i][e]));
-        }
-        top = max_xor32(max_xor16(top));
-        if (g == 0) tops[col][16 * i + r] = live ? top : 0.f;
-      }
-    }
-    __syncthreads();
-    if (ks == 0) {
-#pragma unroll
-      for (int i = 0; i < MB; i++) {
-        float top = tops[0][16 * i + r];
-#pragma unroll
-        for (int c = 1; c < 8; c++) top = fmaxf(top, tops[c][16 * i + r]);
-        const uint32_t byte = e8m0_of(top);
-        const float inv = e8m0_inverse(byte);
-        const int m = m0 + 16 * i + r;
-        if (live && m < p.M)
-          *reinterpret_cast<uint32_t*>((uint8_t*)p.out + (size_t)m * p.N + n0 + 4 * g) =
-              e4m3_pack4(y[i][0] * inv, y[i][1] * inv, y[i][2] * inv, y[i][3] * inv);
-        if (col == 0 && g == 0 && m < p.M) p.out_scales[blk * m16 + m] = (uint8_t)byte;
-      }
-    }
-    __syncthreads();  // tops and red are written again for the next tile
-  }
-}
-
 // ---- tiles: BM rows x BN weight rows per workgroup, K blocks through a double buffer in LDS --------
 // WM x WN waves, each MT x NT tiles of 16 x 16.  Both operands go global -> LDS without registers, a
 // K block (128 bytes of every row) per step; a row's eight 16-byte chunks are stored rotated (xor) by a
@@ -307,28 +213,100 @@ __device__ __forceinline__ void lds_copy_scale(i4v rsrc, uint32_t voff, uint32_t
                  : "memory");
 }
 constexpr uint32_t kOutside = 0x7fffffffu;  // past every descriptor's range
-constexpr int kTileMaxK = 1 << 21;          // 256 rows' bytes fit a descriptor and a lane's offset
 
-template <int SEL, int ST>
-__device__ __forceinline__ void tile_product_sel(const i8v& w, const i8v& a, uint32_t sa4, uint32_t swb, float swf, f4& acc) {
-  const f4 zero = f4{0.f, 0.f, 0.f, 0.f};
-  if constexpr (ST == FP8_E8M0) {
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, (int)swb, SEL, (int)sa4);
-  } else {
-    const f4 t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, zero, 0, 0, 0, 127, SEL, (int)sa4);
-#pragma unroll
-    for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(t[e], swf, acc[e]);
-  }
+// c + one K block of a 16 x 16 tile; sa4: four rows' scale bytes, sel the one; swb: the weights' byte.
+template <int SEL>
+__device__ __forceinline__ f4 scaled_mfma_sel(const i8v& w, const i8v& a, f4 c, uint32_t sa4, uint32_t swb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, (int)swb, SEL, (int)sa4);
 }
-template <int ST>
-__device__ __forceinline__ void tile_product(const i8v& w, const i8v& a, uint32_t sa4, int sel, uint32_t swb, float swf, f4& acc) {
+__device__ __forceinline__ f4 scaled_mfma(const i8v& w, const i8v& a, f4 c, uint32_t sa4, int sel, uint32_t swb) {
   switch (sel) {  // a constant once the loops are unrolled
-    case 0: tile_product_sel<0, ST>(w, a, sa4, swb, swf, acc); break;
-    case 1: tile_product_sel<1, ST>(w, a, sa4, swb, swf, acc); break;
-    case 2: tile_product_sel<2, ST>(w, a, sa4, swb, swf, acc); break;
-    default: tile_product_sel<3, ST>(w, a, sa4, swb, swf, acc); break;
+    case 0: return scaled_mfma_sel<0>(w, a, c, sa4, swb);
+    case 1: return scaled_mfma_sel<1>(w, a, c, sa4, swb);
+    case 2: return scaled_mfma_sel<2>(w, a, c, sa4, swb);
+    default: return scaled_mfma_sel<3>(w, a, c, sa4, swb);
   }
 }
+
+// The products of a wave's stripe of 16 rows with its NT weight operands, in SLOTS parts, so that a
+// caller can put its copies and reads between them.  With byte scales on both sides the instruction adds
+// into the accumulators.  Otherwise a block's sums are multiplied by their scale on the vector unit: a
+// stripe behind, so that the wave never waits for the sums that it has just asked for.  `fold` adds the
+// last stripe's at the end of a tile.
+template <bool EXACT, int ST, int MT, int NT>
+struct Products {
+  static constexpr bool DIRECT = !EXACT && ST == FP8_E8M0;
+  static constexpr int SLOTS = EXACT ? 4 : NT;
+  f4 acc[MT][NT];
+  f4 sums[DIRECT ? 1 : 2][DIRECT ? 1 : NT];
+  float factor[DIRECT ? 1 : 2][DIRECT ? 1 : NT];
+
+  __device__ __forceinline__ void clear() {
+    const f4 zero = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) acc[i][j] = zero;
+    if constexpr (!DIRECT) {
+#pragma unroll
+      for (int j = 0; j < NT; j++) sums[(MT - 1) & 1][j] = zero, factor[(MT - 1) & 1][j] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void add(int i, int j) {  // stripe i's sums
+    if constexpr (!DIRECT) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(sums[i & 1][j][e], factor[i & 1][j], acc[i][j][e]);
+    }
+  }
+  __device__ __forceinline__ void fold() {
+#pragma unroll
+    for (int j = 0; j < NT; j++) add(MT - 1, j);
+  }
+  // EXACT: the operands as f16, a quarter (32 of 128 K) at a time.  A part's products need quarter x; while
+  // they run, the weights' next quarter is widened (first stripe) and the next stripe's rows.
+  Wide ww[EXACT ? NT : 1], wa[EXACT ? 2 : 1];
+  __device__ __forceinline__ void widen_quarter(Wide& to, const i8v& from, int x) { to.v[x] = widen8(from[2 * x], from[2 * x + 1]); }
+  __device__ __forceinline__ void first_row(const i8v& a) {
+    if constexpr (EXACT) wa[0] = widen(a);
+  }
+  __device__ __forceinline__ void begin_step(const i8v (&w)[NT]) {
+    if constexpr (EXACT) {
+#pragma unroll
+      for (int j = 0; j < NT; j++) widen_quarter(ww[j], w[j], 0);
+    }
+  }
+  // Part x of stripe i: w the weight operands, a and next this stripe's rows and the next one's, sw(j) the
+  // bits of the weights' scales.
+  template <typename Scale>
+  __device__ __forceinline__ void part(int i, int x, const i8v (&w)[NT], const i8v& a, const i8v& next, uint32_t sa4, Scale sw) {
+    const f4 zero = f4{0.f, 0.f, 0.f, 0.f};
+    const int before = i ? i - 1 : MT - 1;
+    if constexpr (DIRECT) {
+      acc[i][x] = scaled_mfma(w[x], a, acc[i][x], sa4, i % 4, sw(x));
+    } else if constexpr (!EXACT) {
+      sums[i & 1][x] = scaled_mfma(w[x], a, zero, sa4, i % 4, 127);
+      factor[i & 1][x] = __uint_as_float(sw(x));
+      add(before, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+        sums[i & 1][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ww[j].v[x], wa[i & 1].v[x], x ? sums[i & 1][j] : zero, 0, 0, 0);
+      if (x == 0) {
+        const float f = e8m0_value((sa4 >> (8 * (i % 4))) & 255);
+#pragma unroll
+        for (int j = 0; j < NT; j++) factor[i & 1][j] = f * (ST == FP8_E8M0 ? e8m0_value(sw(j)) : __uint_as_float(sw(j)));
+      }
+#pragma unroll
+      for (int j = x * NT / 4; j < (x + 1) * NT / 4; j++) add(before, j);
+      if (i == 0 && x < 3) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) widen_quarter(ww[j], w[j], x + 1);
+      }
+      if (x > 0) widen_quarter(wa[(i + 1) & 1], next, x - 1);
+      if (x == 3) widen_quarter(wa[(i + 1) & 1], next, 3);
+    }
+  }
+};
 
 // Tile of the launch's index: bands of 8 row tiles, walked column by column, a contiguous stretch of
 // them per XCD (workgroups are dealt to the 8 XCDs in turn), so that what runs at one time on an XCD
@@ -351,6 +329,7 @@ template <int OUT, int MT, int NT>
 __device__ __forceinline__ void store_stripes(const Fp8GemmArgs& p, uint8_t* stage, int lane, int m0, int n0,
                                               const f4 (&v)[MT][NT]) {
   constexpr int SZ = OUT == FP8_IO_F32 ? 4 : 2, TJ = 8 / SZ;  // TJ: columns / 16 of 128 bytes
+  static_assert(NT % TJ == 0, "whole lines");
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int i = 0; i < MT; i++)
@@ -457,6 +436,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
   constexpr int LDS = REST + NW * 2048;
   static_assert(BM % (16 * NW) == 0 && BN % (8 * NW) == 0 && MT % 4 == 0 && BM <= 256, "whole copies, whole scale dwords");
   static_assert(BN <= FP8_BLOCK && FP8_BLOCK % BN == 0, "one weight scale per tile and K block");
+  constexpr int PS = Products<EXACT, ST, MT, NT>::SLOTS;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
@@ -528,9 +508,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
   // All copies but the newest CA + C1 (one step's) have landed, and this wave's reads are complete.
   auto arrive = [&]() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(CA + C1) : "memory"); };
 
-  f4 acc[MT][NT];
+  Products<EXACT, ST, MT, NT> prod;
   i8v a[2], w[NT];
-  Wide ww[EXACT ? NT : 1];
   uint32_t sa[MT / 4], sw;  // scales: of the rows' stripes, of the weights
   // lane's chunks g and g + 4 of its row: places (g ^ f) and (g ^ f) ^ 4
   const int arow = wm * 16 * MT + r * MT, wrow = wn * 16 * NT + r;
@@ -564,24 +543,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
 #pragma unroll
   for (int j = 0; j < NT; j++) read_w(j);
   read(alo, ahi, a[0]);
+  prod.first_row(a[0]);
   uint32_t slot = 0;
 
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int m0 = tm * BM, n0 = tn * BN;
     if (tile + gridDim.x < tiles) tile_place(tiles, tiles_m, tiles_n, tile + gridDim.x, tm, tn);
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+    prod.clear();
     int kb = 0;
     do {
       advance(c1, aim1);
       advance(c2, aim2);
       const uint32_t s = sw;
-      if constexpr (EXACT) {
-#pragma unroll
-        for (int j = 0; j < NT; j++) ww[j] = widen(w[j]);
-      }
+      prod.begin_step(w);
 #pragma unroll
       for (int i = 0; i < MT; i++) {
         const uint32_t sc = sa[i / 4];
@@ -598,24 +572,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
           read(alo, ahi, a[0]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        Wide wa;
-        if constexpr (EXACT) wa = widen(a[i & 1]);
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-          if constexpr (EXACT) wide_product<ST>(ww[j], wa, (sc >> (8 * (i % 4))) & 255, s, __uint_as_float(s), acc[i][j]);
-          else tile_product<ST>(w[j], a[i & 1], sc, i % 4, s, __uint_as_float(s), acc[i][j]);
+        for (int x = 0; x < PS; x++) {
+          prod.part(i, x, w, a[i & 1], a[(i + 1) & 1], sc, [&](int) { return s; });
           __builtin_amdgcn_sched_barrier(0);
-          if (i == MT - 1) read_w(j);  // each weight operand is replaced as soon as it has been used
+          if (i == MT - 1 && x < NT) read_w(x);  // each weight operand is replaced as soon as it has been used
           // this step's share of copies, behind the products: the next step's last stripes into its buffer,
           // then, once this step's first half is read, the step after it into this one's
           if (i < H - 1) {
+            constexpr int PARTS = (H - 1) * PS;
+            const int at = i * PS + x;
 #pragma unroll
-            for (int c = (i * NT + j) * CA / ((H - 1) * NT); c < (i * NT + j + 1) * CA / ((H - 1) * NT); c++) copy2(c, slot ^ 1);
+            for (int c = at * CA / PARTS; c < (at + 1) * CA / PARTS; c++) copy2(c, slot ^ 1);
           } else if (i < MT - 1) {
-            constexpr int SLOTS = (MT - H) * NT;
-            const int at = (i - H + 1) * NT + j;
+            constexpr int PARTS = (MT - H) * PS;
+            const int at = (i - H + 1) * PS + x;
 #pragma unroll
-            for (int c = at * C1 / SLOTS; c < (at + 1) * C1 / SLOTS; c++) copy1(c, slot);
+            for (int c = at * C1 / PARTS; c < (at + 1) * C1 / PARTS; c++) copy1(c, slot);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -623,8 +596,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
       slot ^= 1;
       kb++;
     } while (kb < kbs);
-
-    store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0 + wm * 16 * MT, n0 + wn * NT * 16, acc);
+    prod.fold();
+    store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0 + wm * 16 * MT, n0 + wn * NT * 16, prod.acc);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
 }
@@ -634,12 +607,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
 // columns).  Rows' codes are double-buffered in LDS; the weights have one buffer, a wave's own share:
 // their operands are in registers from a step's start, when the next step's are requested.  The two
 // workgroups run apart, so that one's results are formed and stored behind the other's products.
-template <int OUT, int ST, bool GATED, int MT, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+// DEEP, for launches that leave each compute unit one workgroup: a ring of three K blocks, weights and
+// rows, two of them on their way.
+template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP>
+__global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
   constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
-  constexpr int NT = 4, BM = 16 * MT, STAGE = BM * 128, NM = GATED ? 2 : 1;  // NM: matrices
+  constexpr int NT = 4, BM = 16 * MT, NM = GATED ? 2 : 1;                     // NM: matrices
+  constexpr int STAGES = DEEP ? 3 : 2, STAGE = BM * 128 + (DEEP ? NW * 8192 : 0);
   constexpr int COLS = (GATED ? 32 : 64) * NW, CA = BM / 8 / NW;              // CA: copies of rows per wave and K block
-  constexpr int WEIGHTS = 2 * STAGE, SCALES = WEIGHTS + NW * 8192, REST = SCALES + 512;
+  constexpr int WEIGHTS = DEEP ? BM * 128 : 2 * STAGE;  // DEEP: within a stage
+  constexpr int SCALES = STAGES * STAGE + (DEEP ? 0 : NW * 8192), REST = SCALES + STAGES * 256, OPS = 9 + CA;
   constexpr int LDS = REST + (GATED ? NW * BM * 4 : NW * 2048);
   static_assert(BM % (8 * NW) == 0 && MT % 4 == 0 && (!GATED || NW == 4), "whole copies; all columns of a scale");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
@@ -687,7 +664,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fp8_strip_kernel(Fp8GemmArgs p, in
   auto copy = [&](int j, uint32_t slot) {
     if (j < 8)
       lds_copy16(rw[GATED ? j / 4 : 0], cvw, ckb * 128u + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K,
-                 lds0 + WEIGHTS + wave * 8192 + j * 1024);
+                 lds0 + (DEEP ? slot * STAGE : 0) + WEIGHTS + wave * 8192 + j * 1024);
     else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, ckb * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
     else lds_copy4(rsa, vsa, ckb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
   };
@@ -697,9 +674,8 @@ __global__ __launch_bounds__(64 * NW, 2) void fp8_strip_kernel(Fp8GemmArgs p, in
     cvw = in ? vw : kOutside;
   };
 
-  f4 acc[MT][NT];
+  Products<EXACT, ST, MT, NT> prod;
   i8v a[2], w[NT];
-  Wide ww[EXACT ? NT : 1];
   uint32_t sa[MT / 4];
   // lane's chunks g and g + 4 of its row
   const uint32_t place = 16 * (g ^ (r & 7));
@@ -708,100 +684,108 @@ __global__ __launch_bounds__(64 * NW, 2) void fp8_strip_kernel(Fp8GemmArgs p, in
     const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
     v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   };
-  const uint32_t wat = WEIGHTS + wave * 8192 + r * 128;
+  uint32_t wat = WEIGHTS + wave * 8192 + r * 128;
   auto read_w = [&](int j) { read(wat + place + 2048 * j, wat + (place ^ 64) + 2048 * j, w[j]); };
   auto read_scales = [&]() {
 #pragma unroll
     for (int c = 0; c < MT / 4; c++) sa[c] = *reinterpret_cast<const uint32_t*>(lds + sat + 4 * c);
   };
 
+  auto next_block = [&]() {
+    if (++ckb == kbs) {
+      ckb = 0;
+      ctile += gridDim.x;
+      if (ctile < tiles) aim();
+      else climit = 0;
+    }
+    lane_offsets();
+  };
+  // the newest OPS copies may be on their way (DEEP: the step after next's); reads are complete
+  constexpr int IN_FLIGHT = DEEP ? OPS : 0, WAIT = (IN_FLIGHT & 15) | (IN_FLIGHT >> 4 << 14) | 0x70;
+
   aim();
+  weight_scales(tn * COLS, 0, ws);
+  int ptm = tm, ptn = tn;  // place of the tile that the products are at
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), so that the compiler knows its own loads to be complete
   lane_offsets();
 #pragma unroll
-  for (int j = 0; j < 9 + CA; j++) copy(j, 0);
-  weight_scales(tn * COLS, 0, ws);
-  // through the builtin, so that the compiler knows its own loads to be complete
-  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  for (int j = 0; j < OPS; j++) copy(j, 0);
+  if constexpr (DEEP) {
+    next_block();
+#pragma unroll
+    for (int j = 0; j < OPS; j++) copy(j, 1);
+  }
+  __builtin_amdgcn_s_waitcnt(WAIT);
   asm volatile("s_barrier" ::: "memory");
   read_scales();
 #pragma unroll
   for (int j = 0; j < NT; j++) read_w(j);
   read(alo, ahi, a[0]);
-  uint32_t slot = 0;
+  prod.first_row(a[0]);
+  uint32_t slot = 0, last = 0;
 
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int m0 = tm * BM, n0 = tn * COLS;
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+    const int m0 = ptm * BM, n0 = ptn * COLS;
+    if (tile + gridDim.x < tiles) tile_place(tiles, tiles_m, tiles_n, tile + gridDim.x, ptm, ptn);
+    weight_scales(ptn * COLS, 0, wsn);  // of the next tile
+    prod.clear();
     int kb = 0;
     do {
       if (kb && (kb & 63) == 0) {
         weight_scales(n0, kb, ws);
         __builtin_amdgcn_s_waitcnt(0x0f70);
       }
-      if (++ckb == kbs) {  // the next step begins the next tile
-        ckb = 0;
-        ctile += gridDim.x;
-        if (ctile < tiles) aim();
-        else climit = 0;
-        weight_scales(tn * COLS, 0, wsn);
-      }
-      lane_offsets();
+      next_block();
+      const uint32_t fill = DEEP ? (slot == 0 ? 2 : slot - 1) : slot ^ 1, after = DEEP ? (slot == 2 ? 0 : slot + 1) : slot ^ 1;
       uint32_t swb[NM];
 #pragma unroll
       for (int j = 0; j < NM; j++) swb[j] = __builtin_amdgcn_readlane(ws[j], kb & 63);
-      if constexpr (EXACT) {
-#pragma unroll
-        for (int j = 0; j < NT; j++) ww[j] = widen(w[j]);
-      }
+      prod.begin_step(w);
 #pragma unroll
       for (int i = 0; i < MT; i++) {
         const uint32_t sc = sa[i / 4];
         if (i < MT - 1) {
           read(alo + (i + 1) * 2048, ahi + (i + 1) * 2048, a[(i + 1) & 1]);
         } else {
-          // all copies have landed; every wave has the next step's rows in LDS, and this step's in registers
-          __builtin_amdgcn_s_waitcnt(0x0070);
+          // the next step's copies have landed; every wave has its rows in LDS, and this step's in registers
+          __builtin_amdgcn_s_waitcnt(WAIT);
           asm volatile("s_barrier" ::: "memory");
-          const uint32_t step = slot ? -STAGE : STAGE;
-          alo += step, ahi += step, sat += slot ? -256 : 256;
+          const uint32_t step = after == 0 ? (uint32_t)-((STAGES - 1) * STAGE) : (uint32_t)STAGE;
+          alo += step, ahi += step, sat += after == 0 ? -(STAGES - 1) * 256 : 256;
+          if (DEEP) wat += step;
           read_scales();
           read(alo, ahi, a[0]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        Wide wa;
-        if constexpr (EXACT) wa = widen(a[i & 1]);
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-          const uint32_t s = swb[GATED ? j / 2 : 0];
-          if constexpr (EXACT) wide_product<ST>(ww[j], wa, (sc >> (8 * (i % 4))) & 255, s, __uint_as_float(s), acc[i][j]);
-          else tile_product<ST>(w[j], a[i & 1], sc, i % 4, s, __uint_as_float(s), acc[i][j]);
+        for (int x = 0; x < 4; x++) {
+          prod.part(i, x, w, a[i & 1], a[(i + 1) & 1], sc, [&](int j) { return swb[GATED ? j / 2 : 0]; });
           __builtin_amdgcn_sched_barrier(0);
-          if (i == MT - 1) read_w(j);  // each weight operand is replaced as soon as it has been used
+          if (i == MT - 1) read_w(x);  // each weight operand is replaced as soon as it has been used
           // Behind the products: the next step's weights, whose buffer has been read, and rows.
-          constexpr int OPS = 9 + CA, SLOTS = (MT - 2) * NT;
-          const int at = i * NT + j;
+          constexpr int PARTS = (MT - 2) * 4;
+          const int at = i * 4 + x;
           if (at == 0) __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): w is in registers
-          if (at < SLOTS) {
+          if (at < PARTS) {
 #pragma unroll
-            for (int c = at * OPS / SLOTS; c < (at + 1) * OPS / SLOTS; c++) copy(c, slot ^ 1);
+            for (int c = at * OPS / PARTS; c < (at + 1) * OPS / PARTS; c++) copy(c, fill);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      slot ^= 1;
+      last = slot;
+      slot = after;
       kb++;
     } while (kb < kbs);
 #pragma unroll
     for (int j = 0; j < NM; j++) ws[j] = wsn[j];
+    prod.fold();
 
     if constexpr (!GATED) {
-      store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, acc);
+      store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, prod.acc);
     } else {
       // staged in the rows' buffer that the next step's copies go to
-      gated_stripes<MT>(p, reinterpret_cast<float*>(lds + REST), lds + (slot ^ 1) * STAGE, lane, wave, m0, n0, m16, acc);
+      gated_stripes<MT>(p, reinterpret_cast<float*>(lds + REST), lds + last * STAGE, lane, wave, m0, n0, m16, prod.acc);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
@@ -818,33 +802,24 @@ hipError_t launch_small(const Fp8GemmArgs& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int ST, int MB, int KS>
-hipError_t launch_small_gated(const Fp8GemmArgs& p, hipStream_t s) {
-  const int tiles_n = (p.N + FP8_BLOCK - 1) / FP8_BLOCK;
-  const int64_t tiles = (int64_t)((p.M + 16 * MB - 1) / (16 * MB)) * tiles_n;
-  T5K_LAUNCH((fp8_small_gated_kernel<ST, MB, KS>), dim3((unsigned)std::min(tiles, kMostGroups)), dim3(512 * KS), 0, s,
-             p, tiles_n, tiles);
-  return hipGetLastError();
-}
-
 template <int OUT, int ST, int BM, int BN, int WM, int WN>
 hipError_t launch_tile(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
-  if (p.K > kTileMaxK || tiles >> 30) return hipErrorInvalidValue;
+  if (tiles >> 30) return hipErrorInvalidValue;
   T5K_LAUNCH((fp8_tile_kernel<OUT, ST, BM, BN, WM, WN>), dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / (WM * WN)))),
              dim3(64 * WM * WN), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
-template <int OUT, int ST, bool GATED, int MT, int NW>
+template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP>
 hipError_t launch_strip(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   constexpr int COLS = (GATED ? 32 : 64) * NW;
   const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + COLS - 1) / COLS;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
-  if (p.K > kTileMaxK || tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW>), dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / NW))), dim3(64 * NW), 0,
-             s, p, tiles_m, tiles_n);
+  if (tiles >> 30) return hipErrorInvalidValue;
+  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, DEEP>),
+             dim3((unsigned)std::min<int64_t>(tiles, cus * (DEEP ? 1 : 8 / NW))), dim3(64 * NW), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
@@ -859,27 +834,50 @@ int compute_units() {
   return cus;
 }
 
+// Few tiles: operands straight to the waves, K dealt out over the waves of a workgroup, as many 16 x 16
+// tiles per workgroup as leave about a workgroup or two per compute unit (us, 32 x 2,304 x 768 / 64 x 768 x
+// 2,048 / 64 x 2,304 x 768 / 64 x 8,192 x 4,096: 1 x 1 tiles 3.8 / 4.3 / 4.6 / 31.6, 1 x 2 3.6 / 5.2 / 4.6 /
+// 24.7, 2 x 2 4.2 / 6.4 / 4.2 / 17.4, 4 x 2 4.5 / 8.4 / 5.1 / 14.8, LDS tiles of 128 x 128 5.9 / 10.1 / 6.1 /
+// 17.1).  Then LDS tiles, where they are enough to fill half of the chip or have the rows.
 template <int OUT, int ST>
 hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
-  if (p.M <= 64 || p.K > kTileMaxK) return launch_small<OUT, ST, 2, 2, 4>(p, s);
+  const int64_t m = p.M, n = p.N, t16 = ((m + 15) / 16) * ((n + 15) / 16), t128 = ((m + 127) / 128) * ((n + 127) / 128);
+  if (t16 <= 256) return launch_small<OUT, ST, 1, 1, 8>(p, s);
+  if (t16 <= 512) return launch_small<OUT, ST, 1, 2, 8>(p, s);
+  if (t16 <= 1024) return launch_small<OUT, ST, 2, 2, 4>(p, s);
+  if (m <= 64 || t128 < 32) return launch_small<OUT, ST, 4, 2, 8>(p, s);
   const int cus = compute_units();
-  if constexpr (OUT != FP8_IO_F32) {
-    if ((int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256) >= cus) return launch_strip<OUT, ST, false, 8, 4>(p, cus, s);
+  if constexpr (OUT == FP8_IO_F32) {
+    // 64 x 256 strips against 64 x 128 tiles: 22.6 / 23.9 us for 4,616 x 768 x 2,048 (219 strips), 41 / 29 for
+    // 256 x 8,192 x 4,096 (128 strips)
+    if (((m + 63) / 64) * ((n + 255) / 256) < 200) return launch_tile<OUT, ST, 64, 128, 1, 4>(p, cus, s);
+    return launch_strip<OUT, ST, false, 4, 4, false>(p, cus, s);
+  } else {
+    // strips win once every compute unit has two: 112 against 136 us for 74,640 x 2,048 x 768, 12.4 against
+    // 12.2 for 4,616 x 2,048 x 768 (296 strips), 18.7 against 11.2 for 4,616 x 768 x 2,048 (111)
+    if (((m + 127) / 128) * ((n + 255) / 256) >= 2 * cus) return launch_strip<OUT, ST, false, 8, 4, false>(p, cus, s);
+    return launch_tile<OUT, ST, 128, 128, 2, 2>(p, cus, s);
   }
-  return launch_tile<OUT, ST, 128, 128, 2, 2>(p, cus, s);
 }
 
+// A scale needs all of its 128 columns in one workgroup.  Up to one strip per compute unit the ring of three
+// K blocks is faster (256 x 8,192 x 4,096, 256 strips of 64 rows: 23 against 32 us; 4,616 x 768 x 2,048, 222 of
+// 128 rows: 18.5 against 21.8), beyond that two workgroups on a compute unit (4,616 x 2,048 x 768: 22 against
+// 27).
 template <int ST>
 hipError_t launch_gated(const Fp8GemmArgs& p, hipStream_t s) {
-  if (p.M <= 64 || p.K > kTileMaxK) return launch_small_gated<ST, 2, 1>(p, s);
-  return launch_strip<FP8_IO_NONE, ST, true, 8, 4>(p, compute_units(), s);
+  const int cus = compute_units();
+  const int64_t blocks = (p.N + 127) / 128, t4 = (int64_t)((p.M + 63) / 64) * blocks, t8 = (int64_t)((p.M + 127) / 128) * blocks;
+  if (t4 <= cus) return launch_strip<FP8_IO_NONE, ST, true, 4, 4, true>(p, cus, s);
+  if (t8 <= cus) return launch_strip<FP8_IO_NONE, ST, true, 8, 4, true>(p, cus, s);
+  return launch_strip<FP8_IO_NONE, ST, true, 8, 4, false>(p, cus, s);
 }
 }  // namespace
 
 namespace t5k {
 hipError_t launch_fp8_matmul(const Fp8GemmArgs& p, hipStream_t s) {
   if (p.M == 0 || p.N == 0) return hipSuccess;
-  if (p.M < 0 || p.N < 0 || p.K <= 0 || p.K % 16) return hipErrorInvalidValue;
+  if (p.M < 0 || p.N < 0 || p.K <= 0 || p.K % 16 || p.K > FP8_MAX_K) return hipErrorInvalidValue;
   switch (2 * p.out_type + p.scale_type) {
     case 2 * FP8_IO_F32 + FP8_E8M0: return launch_product<FP8_IO_F32, FP8_E8M0>(p, s);
     case 2 * FP8_IO_F32 + FP8_F32: return launch_product<FP8_IO_F32, FP8_F32>(p, s);
@@ -893,7 +891,7 @@ hipError_t launch_fp8_matmul(const Fp8GemmArgs& p, hipStream_t s) {
 
 hipError_t launch_fp8_gated_gelu(const Fp8GemmArgs& p, hipStream_t s) {
   if (p.M == 0 || p.N == 0) return hipSuccess;
-  if (p.M < 0 || p.N < 0 || p.N % 16 || p.K <= 0 || p.K % 16) return hipErrorInvalidValue;
+  if (p.M < 0 || p.N < 0 || p.N % 16 || p.K <= 0 || p.K % 16 || p.K > FP8_MAX_K) return hipErrorInvalidValue;
   if (p.scale_type == FP8_E8M0) return launch_gated<FP8_E8M0>(p, s);
   if (p.scale_type == FP8_F32) return launch_gated<FP8_F32>(p, s);
   return hipErrorInvalidValue;
