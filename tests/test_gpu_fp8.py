@@ -11,7 +11,7 @@ Products.  Codes of few bits and small integers have exact products and sums, so
 the correctly rounded result (`exact` tests, over all shapes).  On ordinary data an f32 result is
 within f32 summation rounding, (K + 16) 2^-23 sum |a w|; an f16 or bf16 result within its own half step
 (2^-11, 2^-8 of the value) plus the fp8 matrix instructions' alignment: each product is kept to 2^-12
-of the largest of its group at worst, so a K block is off by at most 128 * 2^-12 of its largest
+of the largest of its group at worst (2^-13 as measured), so a K block is off by at most 128 * 2^-12 of its largest
 product, and, errors of either sign, by far less in the 2-norm.
 """
 import numpy as np

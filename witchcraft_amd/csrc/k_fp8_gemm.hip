@@ -10,11 +10,11 @@
 // as the instruction's own scale operand, and so does the weights' byte; float weight scales multiply
 // the block's sum in f32 on the vector unit.
 //
-// Precision.  The fp8 MFMAs add their products in groups of 8 to 16 values, each aligned to the
-// group's largest product with 14 bits or so (measured: 2^14 + 2^0 in one group gives 2^14, 2^14 +
-// 2^2 is kept; sums of groups and blocks are f32).  On normal data that is an error of 1.3e-5 of the
-// result's norm: below the rounding of f16 (2^-11 of a value) and bf16 results and of codes (2^-4),
-// but not what an f32 result promises.  f32 results are therefore computed exactly to f32 sums on
+// Precision.  The fp8 MFMAs align the products of eight consecutive K of a lane to the largest of them and
+// keep 2^-13 of it (measured: 2^16 + 2^3 is exact, 2^16 + 2^2 in one group gives 2^16); sums of groups
+// and blocks are f32.  On normal data that is an error of 1.3e-5 of the result's norm: below the
+// rounding of f16 (2^-11 of a value) and bf16 results and of codes (2^-4), but not what an f32 result
+// promises.  f32 results are therefore computed exactly to f32 sums on
 // v_mfma_f32_16x16x32_f16, at half the rate, from codes widened to f16 (every e4m3 value is one).
 #include "fp8.hpp"
 
@@ -114,7 +114,7 @@ __device__ __forceinline__ void store_out(const Fp8GemmArgs& p, int m, int n, f4
 template <int OUT, int ST, int MB, int NB, int KS>
 __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int tiles_n, int64_t tiles) {
   __shared__ f4 red[KS][MB * NB][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK;
   const size_t m16 = fp8_scale_rows(p.M);
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -369,55 +369,82 @@ __device__ __forceinline__ void store_stripes(const Fp8GemmArgs& p, uint8_t* sta
 // (n0 + 32 wave ..) of the 128 whose scale four waves share.  The rows' maxima meet in tops [16 MT][4],
 // the codes in stage [MT][16][128], from where they are stored in whole lines.
 template <int MT>
-__device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, float* tops, uint8_t* stage, int lane, int wave, int m0,
+__device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, uint32_t* tops, uint8_t* stage, int lane, int wave, int m0,
                                               int n0, int m16, f4 (&acc)[MT][4]) {
   const int r = lane & 15, g = lane >> 4;
-#pragma unroll
-  for (int j = 0; j < 2; j++)
-    if (n0 + wave * 32 + 16 * j >= p.N) {
-#pragma unroll
-      for (int i = 0; i < MT; i++) acc[i][j] = acc[i][j + 2] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-#pragma unroll
-  for (int i = 0; i < MT; i++) {
-    float top = 0.f;
+  const int left = p.N - n0 - wave * 32;  // columns past N do not count (N % 16 == 0: whole 16s)
+  // Magnitudes are compared as their bits, which order alike and need no quieting of NaN.
+  auto largest = [&](int i, bool finite) {
+    uint32_t t[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        acc[i][j][e] = gelu_tanh_dev(acc[i][j][e]) * acc[i][j + 2][e];
-        top = fmaxf(top, fabsf(acc[i][j][e]));
+        const float y = acc[i][j][e];
+        t[j] = max(t[j], __float_as_uint(finite ? finite_abs(y) : fmaxf(0.f, fabsf(y))));  // fmaxf leaves NaN out
       }
-    if (top == INFINITY) {  // taken again over the finite values (fmaxf has left NaN out)
-      top = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, finite_abs(acc[i][j][e]));
-    }
-    top = max_xor32(max_xor16(top));
-    if (g == 0) tops[(16 * i + r) * 4 + wave] = top;
-  }
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  uint8_t* scales = p.out_scales + (size_t)(n0 / FP8_BLOCK) * m16 + m0 + r * MT;
+    return max(left > 0 ? t[0] : 0u, left > 16 ? t[1] : 0u);
+  };
+  uint32_t top[MT], all = 0;
 #pragma unroll
   for (int i = 0; i < MT; i++) {
-    const f4 t4 = *reinterpret_cast<const f4*>(tops + (16 * i + r) * 4);
-    const uint32_t byte = e8m0_of(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
-    const float s = __uint_as_float(byte << 23);
 #pragma unroll
-    for (int j = 0; j < 2; j++)  // 16-byte piece 2 wave + j of the row
-      *reinterpret_cast<uint32_t*>(stage + (16 * i + r) * 128 + 16 * ((2 * wave + j) ^ (r & 7)) + 4 * g) =
-          e4m3_pack4_scaled(acc[i][j], s);
-    if (wave == 0 && g == 0 && m0 + r * MT + i < p.M) scales[i] = (uint8_t)byte;
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[i][j][e] = gelu_tanh_dev(acc[i][j][e]) * acc[i][j + 2][e];
+    top[i] = largest(i, false);
+    all = max(all, top[i]);
+  }
+  if (all >= 0x7f800000u) {  // infinities do not count
+#pragma unroll
+    for (int i = 0; i < MT; i++) top[i] = largest(i, true);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    const auto x = __builtin_amdgcn_permlane16_swap(top[i], top[i], false, false);
+    const uint32_t half = max(x[0], x[1]);
+    const auto y = __builtin_amdgcn_permlane32_swap(half, half, false, false);
+    top[i] = max(y[0], y[1]);
+  }
+  uint32_t* trow = tops + 4 * r;
+  if (g == 0) {
+#pragma unroll
+    for (int i = 0; i < MT; i++) trow[64 * i + wave] = top[i];
   }
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  const int c = lane & 7, n = n0 + 16 * c;
+  uint8_t* to[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) to[j] = stage + r * 128 + 16 * ((2 * wave + j) ^ (r & 7)) + 4 * g;  // 16-byte piece 2 wave + j
+  uint32_t bytes[MT / 4] = {};
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    const uint4 t4 = *reinterpret_cast<const uint4*>(trow + 64 * i);
+    const uint32_t byte = e8m0_of(__uint_as_float(max(max(t4.x, t4.y), max(t4.z, t4.w))));
+    bytes[i / 4] |= byte << (8 * (i % 4));
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      *reinterpret_cast<uint32_t*>(to[j] + 2048 * i) = e4m3_pack4_scaled(acc[i][j], __uint_as_float(byte << 23));
+  }
+  if (wave == 0 && g == 0) {
+    const int m = m0 + r * MT;
+    uint8_t* scales = p.out_scales + (size_t)(n0 / FP8_BLOCK) * m16 + m;
+    if (m + MT <= p.M) {
+#pragma unroll
+      for (int c = 0; c < MT / 4; c++) reinterpret_cast<uint32_t*>(scales)[c] = bytes[c];
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+        if (m + i < p.M) scales[i] = (uint8_t)(bytes[i / 4] >> (8 * (i % 4)));
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  const int c = lane & 7, rr = 8 * (wave & 1) + (lane >> 3), n = n0 + 16 * c;
+  const uint8_t* from = stage + (wave / 2) * 2048 + rr * 128 + 16 * (c ^ (rr & 7));
 #pragma unroll
   for (int q = 0; q < MT / 2; q++) {
-    const int i = 2 * q + wave / 2, rr = 8 * (wave & 1) + (lane >> 3), m = m0 + rr * MT + i;
-    if (m < p.M && n < p.N)  // N % 16 == 0: whole pieces
-      __builtin_nontemporal_store(*reinterpret_cast<const i4v*>(stage + (16 * i + rr) * 128 + 16 * (c ^ (rr & 7))),
+    const int m = m0 + rr * MT + 2 * q + wave / 2;
+    if (m < p.M && n < p.N)  // whole pieces
+      __builtin_nontemporal_store(*reinterpret_cast<const i4v*>(from + 4096 * q),
                                   reinterpret_cast<i4v*>((uint8_t*)p.out + (size_t)m * p.N + n));
   }
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // stage is copied into again
@@ -785,7 +812,7 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
       store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, prod.acc);
     } else {
       // staged in the rows' buffer that the next step's copies go to
-      gated_stripes<MT>(p, reinterpret_cast<float*>(lds + REST), lds + last * STAGE, lane, wave, m0, n0, m16, prod.acc);
+      gated_stripes<MT>(p, reinterpret_cast<uint32_t*>(lds + REST), lds + last * STAGE, lane, wave, m0, n0, m16, prod.acc);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
