@@ -655,7 +655,8 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   // ---- copies of the next step: K block ckb of tile ctile.  One brings 8 rows, lane l chunk (l % 8) ^ (l / 8)
   // of its row l / 8 to place l % 8.  In LDS the activations are ordered by stripe, [MT][16]; consecutive
   // ones lie MT apart in memory.  Descriptors end with the matrix; one whose rows are all past it has
-  // the tile's first rows, which nothing uses.
+  // the tile's first rows, which nothing uses.  No scalar offset passes its descriptor's end (a copy of
+  // weight rows past the matrix is held there): the range check may subtract it from the size.
   uint32_t ctile = blockIdx.x;
   int ckb = 0, climit = p.K;  // climit 0: past the last tile, zeros
   int tm, tn;                 // place of tile ctile
@@ -690,7 +691,8 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   uint32_t cva, cvw;  // this step's lane offsets; chunks past K lie outside
   auto copy = [&](int j, uint32_t slot) {
     if (j < 8)
-      lds_copy16(rw[GATED ? j / 4 : 0], cvw, ckb * 128u + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K,
+      lds_copy16(rw[GATED ? j / 4 : 0], cvw,
+                 min(ckb * 128u + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K, (uint32_t)rw[GATED ? j / 4 : 0][2]),
                  lds0 + (DEEP ? slot * STAGE : 0) + WEIGHTS + wave * 8192 + j * 1024);
     else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, ckb * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
     else lds_copy4(rsa, vsa, ckb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
