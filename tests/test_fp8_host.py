@@ -20,7 +20,7 @@ def _refused(fn, *args, says=""):
 
 @pytest.mark.parametrize("x,t,m,k,codes,scales,says", [
     (P, 0, -1, 128, P, P, "rows"), (P, 0, BIG, 128, P, P, "rows"), (P, 0, 4, 0, P, P, "row length"),
-    (P, 0, 4, 24, P, P, "row length"), (P, 0, 4, -128, P, P, "row length"), (P, 0, 4, BIG, P, P, "row length"),
+    (P, 0, 4, (1 << 21) + 16, P, P, "row length"), (P, 0, 4, 24, P, P, "row length"), (P, 0, 4, -128, P, P, "row length"), (P, 0, 4, BIG, P, P, "row length"),
     (P, 3, 4, 128, P, P, "type"), (P, -1, 4, 128, P, P, "type"), (None, 0, 4, 128, P, P, "NULL"),
     (P, 0, 4, 128, None, P, "NULL"), (P, 0, 4, 128, P, None, "NULL"), (P + 4, 0, 4, 128, P, P, "aligned"),
     (P, 0, 4, 128, P + 8, P, "aligned"), (P, 0, 4, 128, P, P + 1, "aligned"), (P, 0, 1 << 30, 512, P, P, "blocks"),
@@ -62,7 +62,7 @@ def _product(a=P, a_s=P, m=4, w=P, w_s=P, n=32, k=128, st=0, c=P, ct=0):
 
 @pytest.mark.parametrize("args,says", [
     (dict(m=-1), "rows"), (dict(n=-1), "rows"), (dict(n=BIG), "rows"), (dict(k=40), "row length"),
-    (dict(st=7), "scale type"), (dict(ct=3), "type"), (dict(a=None), "NULL"), (dict(a_s=None), "NULL"),
+    (dict(k=(1 << 21) + 16), "row length"), (dict(st=7), "scale type"), (dict(ct=3), "type"), (dict(a=None), "NULL"), (dict(a_s=None), "NULL"),
     (dict(w=None), "NULL"), (dict(w_s=None), "NULL"), (dict(c=None), "NULL"), (dict(a=P + 1), "aligned"),
     (dict(a_s=P + 8), "aligned"), (dict(w=P + 8), "aligned"), (dict(st=1, w_s=P + 1), "aligned"),
     (dict(c=P + 4), "aligned"),

@@ -347,6 +347,61 @@ def test_matmul_exact(fp8, M, N, K, scale):
         assert torch.equal(got, ref), (kind, int((got != ref).sum()))
 
 
+# One shape at least on each side of every border of the kernels' choice, tiles that end inside on both
+# axes, workgroups that walk several tiles, and more than 64 K blocks.
+VARIANTS = [
+    (16, 4096, 144), (16, 4100, 144), (15, 8192, 256), (16, 8200, 128), (13, 16384, 128), (16, 16400, 272),
+    (64, 16390, 144), (65, 3968, 400), (65, 3969, 400), (70, 5001, 8336), (8199, 1100, 272), (8201, 2055, 144),
+    (4161, 1027, 8336), (8201, 2056, 8336), (16413, 1027, 272), (16413, 1032, 16), (33000, 515, 384),
+]
+
+
+@pytest.mark.parametrize("scale", [E8M0, F32S])
+@pytest.mark.parametrize("M,N,K", VARIANTS)
+def test_matmul_variants(fp8, M, N, K, scale):
+    """As test_matmul_exact: at K = 8,336 sums stay below 2^19 over steps of 2^-3."""
+    test_matmul_exact(fp8, M, N, K, scale)
+
+
+def _signs(shape, seed):
+    """Codes of -1, 0 and 1 on the device, and a function that gives a stretch of columns in 64 bits."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    v = torch.randint(0, 3, shape, generator=g, device=DEV, dtype=torch.uint8)
+    codes = torch.tensor([0, 0x38, 0xb8], dtype=torch.uint8, device=DEV)[v.int()]
+    table = torch.from_numpy(TABLE).to(DEV)
+    return codes, lambda a, b: table[codes[:, a:b].int()]
+
+
+def _unit_scales(n, k, rows):
+    return torch.full((_blocks(k), _rows16(n)) if rows else (_blocks(n), _blocks(k)), 127, dtype=torch.uint8, device=DEV)
+
+
+def _long_product(a, w, K):
+    return sum(a(k, min(K, k + 131072)) @ w(k, min(K, k + 131072)).t() for k in range(0, K, 131072))
+
+
+@pytest.mark.parametrize("M,N", [(3, 70), (65, 4100)])
+def test_matmul_longest_rows(fp8, M, N):
+    """K = 2^21; sums of signs are exact."""
+    K = 1 << 21
+    (a, av), (w, wv) = _signs((M, K), 1), _signs((N, K), 2)
+    want = _long_product(av, wv, K).float()
+    for kind in ("f32", "bf16"):
+        got = _matmul(fp8, a, _unit_scales(M, K, True), w, _unit_scales(N, K, False), N, kind, E8M0)
+        assert torch.equal(got, want.to(TYPES[kind][1])), kind
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_matmul_large_offsets(fp8, kind):
+    """More than 2^31 results."""
+    M, N, K = 300001, 8200, 16
+    (a, av), (w, wv) = _signs((M, K), 3), _signs((N, K), 4)
+    got = _matmul(fp8, a, _unit_scales(M, K, True), w, _unit_scales(N, K, False), N, kind, E8M0)
+    want = av(0, K).to(TYPES[kind][1]).float(), wv(0, K).float()
+    for m in range(0, M, 20000):
+        assert torch.equal(got[m:m + 20000].float(), want[0][m:m + 20000] @ want[1].t()), m
+
+
 def _ordinary(fp8, M, N, K, scale, seed):
     """Quantized normal data with outlying channels, through the quantizers, and the values it stands for."""
     g = torch.Generator(device=DEV).manual_seed(seed)
@@ -536,6 +591,44 @@ def test_gated_ordinary(fp8, M, N, K, scale):
     got = TABLE[codes] * np.repeat(2.0 ** (s.T - 127.0), 128, 1)[:, :N]
     y = y.cpu().numpy()
     assert np.linalg.norm(got - y) <= 2.0 ** -4 / 3 ** 0.5 * np.linalg.norm(y)
+
+
+@pytest.mark.parametrize("scale", [E8M0, F32S])
+@pytest.mark.parametrize("M,N,K", [(70, 400, 8336), (1100, 1040, 400), (2100, 1040, 8336), (2100, 1936, 400),
+                                   (2100, 2064, 272), (4200, 1040, 8336), (8201, 1040, 144), (33000, 272, 16)])
+def test_gated_variants(fp8, M, N, K, scale):
+    """Both sides of the borders at one strip of 64 and of 128 rows per compute unit, several tiles per
+    workgroup, more than 64 K blocks."""
+    test_gated_exact_products(fp8, M, N, K, scale)
+
+
+@pytest.mark.parametrize("M,N", [(70, 272), (2100, 1040), (4200, 1040)])
+def test_gated_infinite_products(fp8, M, N):
+    """A product past f32's range has a NaN code and does not count towards its block's scale; huge finite
+    ones do, and a gate of -2^64 closes to -0."""
+    K = 272
+    a, w0, w1 = np.zeros((M, K)), np.zeros((N, K)), np.zeros((N, K))
+    a[1::2, 0], a[:, 200] = 1, 1
+    n = np.arange(N)
+    w0[n % 4 == 0, 0] = w1[n % 4 == 0, 0] = 1       # 2^64 * 2^64
+    w0[n % 4 == 1, 200], w1[n % 4 == 1, 200] = 2, 1.5
+    w0[n % 4 == 2, 200], w1[n % 4 == 2, 0] = 1, 1   # gelu(1) 2^64
+    w0[n % 4 == 3, 0], w1[n % 4 == 3, 0] = -1, 1
+    w0[128:256], w1[128:256] = 0, 0                 # a block with one finite value
+    w0[130, 200] = w1[130, 200] = w0[140, 0] = w1[140, 0] = 1
+    bytes_ = np.full((_blocks(K), M), 127)
+    bytes_[0] += 64
+    ac, asc = _operand(a, bytes_, M, K)
+    w = [torch.from_numpy(_round_e4m3(v)).to(DEV) for v in (w0, w1)]
+    unit = _unit_scales(N, K, False)
+    x = a.copy()
+    x[:, 0] *= 2.0 ** 64
+    gate, up = torch.from_numpy(x @ w0.T), x @ w1.T
+    with np.errstate(over="ignore"):
+        y = (_gelu(gate).numpy() * up).astype(np.float32).astype(np.float64)
+    assert np.isinf(y[1, 0]) and np.isfinite(y[0]).all()
+    codes, s = _gated(fp8, ac, asc, w[0], unit, w[1], unit, E8M0)
+    _check_codes(codes, s, y, GELU_REL)
 
 
 @pytest.mark.parametrize("M", [5, 40, 600])
