@@ -325,14 +325,14 @@ __device__ __forceinline__ void tile_place(uint32_t tiles, int tiles_m, int tile
 // time, 16-byte pieces rotated by the row) and stored in whole lines, past the caches: 64-byte pieces
 // straight from registers took 151 us instead of 114 for 74,640 x 2,048 (x 768) in bf16, whole lines
 // without the non-temporal hint 141.  Rows of C that do not keep 16-byte alignment go value by value.
-template <int OUT, int MT, int NT>
+template <int OUT, int FROM, int TO, int MT, int NT>
 __device__ __forceinline__ void store_stripes(const Fp8GemmArgs& p, uint8_t* stage, int lane, int m0, int n0,
                                               const f4 (&v)[MT][NT]) {
   constexpr int SZ = OUT == FP8_IO_F32 ? 4 : 2, TJ = 8 / SZ;  // TJ: columns / 16 of 128 bytes
   static_assert(NT % TJ == 0, "whole lines");
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int i = 0; i < MT; i++)
+  for (int i = FROM; i < TO; i++)
 #pragma unroll
     for (int h = 0; h < NT / TJ; h++) {
 #pragma unroll
@@ -624,7 +624,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
       kb++;
     } while (kb < kbs);
     prod.fold();
-    store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0 + wm * 16 * MT, n0 + wn * NT * 16, prod.acc);
+    store_stripes<OUT, 0, MT>(p, lds + REST + wave * 2048, lane, m0 + wm * 16 * MT, n0 + wn * NT * 16, prod.acc);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
 }
@@ -635,21 +635,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
 // their operands are in registers from a step's start, when the next step's are requested.  The two
 // workgroups run apart, so that one's results are formed and stored behind the other's products.
 // DEEP, for launches that leave each compute unit one workgroup: a ring of three K blocks, weights and
-// rows, two of them on their way.
-template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP>
-__global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+// rows, two of them on their way.  KG = 2, for f32 results of such launches: a second group of waves takes
+// the second half of the K blocks, so that each SIMD still has two waves (the vector unit widens for one
+// while the matrix unit works for the other), and the two exchange sums at the end; the halves are
+// always added in the same order, first and second (addition commutes).
+template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP, int KG>
+__global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
   constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
   constexpr int NT = 4, BM = 16 * MT, NM = GATED ? 2 : 1;                     // NM: matrices
   constexpr int STAGES = DEEP ? 3 : 2, STAGE = BM * 128 + (DEEP ? NW * 8192 : 0);
   constexpr int COLS = (GATED ? 32 : 64) * NW, CA = BM / 8 / NW;              // CA: copies of rows per wave and K block
   constexpr int WEIGHTS = DEEP ? BM * 128 : 2 * STAGE;  // DEEP: within a stage
-  constexpr int SCALES = STAGES * STAGE + (DEEP ? 0 : NW * 8192), REST = SCALES + STAGES * 256, OPS = 9 + CA;
-  constexpr int LDS = REST + (GATED ? NW * BM * 4 : NW * 2048);
+  constexpr int SCALES = STAGES * STAGE + (DEEP ? 0 : NW * 8192), GROUP = SCALES + STAGES * 256, OPS = 9 + CA;
+  constexpr int REST = KG * GROUP, EXCHANGE = REST + KG * NW * 2048;
+  constexpr int LDS = GATED ? REST + NW * BM * 4 : EXCHANGE + (KG > 1 ? KG * NW * NT * 1024 : 0);
   static_assert(BM % (8 * NW) == 0 && MT % 4 == 0 && (!GATED || NW == 4), "whole copies; all columns of a scale");
+  static_assert(KG == 1 || (KG == 2 && !GATED && !DEEP), "two groups exchange sums");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW), kg = KG > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) / NW) : 0;
+  const int every = kg * NW + wave;
   const int r = lane & 15, g = lane >> 4;
   const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK, m16 = (int)fp8_scale_rows(p.M);
+  const int steps = (kbs + KG - 1) / KG, first = kg * steps;  // this group's K blocks; those past K are zeros
   const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
 
   // ---- copies of the next step: K block ckb of tile ctile.  One brings 8 rows, lane l chunk (l % 8) ^ (l / 8)
@@ -658,7 +666,7 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   // the tile's first rows, which nothing uses.  No scalar offset passes its descriptor's end (a copy of
   // weight rows past the matrix is held there): the range check may subtract it from the size.
   uint32_t ctile = blockIdx.x;
-  int ckb = 0, climit = p.K;  // climit 0: past the last tile, zeros
+  int ckb = first, climit = p.K;  // climit 0: past the last tile, zeros
   int tm, tn;                 // place of tile ctile
   i4v ra[CA], rsa, rw[NM];
   uint32_t ws[NM], wsn[NM];   // weight scales: lane k's are of K block k of a stretch of 64
@@ -687,15 +695,16 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   };
   const uint32_t fx = 16u * ((lane & 7) ^ (lane >> 3)), va = (lane >> 3) * (uint32_t)(MT * p.K) + fx;
   const uint32_t vsa = lane < BM / 4 ? 4u * lane : kOutside, vw = (lane >> 3) * (uint32_t)p.K + fx;
-  const uint32_t lds0 = lds_offset(lds);
+  const uint32_t lds0 = lds_offset(lds) + kg * GROUP;
   uint32_t cva, cvw;  // this step's lane offsets; chunks past K lie outside
   auto copy = [&](int j, uint32_t slot) {
+    const uint32_t at = KG > 1 ? __builtin_amdgcn_readfirstlane(min(ckb, kbs - 1)) : ckb;
     if (j < 8)
       lds_copy16(rw[GATED ? j / 4 : 0], cvw,
-                 min(ckb * 128u + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K, (uint32_t)rw[GATED ? j / 4 : 0][2]),
+                 min(at * 128 + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K, (uint32_t)rw[GATED ? j / 4 : 0][2]),
                  lds0 + (DEEP ? slot * STAGE : 0) + WEIGHTS + wave * 8192 + j * 1024);
-    else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, ckb * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
-    else lds_copy4(rsa, vsa, ckb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
+    else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, at * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
+    else lds_copy4(rsa, vsa, at * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
   };
   auto lane_offsets = [&]() {
     const bool in = ckb * 128 + (int)fx < climit;
@@ -708,12 +717,13 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   uint32_t sa[MT / 4];
   // lane's chunks g and g + 4 of its row
   const uint32_t place = 16 * (g ^ (r & 7));
-  uint32_t alo = r * 128 + place, ahi = r * 128 + (place ^ 64), sat = SCALES + r * MT;  // in the current step's buffer
+  uint32_t alo = kg * GROUP + r * 128 + place, ahi = kg * GROUP + r * 128 + (place ^ 64);  // in the current step's buffer
+  uint32_t sat = kg * GROUP + SCALES + r * MT;
   auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
     const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
     v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   };
-  uint32_t wat = WEIGHTS + wave * 8192 + r * 128;
+  uint32_t wat = kg * GROUP + WEIGHTS + wave * 8192 + r * 128;
   auto read_w = [&](int j) { read(wat + place + 2048 * j, wat + (place ^ 64) + 2048 * j, w[j]); };
   auto read_scales = [&]() {
 #pragma unroll
@@ -721,8 +731,8 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   };
 
   auto next_block = [&]() {
-    if (++ckb == kbs) {
-      ckb = 0;
+    if (++ckb == first + steps) {
+      ckb = first;
       ctile += gridDim.x;
       if (ctile < tiles) aim();
       else climit = 0;
@@ -733,7 +743,7 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   constexpr int IN_FLIGHT = DEEP ? OPS : 0, WAIT = (IN_FLIGHT & 15) | (IN_FLIGHT >> 4 << 14) | 0x70;
 
   aim();
-  weight_scales(tn * COLS, 0, ws);
+  weight_scales(tn * COLS, first, ws);
   int ptm = tm, ptn = tn;  // place of the tile that the products are at
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), so that the compiler knows its own loads to be complete
   lane_offsets();
@@ -756,12 +766,12 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int m0 = ptm * BM, n0 = ptn * COLS;
     if (tile + gridDim.x < tiles) tile_place(tiles, tiles_m, tiles_n, tile + gridDim.x, ptm, ptn);
-    weight_scales(ptn * COLS, 0, wsn);  // of the next tile
+    weight_scales(ptn * COLS, first, wsn);  // of the next tile
     prod.clear();
     int kb = 0;
     do {
       if (kb && (kb & 63) == 0) {
-        weight_scales(n0, kb, ws);
+        weight_scales(n0, first + kb, ws);
         __builtin_amdgcn_s_waitcnt(0x0f70);
       }
       next_block();
@@ -805,13 +815,33 @@ __global__ __launch_bounds__(64 * NW, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8Gem
       last = slot;
       slot = after;
       kb++;
-    } while (kb < kbs);
+    } while (kb < steps);
 #pragma unroll
     for (int j = 0; j < NM; j++) ws[j] = wsn[j];
     prod.fold();
 
-    if constexpr (!GATED) {
-      store_stripes<OUT, MT, NT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, prod.acc);
+    if constexpr (KG > 1) {
+      // a stripe at a time, each group gives the other the sums of a stripe that the other stores
+      f4* give = reinterpret_cast<f4*>(lds + EXCHANGE) + (every * NT) * 64 + lane;
+      const f4* take = reinterpret_cast<const f4*>(lds + EXCHANGE) + ((kg ? wave : NW + wave) * NT) * 64 + lane;
+#pragma unroll
+      for (int i = 0; i < MT / 2; i++) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) give[64 * j] = kg ? prod.acc[i][j] : prod.acc[MT / 2 + i][j];
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const f4 x = take[64 * j];
+          if (kg) prod.acc[MT / 2 + i][j] += x;
+          else prod.acc[i][j] += x;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+      uint8_t* stage = lds + REST + every * 2048;
+      if (kg) store_stripes<OUT, MT / 2, MT>(p, stage, lane, m0, n0 + wave * 64, prod.acc);
+      else store_stripes<OUT, 0, MT / 2>(p, stage, lane, m0, n0 + wave * 64, prod.acc);
+    } else if constexpr (!GATED) {
+      store_stripes<OUT, 0, MT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, prod.acc);
     } else {
       // staged in the rows' buffer that the next step's copies go to
       gated_stripes<MT>(p, reinterpret_cast<uint32_t*>(lds + REST), lds + last * STAGE, lane, wave, m0, n0, m16, prod.acc);
@@ -841,14 +871,14 @@ hipError_t launch_tile(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP>
+template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP, int KG = 1>
 hipError_t launch_strip(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   constexpr int COLS = (GATED ? 32 : 64) * NW;
   const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + COLS - 1) / COLS;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
   if (tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, DEEP>),
-             dim3((unsigned)std::min<int64_t>(tiles, cus * (DEEP ? 1 : 8 / NW))), dim3(64 * NW), 0, s, p, tiles_m, tiles_n);
+  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, DEEP, KG>),
+             dim3((unsigned)std::min<int64_t>(tiles, cus * (DEEP ? 1 : 8 / NW / KG))), dim3(64 * NW * KG), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
@@ -877,10 +907,14 @@ hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
   if (m <= 64 || t128 < 32) return launch_small<OUT, ST, 4, 2, 8>(p, s);
   const int cus = compute_units();
   if constexpr (OUT == FP8_IO_F32) {
-    // 64 x 256 strips against 64 x 128 tiles: 22.6 / 23.9 us for 4,616 x 768 x 2,048 (219 strips), 41 / 29 for
-    // 256 x 8,192 x 4,096 (128 strips)
-    if (((m + 63) / 64) * ((n + 255) / 256) < 200) return launch_tile<OUT, ST, 64, 128, 1, 4>(p, cus, s);
-    return launch_strip<OUT, ST, false, 4, 4, false>(p, cus, s);
+    // us, 64 x 128 tiles / 64 x 256 strips / strips with K halved: 28.9 / 41.2 / 33.3 for 256 x 8,192 x 4,096
+    // (128 strips), 10.9 / 10.5 / 10.3 for 1,000 x 2,304 x 768 (144), 21.5 / 21.0 / 18.2 for 2,800 x 768 x 2,048
+    // (132), 22.1 / 21.7 / 19.6 for 4,600 x 768 x 2,048 (216), 45.0 / 34.3 / 38.5 for 9,232 x 768 x 2,048 (435); with
+    // one K block halving costs 1.7
+    const int64_t strips = ((m + 63) / 64) * ((n + 255) / 256);
+    if (strips > cus) return launch_strip<OUT, ST, false, 4, 4, false>(p, cus, s);
+    if (2 * strips > cus && p.K > 5 * FP8_BLOCK) return launch_strip<OUT, ST, false, 4, 4, false, 2>(p, cus, s);
+    return launch_tile<OUT, ST, 64, 128, 1, 4>(p, cus, s);
   } else {
     // strips win once every compute unit has two: 112 against 136 us for 74,640 x 2,048 x 768, 12.4 against
     // 12.2 for 4,616 x 2,048 x 768 (296 strips), 18.7 against 11.2 for 4,616 x 768 x 2,048 (111)
