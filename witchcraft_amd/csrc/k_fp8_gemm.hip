@@ -365,6 +365,32 @@ __device__ __forceinline__ void store_stripes(const Fp8GemmArgs& p, uint8_t* sta
     }
 }
 
+// Two groups of waves have the sums of a K half each.  STEP 16 x 16 tiles at a time, each wave gives its partner
+// the sums of a stripe that the partner keeps: the first group keeps stripes 0 .. MT / 2 - 1, the second
+// the rest.  Either way a result is first half + second half (addition commutes).  give: the wave's STEP KiB
+// of LDS; take: its partner's.
+template <int STEP, int MT, int NT>
+__device__ __forceinline__ void exchange_halves(uint8_t* give, const uint8_t* take, int lane, bool second, f4 (&acc)[MT][NT]) {
+  f4* to = reinterpret_cast<f4*>(give) + lane;
+  const f4* from = reinterpret_cast<const f4*>(take) + lane;
+#pragma unroll
+  for (int i = 0; i < MT / 2; i++)
+#pragma unroll
+    for (int j = 0; j < NT; j += STEP) {
+#pragma unroll
+      for (int e = 0; e < STEP; e++) to[64 * e] = second ? acc[i][j + e] : acc[MT / 2 + i][j + e];
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+      for (int e = 0; e < STEP; e++) {
+        f4 &lo = acc[i][j + e], &hi = acc[MT / 2 + i][j + e];
+        const f4 sum = (second ? hi : lo) + from[64 * e];
+        lo = second ? lo : sum;
+        hi = second ? sum : hi;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+}
+
 // The gated product's end: a wave has MT stripes of 16 rows, 32 gate columns and the same 32 up columns
 // (n0 + 32 wave ..) of the 128 whose scale four waves share.  The rows' maxima meet in tops [16 MT][4],
 // the codes in stage [MT][16][128], from where they are stored in whole lines.
@@ -451,23 +477,26 @@ __device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, uint32_t* to
 }
 
 // OUT: the result's type; F32 results take the f16 matrix instructions (see the top of the file).
-template <int OUT, int ST, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+template <int OUT, int ST, int BM, int BN, int WM, int WN, int KG>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
   constexpr bool EXACT = OUT == FP8_IO_F32;
   constexpr int WSZ = ST == FP8_F32 ? 4 : 1;  // bytes of a weight scale
   constexpr int NW = WM * WN, MT = BM / 16 / WM, NT = BN / 16 / WN, STAGE = (BM + BN) * 128;
   constexpr int H = MT / 2;                                      // stripes of a half step
   constexpr int CA = BM / 16 / NW, CW = BN / 8 / NW;             // copies per wave: of each half of the rows, of weights
   constexpr int C1 = CA + 2 + CW;                                // with the scales': of cursor 1 together
-  constexpr int SC = 512, SCALES = 2 * STAGE, REST = SCALES + 2 * SC;  // SC: a step's scales, rows' and weights'
-  constexpr int LDS = REST + NW * 2048;
+  constexpr int SC = 512, SCALES = 2 * STAGE, GROUP = SCALES + 2 * SC;  // SC: a step's scales, rows' and weights'
+  constexpr int REST = KG * GROUP, LDS = REST + KG * NW * 2048;          // a wave's: to store from, to exchange sums
+  static_assert(KG == 1 || KG == 2, "two groups exchange sums");
   static_assert(BM % (16 * NW) == 0 && BN % (8 * NW) == 0 && MT % 4 == 0 && BM <= 256, "whole copies, whole scale dwords");
   static_assert(BN <= FP8_BLOCK && FP8_BLOCK % BN == 0, "one weight scale per tile and K block");
   constexpr int PS = Products<EXACT, ST, MT, NT>::SLOTS;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW), kg = KG > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) / NW) : 0;
   const int r = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
   const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK, m16 = (int)fp8_scale_rows(p.M);
+  const int steps = (kbs + KG - 1) / KG, first = kg * steps;  // this group's K blocks; those past K are zeros
   const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
 
   // ---- copies.  One brings K block kb of 8 rows: lane l chunk (l % 8) ^ (l / 8) of its row l / 8, to place
@@ -478,7 +507,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
     uint32_t tile;
     int kb, limit;  // limit: K, or 0 past the last tile (zeros)
   };
-  Cursor c1 = {blockIdx.x, 0, p.K}, c2 = c1;  // of weights and the first stripes, of the last stripes
+  Cursor c1 = {blockIdx.x, first, p.K}, c2 = c1;  // of weights and the first stripes, of the last stripes
   i4v rw[CW], ra[2][CA], rsa, rsw;
   auto row_buffer = [&](const uint8_t* base, int first, int row, int end, int rows) {
     if (first + row >= end) row = 0;
@@ -510,8 +539,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
     aim_rows(1, tm * BM);
   };
   auto advance = [&](Cursor& c, auto aim) {
-    if (++c.kb < kbs) return;
-    c.kb = 0;
+    if (++c.kb < first + steps) return;
+    c.kb = first;
     c.tile += gridDim.x;
     if (c.tile < tiles) aim();
     else c.limit = 0;
@@ -519,18 +548,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
   const uint32_t fx = 16u * ((lane & 7) ^ (lane >> 3)), vw = (lane >> 3) * (uint32_t)p.K + fx;
   const uint32_t va = (lane >> 3) * (uint32_t)(MT * p.K) + fx, vsc = lane < BM / 4 ? 4u * lane : kOutside;
   const uint32_t vws = lane == 0 ? 0 : kOutside;
-  const uint32_t lds0 = lds_offset(lds);
+  const uint32_t lds0 = lds_offset(lds) + kg * GROUP;
+  auto within = [&](int kb) -> uint32_t { return KG > 1 ? __builtin_amdgcn_readfirstlane(min(kb, kbs - 1)) : kb; };
   // copy j of what cursor 1 brings: the first half of the rows, the scales, the weights
   auto copy1 = [&](int j, uint32_t slot) {
     const bool in = c1.kb * 128 + (int)fx < c1.limit;
-    if (j < CA) lds_copy16(ra[0][j], in ? va : kOutside, c1.kb * 128, lds0 + slot * STAGE + (wave * CA + j) * 1024);
-    else if (j == CA) lds_copy4(rsa, vsc, c1.kb * (uint32_t)m16, lds0 + SCALES + SC * slot);  // the same by every wave
-    else if (j == CA + 1) lds_copy_scale<ST>(rsw, vws, c1.kb * WSZ, lds0 + SCALES + SC * slot + 256);
-    else lds_copy16(rw[j - CA - 2], in ? vw : kOutside, c1.kb * 128, lds0 + slot * STAGE + BM * 128 + (wave * CW + j - CA - 2) * 1024);
+    const uint32_t at = within(c1.kb);
+    if (j < CA) lds_copy16(ra[0][j], in ? va : kOutside, at * 128, lds0 + slot * STAGE + (wave * CA + j) * 1024);
+    else if (j == CA) lds_copy4(rsa, vsc, at * (uint32_t)m16, lds0 + SCALES + SC * slot);  // the same by every wave
+    else if (j == CA + 1) lds_copy_scale<ST>(rsw, vws, at * WSZ, lds0 + SCALES + SC * slot + 256);
+    else lds_copy16(rw[j - CA - 2], in ? vw : kOutside, at * 128, lds0 + slot * STAGE + BM * 128 + (wave * CW + j - CA - 2) * 1024);
   };
   auto copy2 = [&](int j, uint32_t slot) {
     const bool in = c2.kb * 128 + (int)fx < c2.limit;
-    lds_copy16(ra[1][j], in ? va : kOutside, c2.kb * 128, lds0 + slot * STAGE + ((NW + wave) * CA + j) * 1024);
+    lds_copy16(ra[1][j], in ? va : kOutside, within(c2.kb) * 128, lds0 + slot * STAGE + ((NW + wave) * CA + j) * 1024);
   };
   // All copies but the newest CA + C1 (one step's) have landed, and this wave's reads are complete.
   auto arrive = [&]() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(CA + C1) : "memory"); };
@@ -541,8 +572,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
   // lane's chunks g and g + 4 of its row: places (g ^ f) and (g ^ f) ^ 4
   const int arow = wm * 16 * MT + r * MT, wrow = wn * 16 * NT + r;
   const uint32_t place = 16 * (g ^ (r & 7));
-  uint32_t alo = (wm * 16 + r) * 128 + place, ahi = (wm * 16 + r) * 128 + (place ^ 64);  // in the current step's buffer
-  uint32_t wlo = (BM + wrow) * 128 + place, whi = (BM + wrow) * 128 + (place ^ 64), sat = SCALES + arow, swat = SCALES + 256;
+  const uint32_t mine = kg * GROUP;
+  uint32_t alo = mine + (wm * 16 + r) * 128 + place, ahi = mine + (wm * 16 + r) * 128 + (place ^ 64);  // in the current step's buffer
+  uint32_t wlo = mine + (BM + wrow) * 128 + place, whi = mine + (BM + wrow) * 128 + (place ^ 64);
+  uint32_t sat = mine + SCALES + arow, swat = mine + SCALES + 256;
   auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
     const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
     v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -622,9 +655,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
       }
       slot ^= 1;
       kb++;
-    } while (kb < kbs);
+    } while (kb < steps);
     prod.fold();
-    store_stripes<OUT, 0, MT>(p, lds + REST + wave * 2048, lane, m0 + wm * 16 * MT, n0 + wn * NT * 16, prod.acc);
+    uint8_t* stage = lds + REST + (kg * NW + wave) * 2048;
+    const int ms = m0 + wm * 16 * MT, ns = n0 + wn * NT * 16;
+    if constexpr (KG == 1) {
+      store_stripes<OUT, 0, MT>(p, stage, lane, ms, ns, prod.acc);
+    } else {
+      exchange_halves<2>(stage, lds + REST + ((kg ? 0 : NW) + wave) * 2048, lane, kg, prod.acc);
+      if (kg) store_stripes<OUT, MT / 2, MT>(p, stage, lane, ms, ns, prod.acc);
+      else store_stripes<OUT, 0, MT / 2>(p, stage, lane, ms, ns, prod.acc);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
 }
@@ -821,22 +862,8 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
     prod.fold();
 
     if constexpr (KG > 1) {
-      // a stripe at a time, each group gives the other the sums of a stripe that the other stores
-      f4* give = reinterpret_cast<f4*>(lds + EXCHANGE) + (every * NT) * 64 + lane;
-      const f4* take = reinterpret_cast<const f4*>(lds + EXCHANGE) + ((kg ? wave : NW + wave) * NT) * 64 + lane;
-#pragma unroll
-      for (int i = 0; i < MT / 2; i++) {
-#pragma unroll
-        for (int j = 0; j < NT; j++) give[64 * j] = kg ? prod.acc[i][j] : prod.acc[MT / 2 + i][j];
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-          const f4 x = take[64 * j];
-          if (kg) prod.acc[MT / 2 + i][j] += x;
-          else prod.acc[i][j] += x;
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      }
+      uint8_t* ex = lds + EXCHANGE;
+      exchange_halves<NT>(ex + every * NT * 1024, ex + (kg ? wave : NW + wave) * NT * 1024, lane, kg, prod.acc);
       uint8_t* stage = lds + REST + every * 2048;
       if (kg) store_stripes<OUT, MT / 2, MT>(p, stage, lane, m0, n0 + wave * 64, prod.acc);
       else store_stripes<OUT, 0, MT / 2>(p, stage, lane, m0, n0 + wave * 64, prod.acc);
@@ -861,13 +888,14 @@ hipError_t launch_small(const Fp8GemmArgs& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int OUT, int ST, int BM, int BN, int WM, int WN>
+template <int OUT, int ST, int BM, int BN, int WM, int WN, int KG = 1>
 hipError_t launch_tile(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
   if (tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_tile_kernel<OUT, ST, BM, BN, WM, WN>), dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / (WM * WN)))),
-             dim3(64 * WM * WN), 0, s, p, tiles_m, tiles_n);
+  T5K_LAUNCH((fp8_tile_kernel<OUT, ST, BM, BN, WM, WN, KG>),
+             dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / (WM * WN * KG)))), dim3(64 * WM * WN * KG), 0, s, p, tiles_m,
+             tiles_n);
   return hipGetLastError();
 }
 
@@ -893,40 +921,45 @@ int compute_units() {
   return cus;
 }
 
-// Few tiles: operands straight to the waves, K dealt out over the waves of a workgroup, as many 16 x 16
-// tiles per workgroup as leave about a workgroup or two per compute unit (us, 32 x 2,304 x 768 / 64 x 768 x
-// 2,048 / 64 x 2,304 x 768 / 64 x 8,192 x 4,096: 1 x 1 tiles 3.8 / 4.3 / 4.6 / 31.6, 1 x 2 3.6 / 5.2 / 4.6 /
-// 24.7, 2 x 2 4.2 / 6.4 / 4.2 / 17.4, 4 x 2 4.5 / 8.4 / 5.1 / 14.8, LDS tiles of 128 x 128 5.9 / 10.1 / 6.1 /
-// 17.1).  Then LDS tiles, where they are enough to fill half of the chip or have the rows.
+// Few tiles: operands straight to the waves, K dealt out over the waves of a workgroup, with the smallest tiles
+// that leave a workgroup per compute unit.  Twice as many still win for one row of them (us, 1 x 16,384 x 4,096: 1 x 2
+// tiles of 16 14.5, LDS tiles 17.3), and for f32 results, whose LDS tiles are slower (32 x 16,384 x 4,096: 18.1 / 23.2);
+// past that LDS tiles do (64 x 32,768 x 4,096: 48 / 22).  us of 1 x 1, 1 x 2, 2 x 2, 4 x 2 and LDS tiles in bf16: 3.8,
+// 3.6, 4.2, 4.5, 6.0 for 32 x 2,304 x 768; 4.2, 5.2, 6.6, 8.3, 10.0 for 64 x 768 x 2,048; 4.5, 4.6, 4.2, 5.0, 6.1 for 64 x
+// 2,304 x 768; 32, 25, 20, 14.9, 17.6 for 64 x 8,192 x 4,096.
 template <int OUT, int ST>
 hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
-  const int64_t m = p.M, n = p.N, t16 = ((m + 15) / 16) * ((n + 15) / 16), t128 = ((m + 127) / 128) * ((n + 127) / 128);
-  if (t16 <= 256) return launch_small<OUT, ST, 1, 1, 8>(p, s);
-  if (t16 <= 512) return launch_small<OUT, ST, 1, 2, 8>(p, s);
-  if (t16 <= 1024) return launch_small<OUT, ST, 2, 2, 4>(p, s);
-  if (m <= 64 || t128 < 32) return launch_small<OUT, ST, 4, 2, 8>(p, s);
   const int cus = compute_units();
+  auto groups = [&](int rows, int cols) { return (((int64_t)p.M + rows - 1) / rows) * (((int64_t)p.N + cols - 1) / cols); };
+  if (groups(16, 16) <= cus) return launch_small<OUT, ST, 1, 1, 8>(p, s);
+  if (groups(16, 32) <= (p.M <= 16 ? 2 * cus : cus)) return launch_small<OUT, ST, 1, 2, 8>(p, s);
+  if (groups(32, 32) <= cus) return launch_small<OUT, ST, 2, 2, 4>(p, s);
+  if (groups(64, 32) <= cus) return launch_small<OUT, ST, 4, 2, 8>(p, s);
   if constexpr (OUT == FP8_IO_F32) {
-    // us, 64 x 128 tiles / 64 x 256 strips / strips with K halved: 28.9 / 41.2 / 33.3 for 256 x 8,192 x 4,096
-    // (128 strips), 10.9 / 10.5 / 10.3 for 1,000 x 2,304 x 768 (144), 21.5 / 21.0 / 18.2 for 2,800 x 768 x 2,048
-    // (132), 22.1 / 21.7 / 19.6 for 4,600 x 768 x 2,048 (216), 45.0 / 34.3 / 38.5 for 9,232 x 768 x 2,048 (435); with
-    // one K block halving costs 1.7
-    const int64_t strips = ((m + 63) / 64) * ((n + 255) / 256);
-    if (strips > cus) return launch_strip<OUT, ST, false, 4, 4, false>(p, cus, s);
-    if (2 * strips > cus && p.K > 5 * FP8_BLOCK) return launch_strip<OUT, ST, false, 4, 4, false, 2>(p, cus, s);
-    return launch_tile<OUT, ST, 64, 128, 1, 4>(p, cus, s);
+    if (groups(32, 32) <= 2 * cus) return launch_small<OUT, ST, 2, 2, 4>(p, s);
+    // us, tiles of 64 x 128 / strips of 64 x 256, and each with K halved: 27.4, 22.7 / -, 29.2 for 256 x 2,048 x 4,096 (64
+    // tiles), 15.6, 13.9 / -, 17.3 for 1,000 x 768 x 2,048 (96), 21.5, - / 21.0, 18.2 for 2,800 x 768 x 2,048 (132 strips),
+    // 22.1, 25.8 / 21.7, 19.6 for 4,600 x 768 x 2,048 (216), 45.0, - / 34.3, 38.5 for 9,232 x 768 x 2,048 (435); halving costs
+    // as much as it gives at K = 768 and 1.5 us at one block.
+    const bool halve = p.K >= 8 * FP8_BLOCK;
+    if (groups(64, 256) > cus) return launch_strip<OUT, ST, false, 4, 4, false>(p, cus, s);
+    if (!halve) return launch_tile<OUT, ST, 64, 128, 1, 4>(p, cus, s);
+    if (groups(64, 128) <= cus) return launch_tile<OUT, ST, 64, 128, 1, 4, 2>(p, cus, s);
+    return launch_strip<OUT, ST, false, 4, 4, false, 2>(p, cus, s);
   } else {
-    // strips win once every compute unit has two: 112 against 136 us for 74,640 x 2,048 x 768, 12.4 against
-    // 12.2 for 4,616 x 2,048 x 768 (296 strips), 18.7 against 11.2 for 4,616 x 768 x 2,048 (111)
-    if (((m + 127) / 128) * ((n + 255) / 256) >= 2 * cus) return launch_strip<OUT, ST, false, 8, 4, false>(p, cus, s);
+    // strips win once every compute unit has two: 113 against 139 us for 74,640 x 2,048 x 768, 12.6 against 12.5
+    // for 4,616 x 2,048 x 768 (296 strips), 18.8 against 11.3 for 4,616 x 768 x 2,048 (111)
+    if (groups(128, 256) >= 2 * cus) return launch_strip<OUT, ST, false, 8, 4, false>(p, cus, s);
     return launch_tile<OUT, ST, 128, 128, 2, 2>(p, cus, s);
   }
 }
 
 // A scale needs all of its 128 columns in one workgroup.  Up to one strip per compute unit the ring of three
-// K blocks is faster (256 x 8,192 x 4,096, 256 strips of 64 rows: 23 against 32 us; 4,616 x 768 x 2,048, 222 of
-// 128 rows: 18.5 against 21.8), beyond that two workgroups on a compute unit (4,616 x 2,048 x 768: 22 against
-// 27).
+// K blocks is faster (256 x 8,192 x 4,096, 256 strips of 64 rows: 24 against 36 us; 4,616 x 768 x 2,048, 222 of
+// 128 rows: 18 against 21), beyond that two workgroups on a compute unit (4,616 x 2,048 x 768: 21 against
+// 26; strips of 64 rows 23).  For few rows that leaves most compute units without work, and a strip's time is that of its
+// weights through one of them (7 us for 32 x 2,048 x 768, 16 strips); operands straight to registers, 16 rows a
+// workgroup, took 9.
 template <int ST>
 hipError_t launch_gated(const Fp8GemmArgs& p, hipStream_t s) {
   const int cus = compute_units();
