@@ -596,15 +596,15 @@ def test_gated_ordinary(fp8, M, N, K, scale):
 
 
 @pytest.mark.parametrize("scale", [E8M0, F32S])
-@pytest.mark.parametrize("M,N,K", [(70, 400, 8336), (1100, 1040, 400), (2100, 1040, 8336), (2100, 1936, 400),
+@pytest.mark.parametrize("M,N,K", [(70, 400, 8336), (700, 1424, 400), (700, 1440, 8336), (1100, 1040, 400), (2100, 1040, 8336), (2100, 1936, 400),
                                    (2100, 2064, 272), (4200, 1040, 8336), (8201, 1040, 144), (33000, 272, 16)])
 def test_gated_variants(fp8, M, N, K, scale):
-    """Both sides of the borders at one strip of 64 and of 128 rows per compute unit, several tiles per
+    """Both sides of the borders at one strip of 32, 64 and of 128 rows per compute unit, several tiles per
     workgroup, more than 64 K blocks."""
     test_gated_exact_products(fp8, M, N, K, scale)
 
 
-@pytest.mark.parametrize("M,N", [(70, 272), (2100, 1040), (4200, 1040)])
+@pytest.mark.parametrize("M,N", [(70, 272), (1100, 1040), (2100, 1040), (4200, 1040)])
 def test_gated_infinite_products(fp8, M, N):
     """A product past f32's range has a NaN code and does not count towards its block's scale; huge finite
     ones do, and a gate of -2^64 closes to -0."""

@@ -441,7 +441,7 @@ __device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, uint32_t* to
   uint8_t* to[2];
 #pragma unroll
   for (int j = 0; j < 2; j++) to[j] = stage + r * 128 + 16 * ((2 * wave + j) ^ (r & 7)) + 4 * g;  // 16-byte piece 2 wave + j
-  uint32_t bytes[MT / 4] = {};
+  uint32_t bytes[(MT + 3) / 4] = {};
 #pragma unroll
   for (int i = 0; i < MT; i++) {
     const uint4 t4 = *reinterpret_cast<const uint4*>(trow + 64 * i);
@@ -454,7 +454,7 @@ __device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, uint32_t* to
   if (wave == 0 && g == 0) {
     const int m = m0 + r * MT;
     uint8_t* scales = p.out_scales + (size_t)(n0 / FP8_BLOCK) * m16 + m;
-    if (m + MT <= p.M) {
+    if (MT % 4 == 0 && m + MT <= p.M) {
 #pragma unroll
       for (int c = 0; c < MT / 4; c++) reinterpret_cast<uint32_t*>(scales)[c] = bytes[c];
     } else {
@@ -675,23 +675,23 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
 // columns).  Rows' codes are double-buffered in LDS; the weights have one buffer, a wave's own share:
 // their operands are in registers from a step's start, when the next step's are requested.  The two
 // workgroups run apart, so that one's results are formed and stored behind the other's products.
-// DEEP, for launches that leave each compute unit one workgroup: a ring of three K blocks, weights and
-// rows, two of them on their way.  KG = 2, for f32 results of such launches: a second group of waves takes
+// RING, for launches that leave each compute unit one workgroup: a ring of that many K blocks, weights and
+// rows, all but one of them on their way.  KG = 2, for f32 results of such launches: a second group of waves takes
 // the second half of the K blocks, so that each SIMD still has two waves (the vector unit widens for one
 // while the matrix unit works for the other), and the two exchange sums at the end; the halves are
 // always added in the same order, first and second (addition commutes).
-template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP, int KG>
-__global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+template <int OUT, int ST, bool GATED, int MT, int NW, int RING, int KG>
+__global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
   constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
   constexpr int NT = 4, BM = 16 * MT, NM = GATED ? 2 : 1;                     // NM: matrices
-  constexpr int STAGES = DEEP ? 3 : 2, STAGE = BM * 128 + (DEEP ? NW * 8192 : 0);
+  constexpr int STAGES = RING ? RING : 2, STAGE = BM * 128 + (RING ? NW * 8192 : 0);
   constexpr int COLS = (GATED ? 32 : 64) * NW, CA = BM / 8 / NW;              // CA: copies of rows per wave and K block
-  constexpr int WEIGHTS = DEEP ? BM * 128 : 2 * STAGE;  // DEEP: within a stage
-  constexpr int SCALES = STAGES * STAGE + (DEEP ? 0 : NW * 8192), GROUP = SCALES + STAGES * 256, OPS = 9 + CA;
+  constexpr int WEIGHTS = RING ? BM * 128 : 2 * STAGE;  // RING: within a stage
+  constexpr int SCALES = STAGES * STAGE + (RING ? 0 : NW * 8192), GROUP = SCALES + STAGES * 256, OPS = 9 + CA;
   constexpr int REST = KG * GROUP, EXCHANGE = REST + KG * NW * 2048;
   constexpr int LDS = GATED ? REST + NW * BM * 4 : EXCHANGE + (KG > 1 ? KG * NW * NT * 1024 : 0);
-  static_assert(BM % (8 * NW) == 0 && MT % 4 == 0 && (!GATED || NW == 4), "whole copies; all columns of a scale");
-  static_assert(KG == 1 || (KG == 2 && !GATED && !DEEP), "two groups exchange sums");
+  static_assert(BM % (8 * NW) == 0 && (MT % 4 == 0 || MT == 2) && (!GATED || NW == 4), "whole copies; all columns of a scale");
+  static_assert(KG == 1 || (KG == 2 && !GATED && !RING), "two groups exchange sums");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW), kg = KG > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) / NW) : 0;
@@ -743,7 +743,7 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
     if (j < 8)
       lds_copy16(rw[GATED ? j / 4 : 0], cvw,
                  min(at * 128 + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K, (uint32_t)rw[GATED ? j / 4 : 0][2]),
-                 lds0 + (DEEP ? slot * STAGE : 0) + WEIGHTS + wave * 8192 + j * 1024);
+                 lds0 + (RING ? slot * STAGE : 0) + WEIGHTS + wave * 8192 + j * 1024);
     else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, at * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
     else lds_copy4(rsa, vsa, at * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
   };
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
 
   Products<EXACT, ST, MT, NT> prod;
   i8v a[2], w[NT];
-  uint32_t sa[MT / 4];
+  uint32_t sa[(MT + 3) / 4];
   // lane's chunks g and g + 4 of its row
   const uint32_t place = 16 * (g ^ (r & 7));
   uint32_t alo = kg * GROUP + r * 128 + place, ahi = kg * GROUP + r * 128 + (place ^ 64);  // in the current step's buffer
@@ -767,6 +767,7 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
   uint32_t wat = kg * GROUP + WEIGHTS + wave * 8192 + r * 128;
   auto read_w = [&](int j) { read(wat + place + 2048 * j, wat + (place ^ 64) + 2048 * j, w[j]); };
   auto read_scales = [&]() {
+    if constexpr (MT == 2) sa[0] = *reinterpret_cast<const uint16_t*>(lds + sat);
 #pragma unroll
     for (int c = 0; c < MT / 4; c++) sa[c] = *reinterpret_cast<const uint32_t*>(lds + sat + 4 * c);
   };
@@ -780,8 +781,8 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
     }
     lane_offsets();
   };
-  // the newest OPS copies may be on their way (DEEP: the step after next's); reads are complete
-  constexpr int IN_FLIGHT = DEEP ? OPS : 0, WAIT = (IN_FLIGHT & 15) | (IN_FLIGHT >> 4 << 14) | 0x70;
+  // the next step's copies have landed, those of the steps after it (RING) may be on their way; reads are complete
+  constexpr int IN_FLIGHT = (STAGES - 2) * OPS, WAIT = (IN_FLIGHT & 15) | (IN_FLIGHT >> 4 << 14) | 0x70;
 
   aim();
   weight_scales(tn * COLS, first, ws);
@@ -790,10 +791,11 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
   lane_offsets();
 #pragma unroll
   for (int j = 0; j < OPS; j++) copy(j, 0);
-  if constexpr (DEEP) {
+#pragma unroll
+  for (int n = 1; n < STAGES - 1; n++) {
     next_block();
 #pragma unroll
-    for (int j = 0; j < OPS; j++) copy(j, 1);
+    for (int j = 0; j < OPS; j++) copy(j, n);
   }
   __builtin_amdgcn_s_waitcnt(WAIT);
   asm volatile("s_barrier" ::: "memory");
@@ -816,7 +818,7 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
         __builtin_amdgcn_s_waitcnt(0x0f70);
       }
       next_block();
-      const uint32_t fill = DEEP ? (slot == 0 ? 2 : slot - 1) : slot ^ 1, after = DEEP ? (slot == 2 ? 0 : slot + 1) : slot ^ 1;
+      const uint32_t fill = slot == 0 ? STAGES - 1 : slot - 1, after = slot == STAGES - 1 ? 0 : slot + 1;
       uint32_t swb[NM];
 #pragma unroll
       for (int j = 0; j < NM; j++) swb[j] = __builtin_amdgcn_readlane(ws[j], kb & 63);
@@ -832,7 +834,7 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
           asm volatile("s_barrier" ::: "memory");
           const uint32_t step = after == 0 ? (uint32_t)-((STAGES - 1) * STAGE) : (uint32_t)STAGE;
           alo += step, ahi += step, sat += after == 0 ? -(STAGES - 1) * 256 : 256;
-          if (DEEP) wat += step;
+          if (RING) wat += step;
           read_scales();
           read(alo, ahi, a[0]);
         }
@@ -843,7 +845,7 @@ __global__ __launch_bounds__(64 * NW * KG, DEEP ? 1 : 2) void fp8_strip_kernel(F
           __builtin_amdgcn_sched_barrier(0);
           if (i == MT - 1) read_w(x);  // each weight operand is replaced as soon as it has been used
           // Behind the products: the next step's weights, whose buffer has been read, and rows.
-          constexpr int PARTS = (MT - 2) * 4;
+          constexpr int PARTS = (MT > 2 ? MT - 2 : 1) * 4;
           const int at = i * 4 + x;
           if (at == 0) __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): w is in registers
           if (at < PARTS) {
@@ -899,14 +901,14 @@ hipError_t launch_tile(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int OUT, int ST, bool GATED, int MT, int NW, bool DEEP, int KG = 1>
+template <int OUT, int ST, bool GATED, int MT, int NW, int RING, int KG = 1>
 hipError_t launch_strip(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   constexpr int COLS = (GATED ? 32 : 64) * NW;
   const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + COLS - 1) / COLS;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
   if (tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, DEEP, KG>),
-             dim3((unsigned)std::min<int64_t>(tiles, cus * (DEEP ? 1 : 8 / NW / KG))), dim3(64 * NW * KG), 0, s, p, tiles_m, tiles_n);
+  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, RING, KG>),
+             dim3((unsigned)std::min<int64_t>(tiles, cus * (RING ? 1 : 8 / NW / KG))), dim3(64 * NW * KG), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
@@ -942,31 +944,32 @@ hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
     // 22.1, 25.8 / 21.7, 19.6 for 4,600 x 768 x 2,048 (216), 45.0, - / 34.3, 38.5 for 9,232 x 768 x 2,048 (435); halving costs
     // as much as it gives at K = 768 and 1.5 us at one block.
     const bool halve = p.K >= 8 * FP8_BLOCK;
-    if (groups(64, 256) > cus) return launch_strip<OUT, ST, false, 4, 4, false>(p, cus, s);
+    if (groups(64, 256) > cus) return launch_strip<OUT, ST, false, 4, 4, 0>(p, cus, s);
     if (!halve) return launch_tile<OUT, ST, 64, 128, 1, 4>(p, cus, s);
     if (groups(64, 128) <= cus) return launch_tile<OUT, ST, 64, 128, 1, 4, 2>(p, cus, s);
-    return launch_strip<OUT, ST, false, 4, 4, false, 2>(p, cus, s);
+    return launch_strip<OUT, ST, false, 4, 4, 0, 2>(p, cus, s);
   } else {
     // strips win once every compute unit has two: 113 against 139 us for 74,640 x 2,048 x 768, 12.6 against 12.5
     // for 4,616 x 2,048 x 768 (296 strips), 18.8 against 11.3 for 4,616 x 768 x 2,048 (111)
-    if (groups(128, 256) >= 2 * cus) return launch_strip<OUT, ST, false, 8, 4, false>(p, cus, s);
+    if (groups(128, 256) >= 2 * cus) return launch_strip<OUT, ST, false, 8, 4, 0>(p, cus, s);
     return launch_tile<OUT, ST, 128, 128, 2, 2>(p, cus, s);
   }
 }
 
-// A scale needs all of its 128 columns in one workgroup.  Up to one strip per compute unit the ring of three
-// K blocks is faster (256 x 8,192 x 4,096, 256 strips of 64 rows: 24 against 36 us; 4,616 x 768 x 2,048, 222 of
-// 128 rows: 18 against 21), beyond that two workgroups on a compute unit (4,616 x 2,048 x 768: 21 against
-// 26; strips of 64 rows 23).  For few rows that leaves most compute units without work, and a strip's time is that of its
-// weights through one of them (7 us for 32 x 2,048 x 768, 16 strips); operands straight to registers, 16 rows a
-// workgroup, took 9.
+// A scale needs all of its 128 columns in one workgroup.  Up to one strip per compute unit, as few rows each as that
+// allows, and the ring of three K blocks: us of 32 / 64 rows in the ring / 128 in the ring / 128 without, 6.2 / 7.3 / - / 9.4
+// for 32 x 2,048 x 768, 18.9 / 21.6 / - / 35 for 64 x 8,192 x 4,096, - / 24 / 32 / 36 for 256 x 8,192 x 4,096 (256 strips of
+// 64), - / - / 18 / 21 for 4,616 x 768 x 2,048 (222 of 128).  Beyond that two workgroups on a compute unit: 26 / 21 for 4,616 x
+// 2,048 x 768, where strips of 64 rows take 23.  Few rows leave most compute units without work, and a strip's time is
+// that of its weights through one of them; a ring of four is no faster (6.3), operands straight to registers take 9.0.
 template <int ST>
 hipError_t launch_gated(const Fp8GemmArgs& p, hipStream_t s) {
   const int cus = compute_units();
-  const int64_t blocks = (p.N + 127) / 128, t4 = (int64_t)((p.M + 63) / 64) * blocks, t8 = (int64_t)((p.M + 127) / 128) * blocks;
-  if (t4 <= cus) return launch_strip<FP8_IO_NONE, ST, true, 4, 4, true>(p, cus, s);
-  if (t8 <= cus) return launch_strip<FP8_IO_NONE, ST, true, 8, 4, true>(p, cus, s);
-  return launch_strip<FP8_IO_NONE, ST, true, 8, 4, false>(p, cus, s);
+  auto strips = [&](int rows) { return (((int64_t)p.M + rows - 1) / rows) * ((p.N + FP8_BLOCK - 1) / FP8_BLOCK); };
+  if (strips(32) <= cus) return launch_strip<FP8_IO_NONE, ST, true, 2, 4, 3>(p, cus, s);
+  if (strips(64) <= cus) return launch_strip<FP8_IO_NONE, ST, true, 4, 4, 3>(p, cus, s);
+  if (strips(128) <= cus) return launch_strip<FP8_IO_NONE, ST, true, 8, 4, 3>(p, cus, s);
+  return launch_strip<FP8_IO_NONE, ST, true, 8, 4, 0>(p, cus, s);
 }
 }  // namespace
 
