@@ -352,9 +352,10 @@ def test_matmul_exact(fp8, M, N, K, scale):
 VARIANTS = [
     (16, 4096, 144), (16, 4100, 144), (15, 8192, 256), (16, 8200, 128), (13, 16384, 128), (16, 16400, 272),
     (17, 4096, 400), (32, 8192, 144), (31, 8200, 272), (32, 16384, 144), (33, 16390, 128), (64, 8192, 400),
-    (64, 16390, 144), (65, 4000, 400), (65, 4100, 400), (65, 4100, 1040), (70, 5001, 8336), (513, 2048, 1024),
-    (8199, 1100, 272), (8201, 2055, 144), (2817, 770, 1008), (4099, 1024, 1024), (2050, 1030, 16400), (3330, 772, 640),
-    (4161, 1027, 8336), (8201, 2056, 8336), (16413, 1027, 272), (16413, 1032, 16), (33000, 515, 384),
+    (64, 16390, 144), (65, 4100, 1040), (70, 5001, 8336), (512, 2048, 400), (513, 2041, 272), (512, 2000, 8336),
+    (1024, 2048, 144), (1024, 2041, 8336), (1025, 2048, 272), (1100, 1600, 8336), (2048, 2048, 144), (2030, 2041, 8336),
+    (2049, 2048, 400), (3000, 2041, 8336), (4096, 2041, 144), (4097, 2048, 272), (6144, 2041, 272), (6145, 2048, 144),
+    (6150, 2041, 8336), (16413, 1027, 272), (16413, 1032, 16), (33000, 515, 384), (1500, 770, 16400),
 ]
 
 

@@ -228,7 +228,7 @@ __device__ __forceinline__ f4 scaled_mfma(const i8v& w, const i8v& a, f4 c, uint
   }
 }
 
-// The products of a wave's stripe of 16 rows with its NT weight operands, in SLOTS parts, so that a
+// The products of a wave's stripe of 16 rows with its NT weight operands, in four parts, so that a
 // caller can put its copies and reads between them.  With byte scales on both sides the instruction adds
 // into the accumulators.  Otherwise a block's sums are multiplied by their scale on the vector unit: a
 // stripe behind, so that the wave never waits for the sums that it has just asked for.  `fold` adds the
@@ -236,7 +236,6 @@ __device__ __forceinline__ f4 scaled_mfma(const i8v& w, const i8v& a, f4 c, uint
 template <bool EXACT, int ST, int MT, int NT>
 struct Products {
   static constexpr bool DIRECT = !EXACT && ST == FP8_E8M0;
-  static constexpr int SLOTS = EXACT ? 4 : NT;
   f4 acc[MT][NT];
   f4 sums[DIRECT ? 1 : 2][DIRECT ? 1 : NT];
   float factor[DIRECT ? 1 : 2][DIRECT ? 1 : NT];
@@ -325,14 +324,14 @@ __device__ __forceinline__ void tile_place(uint32_t tiles, int tiles_m, int tile
 // time, 16-byte pieces rotated by the row) and stored in whole lines, past the caches: 64-byte pieces
 // straight from registers took 151 us instead of 114 for 74,640 x 2,048 (x 768) in bf16, whole lines
 // without the non-temporal hint 141.  Rows of C that do not keep 16-byte alignment go value by value.
-template <int OUT, int FROM, int TO, int MT, int NT>
+template <int OUT, int MT, int NT>
 __device__ __forceinline__ void store_stripes(const Fp8GemmArgs& p, uint8_t* stage, int lane, int m0, int n0,
                                               const f4 (&v)[MT][NT]) {
   constexpr int SZ = OUT == FP8_IO_F32 ? 4 : 2, TJ = 8 / SZ;  // TJ: columns / 16 of 128 bytes
   static_assert(NT % TJ == 0, "whole lines");
   const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int i = FROM; i < TO; i++)
+  for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int h = 0; h < NT / TJ; h++) {
 #pragma unroll
@@ -362,32 +361,6 @@ __device__ __forceinline__ void store_stripes(const Fp8GemmArgs& p, uint8_t* sta
           }
         }
       }
-    }
-}
-
-// Two groups of waves have the sums of a K half each.  STEP 16 x 16 tiles at a time, each wave gives its partner
-// the sums of a stripe that the partner keeps: the first group keeps stripes 0 .. MT / 2 - 1, the second
-// the rest.  Either way a result is first half + second half (addition commutes).  give: the wave's STEP KiB
-// of LDS; take: its partner's.
-template <int STEP, int MT, int NT>
-__device__ __forceinline__ void exchange_halves(uint8_t* give, const uint8_t* take, int lane, bool second, f4 (&acc)[MT][NT]) {
-  f4* to = reinterpret_cast<f4*>(give) + lane;
-  const f4* from = reinterpret_cast<const f4*>(take) + lane;
-#pragma unroll
-  for (int i = 0; i < MT / 2; i++)
-#pragma unroll
-    for (int j = 0; j < NT; j += STEP) {
-#pragma unroll
-      for (int e = 0; e < STEP; e++) to[64 * e] = second ? acc[i][j + e] : acc[MT / 2 + i][j + e];
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-      for (int e = 0; e < STEP; e++) {
-        f4 &lo = acc[i][j + e], &hi = acc[MT / 2 + i][j + e];
-        const f4 sum = (second ? hi : lo) + from[64 * e];
-        lo = second ? lo : sum;
-        hi = second ? sum : hi;
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 }
 
@@ -476,27 +449,21 @@ __device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, uint32_t* to
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // stage is copied into again
 }
 
-// OUT: the result's type; F32 results take the f16 matrix instructions (see the top of the file).
-template <int OUT, int ST, int BM, int BN, int WM, int WN, int KG>
-__global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
-  constexpr bool EXACT = OUT == FP8_IO_F32;
+template <int OUT, int ST, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
   constexpr int WSZ = ST == FP8_F32 ? 4 : 1;  // bytes of a weight scale
   constexpr int NW = WM * WN, MT = BM / 16 / WM, NT = BN / 16 / WN, STAGE = (BM + BN) * 128;
   constexpr int H = MT / 2;                                      // stripes of a half step
   constexpr int CA = BM / 16 / NW, CW = BN / 8 / NW;             // copies per wave: of each half of the rows, of weights
   constexpr int C1 = CA + 2 + CW;                                // with the scales': of cursor 1 together
-  constexpr int SC = 512, SCALES = 2 * STAGE, GROUP = SCALES + 2 * SC;  // SC: a step's scales, rows' and weights'
-  constexpr int REST = KG * GROUP, LDS = REST + KG * NW * 2048;          // a wave's: to store from, to exchange sums
-  static_assert(KG == 1 || KG == 2, "two groups exchange sums");
+  constexpr int SC = 512, SCALES = 2 * STAGE, REST = SCALES + 2 * SC;  // SC: a step's scales, rows' and weights'
+  constexpr int LDS = REST + NW * 2048;
   static_assert(BM % (16 * NW) == 0 && BN % (8 * NW) == 0 && MT % 4 == 0 && BM <= 256, "whole copies, whole scale dwords");
   static_assert(BN <= FP8_BLOCK && FP8_BLOCK % BN == 0, "one weight scale per tile and K block");
-  constexpr int PS = Products<EXACT, ST, MT, NT>::SLOTS;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW), kg = KG > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) / NW) : 0;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
   const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK, m16 = (int)fp8_scale_rows(p.M);
-  const int steps = (kbs + KG - 1) / KG, first = kg * steps;  // this group's K blocks; those past K are zeros
   const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
 
   // ---- copies.  One brings K block kb of 8 rows: lane l chunk (l % 8) ^ (l / 8) of its row l / 8, to place
@@ -507,7 +474,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
     uint32_t tile;
     int kb, limit;  // limit: K, or 0 past the last tile (zeros)
   };
-  Cursor c1 = {blockIdx.x, first, p.K}, c2 = c1;  // of weights and the first stripes, of the last stripes
+  Cursor c1 = {blockIdx.x, 0, p.K}, c2 = c1;  // of weights and the first stripes, of the last stripes
   i4v rw[CW], ra[2][CA], rsa, rsw;
   auto row_buffer = [&](const uint8_t* base, int first, int row, int end, int rows) {
     if (first + row >= end) row = 0;
@@ -539,8 +506,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
     aim_rows(1, tm * BM);
   };
   auto advance = [&](Cursor& c, auto aim) {
-    if (++c.kb < first + steps) return;
-    c.kb = first;
+    if (++c.kb < kbs) return;
+    c.kb = 0;
     c.tile += gridDim.x;
     if (c.tile < tiles) aim();
     else c.limit = 0;
@@ -548,34 +515,30 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
   const uint32_t fx = 16u * ((lane & 7) ^ (lane >> 3)), vw = (lane >> 3) * (uint32_t)p.K + fx;
   const uint32_t va = (lane >> 3) * (uint32_t)(MT * p.K) + fx, vsc = lane < BM / 4 ? 4u * lane : kOutside;
   const uint32_t vws = lane == 0 ? 0 : kOutside;
-  const uint32_t lds0 = lds_offset(lds) + kg * GROUP;
-  auto within = [&](int kb) -> uint32_t { return KG > 1 ? __builtin_amdgcn_readfirstlane(min(kb, kbs - 1)) : kb; };
+  const uint32_t lds0 = lds_offset(lds);
   // copy j of what cursor 1 brings: the first half of the rows, the scales, the weights
   auto copy1 = [&](int j, uint32_t slot) {
     const bool in = c1.kb * 128 + (int)fx < c1.limit;
-    const uint32_t at = within(c1.kb);
-    if (j < CA) lds_copy16(ra[0][j], in ? va : kOutside, at * 128, lds0 + slot * STAGE + (wave * CA + j) * 1024);
-    else if (j == CA) lds_copy4(rsa, vsc, at * (uint32_t)m16, lds0 + SCALES + SC * slot);  // the same by every wave
-    else if (j == CA + 1) lds_copy_scale<ST>(rsw, vws, at * WSZ, lds0 + SCALES + SC * slot + 256);
-    else lds_copy16(rw[j - CA - 2], in ? vw : kOutside, at * 128, lds0 + slot * STAGE + BM * 128 + (wave * CW + j - CA - 2) * 1024);
+    if (j < CA) lds_copy16(ra[0][j], in ? va : kOutside, c1.kb * 128, lds0 + slot * STAGE + (wave * CA + j) * 1024);
+    else if (j == CA) lds_copy4(rsa, vsc, c1.kb * (uint32_t)m16, lds0 + SCALES + SC * slot);  // the same by every wave
+    else if (j == CA + 1) lds_copy_scale<ST>(rsw, vws, c1.kb * WSZ, lds0 + SCALES + SC * slot + 256);
+    else lds_copy16(rw[j - CA - 2], in ? vw : kOutside, c1.kb * 128, lds0 + slot * STAGE + BM * 128 + (wave * CW + j - CA - 2) * 1024);
   };
   auto copy2 = [&](int j, uint32_t slot) {
     const bool in = c2.kb * 128 + (int)fx < c2.limit;
-    lds_copy16(ra[1][j], in ? va : kOutside, within(c2.kb) * 128, lds0 + slot * STAGE + ((NW + wave) * CA + j) * 1024);
+    lds_copy16(ra[1][j], in ? va : kOutside, c2.kb * 128, lds0 + slot * STAGE + ((NW + wave) * CA + j) * 1024);
   };
   // All copies but the newest CA + C1 (one step's) have landed, and this wave's reads are complete.
   auto arrive = [&]() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(CA + C1) : "memory"); };
 
-  Products<EXACT, ST, MT, NT> prod;
+  Products<false, ST, MT, NT> prod;
   i8v a[2], w[NT];
   uint32_t sa[MT / 4], sw;  // scales: of the rows' stripes, of the weights
   // lane's chunks g and g + 4 of its row: places (g ^ f) and (g ^ f) ^ 4
   const int arow = wm * 16 * MT + r * MT, wrow = wn * 16 * NT + r;
   const uint32_t place = 16 * (g ^ (r & 7));
-  const uint32_t mine = kg * GROUP;
-  uint32_t alo = mine + (wm * 16 + r) * 128 + place, ahi = mine + (wm * 16 + r) * 128 + (place ^ 64);  // in the current step's buffer
-  uint32_t wlo = mine + (BM + wrow) * 128 + place, whi = mine + (BM + wrow) * 128 + (place ^ 64);
-  uint32_t sat = mine + SCALES + arow, swat = mine + SCALES + 256;
+  uint32_t alo = (wm * 16 + r) * 128 + place, ahi = (wm * 16 + r) * 128 + (place ^ 64);  // in the current step's buffer
+  uint32_t wlo = (BM + wrow) * 128 + place, whi = (BM + wrow) * 128 + (place ^ 64), sat = SCALES + arow, swat = SCALES + 256;
   auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
     const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
     v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -603,7 +566,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
 #pragma unroll
   for (int j = 0; j < NT; j++) read_w(j);
   read(alo, ahi, a[0]);
-  prod.first_row(a[0]);
   uint32_t slot = 0;
 
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -615,7 +577,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
       advance(c1, aim1);
       advance(c2, aim2);
       const uint32_t s = sw;
-      prod.begin_step(w);
 #pragma unroll
       for (int i = 0; i < MT; i++) {
         const uint32_t sc = sa[i / 4];
@@ -633,20 +594,20 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int x = 0; x < PS; x++) {
+        for (int x = 0; x < NT; x++) {
           prod.part(i, x, w, a[i & 1], a[(i + 1) & 1], sc, [&](int) { return s; });
           __builtin_amdgcn_sched_barrier(0);
-          if (i == MT - 1 && x < NT) read_w(x);  // each weight operand is replaced as soon as it has been used
+          if (i == MT - 1) read_w(x);  // each weight operand is replaced as soon as it has been used
           // this step's share of copies, behind the products: the next step's last stripes into its buffer,
           // then, once this step's first half is read, the step after it into this one's
           if (i < H - 1) {
-            constexpr int PARTS = (H - 1) * PS;
-            const int at = i * PS + x;
+            constexpr int PARTS = (H - 1) * NT;
+            const int at = i * NT + x;
 #pragma unroll
             for (int c = at * CA / PARTS; c < (at + 1) * CA / PARTS; c++) copy2(c, slot ^ 1);
           } else if (i < MT - 1) {
-            constexpr int PARTS = (MT - H) * PS;
-            const int at = (i - H + 1) * PS + x;
+            constexpr int PARTS = (MT - H) * NT;
+            const int at = (i - H + 1) * NT + x;
 #pragma unroll
             for (int c = at * C1 / PARTS; c < (at + 1) * C1 / PARTS; c++) copy1(c, slot);
           }
@@ -655,17 +616,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
       }
       slot ^= 1;
       kb++;
-    } while (kb < steps);
+    } while (kb < kbs);
     prod.fold();
-    uint8_t* stage = lds + REST + (kg * NW + wave) * 2048;
-    const int ms = m0 + wm * 16 * MT, ns = n0 + wn * NT * 16;
-    if constexpr (KG == 1) {
-      store_stripes<OUT, 0, MT>(p, stage, lane, ms, ns, prod.acc);
-    } else {
-      exchange_halves<2>(stage, lds + REST + ((kg ? 0 : NW) + wave) * 2048, lane, kg, prod.acc);
-      if (kg) store_stripes<OUT, MT / 2, MT>(p, stage, lane, ms, ns, prod.acc);
-      else store_stripes<OUT, 0, MT / 2>(p, stage, lane, ms, ns, prod.acc);
-    }
+    store_stripes<OUT>(p, lds + REST + wave * 2048, lane, m0 + wm * 16 * MT, n0 + wn * NT * 16, prod.acc);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
 }
@@ -675,30 +628,27 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void fp8_tile_kernel(Fp8GemmA
 // columns).  Rows' codes are double-buffered in LDS; the weights have one buffer, a wave's own share:
 // their operands are in registers from a step's start, when the next step's are requested.  The two
 // workgroups run apart, so that one's results are formed and stored behind the other's products.
-// RING, for launches that leave each compute unit one workgroup: a ring of that many K blocks, weights and
-// rows, all but one of them on their way.  KG = 2, for f32 results of such launches: a second group of waves takes
-// the second half of the K blocks, so that each SIMD still has two waves (the vector unit widens for one
-// while the matrix unit works for the other), and the two exchange sums at the end; the halves are
-// always added in the same order, first and second (addition commutes).
-template <int OUT, int ST, bool GATED, int MT, int NW, int RING, int KG>
-__global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
+// RING, for launches that leave each compute unit one workgroup (or two small ones): as many waves again do
+// nothing but copy, through a ring of that many K blocks, weights and rows.  A copy holds its wave up for some 36
+// clocks, and a compute unit receives 64 bytes per clock: in waves that also multiply, copies and products of one
+// workgroup add up (0.43 us a K block of 64 x 256 in bf16), with copying waves a step takes 0.33, near the larger
+// of the two.  Where two workgroups share a compute unit one's copies run behind the other's products, and the
+// copying waves' registers would be missed.
+template <int OUT, int ST, bool GATED, int MT, int NW, int RING>
+__global__ __launch_bounds__(64 * NW * (RING ? 2 : 1), 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
   constexpr bool EXACT = OUT == FP8_IO_F32 && !GATED;
   constexpr int NT = 4, BM = 16 * MT, NM = GATED ? 2 : 1;                     // NM: matrices
   constexpr int STAGES = RING ? RING : 2, STAGE = BM * 128 + (RING ? NW * 8192 : 0);
   constexpr int COLS = (GATED ? 32 : 64) * NW, CA = BM / 8 / NW;              // CA: copies of rows per wave and K block
   constexpr int WEIGHTS = RING ? BM * 128 : 2 * STAGE;  // RING: within a stage
-  constexpr int SCALES = STAGES * STAGE + (RING ? 0 : NW * 8192), GROUP = SCALES + STAGES * 256, OPS = 9 + CA;
-  constexpr int REST = KG * GROUP, EXCHANGE = REST + KG * NW * 2048;
-  constexpr int LDS = GATED ? REST + NW * BM * 4 : EXCHANGE + (KG > 1 ? KG * NW * NT * 1024 : 0);
+  constexpr int SCALES = STAGES * STAGE + (RING ? 0 : NW * 8192), REST = SCALES + STAGES * 256, OPS = 9 + CA;
+  constexpr int LDS = REST + (GATED ? NW * BM * 4 : NW * 2048);
   static_assert(BM % (8 * NW) == 0 && (MT % 4 == 0 || MT == 2) && (!GATED || NW == 4), "whole copies; all columns of a scale");
-  static_assert(KG == 1 || (KG == 2 && !GATED && !RING), "two groups exchange sums");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW), kg = KG > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) / NW) : 0;
-  const int every = kg * NW + wave;
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % NW), copies = RING ? __builtin_amdgcn_readfirstlane((tid >> 6) / NW) : 0;
   const int r = lane & 15, g = lane >> 4;
   const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK, m16 = (int)fp8_scale_rows(p.M);
-  const int steps = (kbs + KG - 1) / KG, first = kg * steps;  // this group's K blocks; those past K are zeros
   const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
 
   // ---- copies of the next step: K block ckb of tile ctile.  One brings 8 rows, lane l chunk (l % 8) ^ (l / 8)
@@ -707,7 +657,7 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
   // the tile's first rows, which nothing uses.  No scalar offset passes its descriptor's end (a copy of
   // weight rows past the matrix is held there): the range check may subtract it from the size.
   uint32_t ctile = blockIdx.x;
-  int ckb = first, climit = p.K;  // climit 0: past the last tile, zeros
+  int ckb = 0, climit = p.K;  // climit 0: past the last tile, zeros
   int tm, tn;                 // place of tile ctile
   i4v ra[CA], rsa, rw[NM];
   uint32_t ws[NM], wsn[NM];   // weight scales: lane k's are of K block k of a stretch of 64
@@ -736,16 +686,15 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
   };
   const uint32_t fx = 16u * ((lane & 7) ^ (lane >> 3)), va = (lane >> 3) * (uint32_t)(MT * p.K) + fx;
   const uint32_t vsa = lane < BM / 4 ? 4u * lane : kOutside, vw = (lane >> 3) * (uint32_t)p.K + fx;
-  const uint32_t lds0 = lds_offset(lds) + kg * GROUP;
+  const uint32_t lds0 = lds_offset(lds);
   uint32_t cva, cvw;  // this step's lane offsets; chunks past K lie outside
   auto copy = [&](int j, uint32_t slot) {
-    const uint32_t at = KG > 1 ? __builtin_amdgcn_readfirstlane(min(ckb, kbs - 1)) : ckb;
     if (j < 8)
       lds_copy16(rw[GATED ? j / 4 : 0], cvw,
-                 min(at * 128 + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K, (uint32_t)rw[GATED ? j / 4 : 0][2]),
+                 min(ckb * 128u + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K, (uint32_t)rw[GATED ? j / 4 : 0][2]),
                  lds0 + (RING ? slot * STAGE : 0) + WEIGHTS + wave * 8192 + j * 1024);
-    else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, at * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
-    else lds_copy4(rsa, vsa, at * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
+    else if (j < 8 + CA) lds_copy16(ra[j - 8], cva, ckb * 128, lds0 + slot * STAGE + (wave * CA + j - 8) * 1024);
+    else lds_copy4(rsa, vsa, ckb * (uint32_t)m16, lds0 + SCALES + 256 * slot);  // the same by every wave
   };
   auto lane_offsets = [&]() {
     const bool in = ckb * 128 + (int)fx < climit;
@@ -758,13 +707,12 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
   uint32_t sa[(MT + 3) / 4];
   // lane's chunks g and g + 4 of its row
   const uint32_t place = 16 * (g ^ (r & 7));
-  uint32_t alo = kg * GROUP + r * 128 + place, ahi = kg * GROUP + r * 128 + (place ^ 64);  // in the current step's buffer
-  uint32_t sat = kg * GROUP + SCALES + r * MT;
+  uint32_t alo = r * 128 + place, ahi = r * 128 + (place ^ 64), sat = SCALES + r * MT;  // in the current step's buffer
   auto read = [&](uint32_t lo, uint32_t hi, i8v& v) {
     const i4v x = *reinterpret_cast<const i4v*>(lds + lo), y = *reinterpret_cast<const i4v*>(lds + hi);
     v = i8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   };
-  uint32_t wat = kg * GROUP + WEIGHTS + wave * 8192 + r * 128;
+  uint32_t wat = WEIGHTS + wave * 8192 + r * 128;
   auto read_w = [&](int j) { read(wat + place + 2048 * j, wat + (place ^ 64) + 2048 * j, w[j]); };
   auto read_scales = [&]() {
     if constexpr (MT == 2) sa[0] = *reinterpret_cast<const uint16_t*>(lds + sat);
@@ -773,8 +721,8 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
   };
 
   auto next_block = [&]() {
-    if (++ckb == first + steps) {
-      ckb = first;
+    if (++ckb == kbs) {
+      ckb = 0;
       ctile += gridDim.x;
       if (ctile < tiles) aim();
       else climit = 0;
@@ -784,20 +732,45 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
   // the next step's copies have landed, those of the steps after it (RING) may be on their way; reads are complete
   constexpr int IN_FLIGHT = (STAGES - 2) * OPS, WAIT = (IN_FLIGHT & 15) | (IN_FLIGHT >> 4 << 14) | 0x70;
 
-  aim();
-  weight_scales(tn * COLS, first, ws);
+  if (copies) {
+    aim();
+    lane_offsets();
+#pragma unroll
+    for (int n = 0; n < STAGES - 1; n++) {
+      if (n) next_block();
+#pragma unroll
+      for (int j = 0; j < OPS; j++) copy(j, n);
+    }
+    __builtin_amdgcn_s_waitcnt(WAIT);
+    asm volatile("s_barrier" ::: "memory");
+    uint32_t fill = STAGES - 1;
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+      for (int kb = 0; kb < kbs; kb++) {
+        next_block();
+#pragma unroll
+        for (int j = 0; j < OPS; j++) copy(j, fill);
+        fill = fill == STAGES - 1 ? 0 : fill + 1;
+        __builtin_amdgcn_s_waitcnt(WAIT);
+        asm volatile("s_barrier" ::: "memory");
+      }
+      if (GATED)  // those of the tile's end
+        for (int n = 0; n < 3; n++) asm volatile("s_barrier" ::: "memory");
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    return;
+  }
+
+  if (RING) tile_place(tiles, tiles_m, tiles_n, ctile, tm, tn);
+  else aim();
+  weight_scales(tn * COLS, 0, ws);
   int ptm = tm, ptn = tn;  // place of the tile that the products are at
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), so that the compiler knows its own loads to be complete
-  lane_offsets();
+  if constexpr (!RING) {
+    lane_offsets();
 #pragma unroll
-  for (int j = 0; j < OPS; j++) copy(j, 0);
-#pragma unroll
-  for (int n = 1; n < STAGES - 1; n++) {
-    next_block();
-#pragma unroll
-    for (int j = 0; j < OPS; j++) copy(j, n);
+    for (int j = 0; j < OPS; j++) copy(j, 0);
+    __builtin_amdgcn_s_waitcnt(WAIT);
   }
-  __builtin_amdgcn_s_waitcnt(WAIT);
   asm volatile("s_barrier" ::: "memory");
   read_scales();
 #pragma unroll
@@ -809,15 +782,15 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int m0 = ptm * BM, n0 = ptn * COLS;
     if (tile + gridDim.x < tiles) tile_place(tiles, tiles_m, tiles_n, tile + gridDim.x, ptm, ptn);
-    weight_scales(ptn * COLS, first, wsn);  // of the next tile
+    weight_scales(ptn * COLS, 0, wsn);  // of the next tile
     prod.clear();
     int kb = 0;
     do {
       if (kb && (kb & 63) == 0) {
-        weight_scales(n0, first + kb, ws);
+        weight_scales(n0, kb, ws);
         __builtin_amdgcn_s_waitcnt(0x0f70);
       }
-      next_block();
+      if (!RING) next_block();
       const uint32_t fill = slot == 0 ? STAGES - 1 : slot - 1, after = slot == STAGES - 1 ? 0 : slot + 1;
       uint32_t swb[NM];
 #pragma unroll
@@ -830,7 +803,7 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
           read(alo + (i + 1) * 2048, ahi + (i + 1) * 2048, a[(i + 1) & 1]);
         } else {
           // the next step's copies have landed; every wave has its rows in LDS, and this step's in registers
-          __builtin_amdgcn_s_waitcnt(WAIT);
+          __builtin_amdgcn_s_waitcnt(RING ? 0xc07f : WAIT);
           asm volatile("s_barrier" ::: "memory");
           const uint32_t step = after == 0 ? (uint32_t)-((STAGES - 1) * STAGE) : (uint32_t)STAGE;
           alo += step, ahi += step, sat += after == 0 ? -(STAGES - 1) * 256 : 256;
@@ -847,8 +820,8 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
           // Behind the products: the next step's weights, whose buffer has been read, and rows.
           constexpr int PARTS = (MT > 2 ? MT - 2 : 1) * 4;
           const int at = i * 4 + x;
-          if (at == 0) __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): w is in registers
-          if (at < PARTS) {
+          if (!RING && at == 0) __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): w is in registers
+          if (!RING && at < PARTS) {
 #pragma unroll
             for (int c = at * OPS / PARTS; c < (at + 1) * OPS / PARTS; c++) copy(c, fill);
           }
@@ -858,19 +831,13 @@ __global__ __launch_bounds__(64 * NW * KG, RING ? 1 : 2) void fp8_strip_kernel(F
       last = slot;
       slot = after;
       kb++;
-    } while (kb < steps);
+    } while (kb < kbs);
 #pragma unroll
     for (int j = 0; j < NM; j++) ws[j] = wsn[j];
     prod.fold();
 
-    if constexpr (KG > 1) {
-      uint8_t* ex = lds + EXCHANGE;
-      exchange_halves<NT>(ex + every * NT * 1024, ex + (kg ? wave : NW + wave) * NT * 1024, lane, kg, prod.acc);
-      uint8_t* stage = lds + REST + every * 2048;
-      if (kg) store_stripes<OUT, MT / 2, MT>(p, stage, lane, m0, n0 + wave * 64, prod.acc);
-      else store_stripes<OUT, 0, MT / 2>(p, stage, lane, m0, n0 + wave * 64, prod.acc);
-    } else if constexpr (!GATED) {
-      store_stripes<OUT, 0, MT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, prod.acc);
+    if constexpr (!GATED) {
+      store_stripes<OUT>(p, lds + REST + wave * 2048, lane, m0, n0 + wave * 64, prod.acc);
     } else {
       // staged in the rows' buffer that the next step's copies go to
       gated_stripes<MT>(p, reinterpret_cast<uint32_t*>(lds + REST), lds + last * STAGE, lane, wave, m0, n0, m16, prod.acc);
@@ -890,25 +857,25 @@ hipError_t launch_small(const Fp8GemmArgs& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int OUT, int ST, int BM, int BN, int WM, int WN, int KG = 1>
+template <int OUT, int ST, int BM, int BN, int WM, int WN>
 hipError_t launch_tile(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
   if (tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_tile_kernel<OUT, ST, BM, BN, WM, WN, KG>),
-             dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / (WM * WN * KG)))), dim3(64 * WM * WN * KG), 0, s, p, tiles_m,
-             tiles_n);
+  T5K_LAUNCH((fp8_tile_kernel<OUT, ST, BM, BN, WM, WN>), dim3((unsigned)std::min<int64_t>(tiles, cus * (8 / (WM * WN)))),
+             dim3(64 * WM * WN), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
 
-template <int OUT, int ST, bool GATED, int MT, int NW, int RING, int KG = 1>
+template <int OUT, int ST, bool GATED, int MT, int NW, int RING>
 hipError_t launch_strip(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   constexpr int COLS = (GATED ? 32 : 64) * NW;
   const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + COLS - 1) / COLS;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
   if (tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, RING, KG>),
-             dim3((unsigned)std::min<int64_t>(tiles, cus * (RING ? 1 : 8 / NW / KG))), dim3(64 * NW * KG), 0, s, p, tiles_m, tiles_n);
+  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, RING>),
+             dim3((unsigned)std::min<int64_t>(tiles, cus * ((RING ? 4 : 8) / NW))), dim3(64 * NW * (RING ? 2 : 1)), 0, s, p,
+             tiles_m, tiles_n);
   return hipGetLastError();
 }
 
@@ -923,45 +890,50 @@ int compute_units() {
   return cus;
 }
 
-// Few tiles: operands straight to the waves, K dealt out over the waves of a workgroup, with the smallest tiles
-// that leave a workgroup per compute unit.  Twice as many still win for one row of them (us, 1 x 16,384 x 4,096: 1 x 2
-// tiles of 16 14.5, LDS tiles 17.3), and for f32 results, whose LDS tiles are slower (32 x 16,384 x 4,096: 18.1 / 23.2);
-// past that LDS tiles do (64 x 32,768 x 4,096: 48 / 22).  us of 1 x 1, 1 x 2, 2 x 2, 4 x 2 and LDS tiles in bf16: 3.8,
-// 3.6, 4.2, 4.5, 6.0 for 32 x 2,304 x 768; 4.2, 5.2, 6.6, 8.3, 10.0 for 64 x 768 x 2,048; 4.5, 4.6, 4.2, 5.0, 6.1 for 64 x
-// 2,304 x 768; 32, 25, 20, 14.9, 17.6 for 64 x 8,192 x 4,096.
+// The smallest tiles that leave each compute unit at most a workgroup, of the kernel that is fastest at that.  us
+// of small kernels of 1 x 1 / 1 x 2 / 2 x 2 / 4 x 2 tiles of 16, then strips through the ring of 32 x 128 / 64 x 128 /
+// 64 x 256; in bf16
+//   1 x 8,192 x 4,096  7.2 / 6.8 / 9.4 / 9.7, 9.9 / 11.7 / 14.1     33 x 2,048 x 4,096  8.4 / 7.9 / 10.5 / 11.3, 8.4 / 11.7 / 13.5
+//   65 x 2,304 x 768   4.6 / 4.6 / 4.2 / 5.1, 3.8 / 4.8 / 5.4       256 x 768 x 2,048   8.0 / 8.0 / 6.6 / 8.4, 5.6 / 7.5 / 8.6
+//   256 x 8,192 x 4,096  - / - / 62 / 48, 16.5 / 13.8 / 16.6        1,000 x 2,304 x 768  - / - / 16 / 15, 7.1 / 6.9 / 6.0
+// and for f32 results, whose widening makes strips slower (32 x 256 in place of 64 x 128)
+//   65 x 2,048 x 4,096  12.2 / 12.6 / 10.5 / 14.5, 20.5 / 21.8 / -  500 x 768 x 2,048   - / 11.1 / 10.5 / 8.9, 11.9 / 12.7 / 17.9
+//   500 x 2,304 x 768  - / - / 10.6 / 12.9, 9.4 / 7.6 / 9.7         1,000 x 2,304 x 768  - / - / 17 / 21, 11.8 / 12.2 / 10.0
 template <int OUT, int ST>
 hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
   const int cus = compute_units();
   auto groups = [&](int rows, int cols) { return (((int64_t)p.M + rows - 1) / rows) * (((int64_t)p.N + cols - 1) / cols); };
   if (groups(16, 16) <= cus) return launch_small<OUT, ST, 1, 1, 8>(p, s);
-  if (groups(16, 32) <= (p.M <= 16 ? 2 * cus : cus)) return launch_small<OUT, ST, 1, 2, 8>(p, s);
-  if (groups(32, 32) <= cus) return launch_small<OUT, ST, 2, 2, 4>(p, s);
-  if (groups(64, 32) <= cus) return launch_small<OUT, ST, 4, 2, 8>(p, s);
+  if (groups(16, 32) <= cus) return launch_small<OUT, ST, 1, 2, 8>(p, s);
   if constexpr (OUT == FP8_IO_F32) {
+    // two workgroups per compute unit: 14.8 against 20 for 1 x 16,384 x 4,096, 18 against 21 for 32 x 16,384 x 4,096
+    if (p.M <= 16 && groups(16, 32) <= 2 * cus) return launch_small<OUT, ST, 1, 2, 8>(p, s);
+    if (groups(32, 32) <= cus) return launch_small<OUT, ST, 2, 2, 4>(p, s);
+    if (groups(64, 32) <= cus) return launch_small<OUT, ST, 4, 2, 8>(p, s);
     if (groups(32, 32) <= 2 * cus) return launch_small<OUT, ST, 2, 2, 4>(p, s);
-    // us, tiles of 64 x 128 / strips of 64 x 256, and each with K halved: 27.4, 22.7 / -, 29.2 for 256 x 2,048 x 4,096 (64
-    // tiles), 15.6, 13.9 / -, 17.3 for 1,000 x 768 x 2,048 (96), 21.5, - / 21.0, 18.2 for 2,800 x 768 x 2,048 (132 strips),
-    // 22.1, 25.8 / 21.7, 19.6 for 4,600 x 768 x 2,048 (216), 45.0, - / 34.3, 38.5 for 9,232 x 768 x 2,048 (435); halving costs
-    // as much as it gives at K = 768 and 1.5 us at one block.
-    const bool halve = p.K >= 8 * FP8_BLOCK;
-    if (groups(64, 256) > cus) return launch_strip<OUT, ST, false, 4, 4, 0>(p, cus, s);
-    if (!halve) return launch_tile<OUT, ST, 64, 128, 1, 4>(p, cus, s);
-    if (groups(64, 128) <= cus) return launch_tile<OUT, ST, 64, 128, 1, 4, 2>(p, cus, s);
-    return launch_strip<OUT, ST, false, 4, 4, 0, 2>(p, cus, s);
+    if (groups(32, 128) <= cus) return launch_strip<OUT, ST, false, 2, 2, 3>(p, cus, s);
+    if (groups(32, 256) <= cus) return launch_strip<OUT, ST, false, 2, 4, 3>(p, cus, s);
+    if (groups(64, 256) <= cus) return launch_strip<OUT, ST, false, 4, 4, 3>(p, cus, s);
+    return launch_strip<OUT, ST, false, 4, 4, 0>(p, cus, s);  // 9,232 x 768 x 2,048: 34.3, through the ring 37
   } else {
-    // strips win once every compute unit has two: 113 against 139 us for 74,640 x 2,048 x 768, 12.6 against 12.5
-    // for 4,616 x 2,048 x 768 (296 strips), 18.8 against 11.3 for 4,616 x 768 x 2,048 (111)
-    if (groups(128, 256) >= 2 * cus) return launch_strip<OUT, ST, false, 8, 4, 0>(p, cus, s);
+    if (groups(32, 128) <= cus) return launch_strip<OUT, ST, false, 2, 2, 3>(p, cus, s);
+    if (groups(64, 128) <= cus) return launch_strip<OUT, ST, false, 4, 2, 3>(p, cus, s);
+    if (groups(64, 256) <= cus) return launch_strip<OUT, ST, false, 4, 4, 3>(p, cus, s);
+    if (groups(128, 256) <= cus) return launch_strip<OUT, ST, false, 8, 4, 3>(p, cus, s);
+    // us of 128 x 256 strips, two workgroups on a compute unit / through the ring / tiles of 128 x 128: 12.0 / 13.1 / 11.6
+    // for 4,616 x 2,048 x 768 (296 strips), 50 / 48 / 45 for 1,500 x 8,192 x 4,096 (384); 12.5 / 13.5 / 14.6 for 6,500 x
+    // 2,304 x 768 (459), 117 / 123 / 136 for 74,640 x 2,048 x 768, 468 / 463 / 530 for 16,391 x 8,192 x 4,096
+    if (2 * groups(128, 256) > 3 * cus) return launch_strip<OUT, ST, false, 8, 4, 0>(p, cus, s);
     return launch_tile<OUT, ST, 128, 128, 2, 2>(p, cus, s);
   }
 }
 
 // A scale needs all of its 128 columns in one workgroup.  Up to one strip per compute unit, as few rows each as that
-// allows, and the ring of three K blocks: us of 32 / 64 rows in the ring / 128 in the ring / 128 without, 6.2 / 7.3 / - / 9.4
-// for 32 x 2,048 x 768, 18.9 / 21.6 / - / 35 for 64 x 8,192 x 4,096, - / 24 / 32 / 36 for 256 x 8,192 x 4,096 (256 strips of
-// 64), - / - / 18 / 21 for 4,616 x 768 x 2,048 (222 of 128).  Beyond that two workgroups on a compute unit: 26 / 21 for 4,616 x
-// 2,048 x 768, where strips of 64 rows take 23.  Few rows leave most compute units without work, and a strip's time is
-// that of its weights through one of them; a ring of four is no faster (6.3), operands straight to registers take 9.0.
+// allows, through the ring: us of 32 / 64 / 128 rows / 128 without the ring, 5.2 / 6.2 / 8.9 / 9.4 for 32 x 2,048 x 768,
+// 16 / 17 / 24 / 35 for 32 x 8,192 x 4,096, 30 / 19 / 27 / - for 200 x 8,192 x 4,096, 30 / 19 / 16 / 21 for 4,616 x 768 x
+// 2,048 (222 of 128).  Beyond that two workgroups on a compute unit: 20.2 against 21.9 for 4,616 x 2,048 x 768, 239
+// against 261 for 74,640 x 2,048 x 768.  Few rows leave most compute units without work, and a strip's time is that of
+// its weights through one of them, at 64 bytes per clock; operands straight to registers take 9.0 for 32 x 2,048 x 768.
 template <int ST>
 hipError_t launch_gated(const Fp8GemmArgs& p, hipStream_t s) {
   const int cus = compute_units();
