@@ -110,7 +110,8 @@ __device__ __forceinline__ void store_out(const Fp8GemmArgs& p, int m, int n, f4
 
 // ---- few rows: 16 MB rows x 16 NB columns per workgroup, its waves on the K blocks in turn ---
 // Each operand goes from memory straight to the wave that multiplies it; the waves' partial sums
-// meet in LDS and are added in wave order.
+// meet in LDS and are added in wave order.  What bounds it is memory: 1 x 8,192 x 4,096 takes 6.8 us in bf16, its
+// 33.6 MB of weights at 5.0 TB/s, a large copy's rate; 32 x 2,304 x 768 3.6, where a launch alone is 2.7.
 template <int OUT, int ST, int MB, int NB, int KS>
 __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int tiles_n, int64_t tiles) {
   __shared__ f4 red[KS][MB * NB][64];
@@ -181,6 +182,9 @@ __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int t
 //    step kb's buffer is refilled, come before the last row of MFMAs of step kb, whose operands are
 //    in registers by then, so the first operands of step kb + 1 are read behind those MFMAs.
 // Out-of-range rows and K chunks past K read as zero through the buffer descriptors' range.
+// For 16-bit results of launches between one and one and a half strips of 128 x 256 per compute unit, whose
+// last round these smaller tiles fill better.  4,616 x 2,048 x 768: 11.6 us, 1.25 PFLOP/s; what bounds it is the
+// last round, and LDS (64 KiB read and 32 written for 16 products of a wave).
 
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
@@ -627,12 +631,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
 // Wave w has all rows and 64 weight rows of its own (gated: 32 gate rows and the 32 up rows of the same
 // columns).  Rows' codes are double-buffered in LDS; the weights have one buffer, a wave's own share:
 // their operands are in registers from a step's start, when the next step's are requested.  The two
-// workgroups run apart, so that one's results are formed and stored behind the other's products.
+// workgroups run apart, so that one's results are formed and stored behind the other's products.  The large
+// sizes: 16,391 x 8,192 x 4,096 in bf16 takes 440 to 470 us, 2.3 to 2.5 PFLOP/s, at the clock that power leaves (a
+// library product of 8,192 cubed reaches 2.6); 74,640 x 2,048 x 768 115 us; gated 229 to 240 us, 2.0 PFLOP/s, the
+// rest its gelu and codes on the vector unit, which adds to the matrix unit's time.  f32 results from 9,232 x 768 x
+// 2,048 34 us, 0.85 PFLOP/s: widening and scaling take the vector unit as long as the products take theirs.
 // RING, for launches that leave each compute unit one workgroup (or two small ones): as many waves again do
 // nothing but copy, through a ring of that many K blocks, weights and rows.  A copy holds its wave up for some 36
 // clocks, and a compute unit receives 64 bytes per clock: in waves that also multiply, copies and products of one
-// workgroup add up (0.43 us a K block of 64 x 256 in bf16), with copying waves a step takes 0.33, near the larger
-// of the two.  Where two workgroups share a compute unit one's copies run behind the other's products, and the
+// workgroup add up (0.52 us a K block of the gated product's 64 x 256), with copying waves a step takes 0.33, near
+// the larger of the two.  Where two workgroups share a compute unit one's copies run behind the other's products, and the
 // copying waves' registers would be missed.
 template <int OUT, int ST, bool GATED, int MT, int NW, int RING>
 __global__ __launch_bounds__(64 * NW * (RING ? 2 : 1), 2) void fp8_strip_kernel(Fp8GemmArgs p, int tiles_m, int tiles_n) {
