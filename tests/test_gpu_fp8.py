@@ -289,6 +289,52 @@ def test_rmsnorm_many_rows(fp8):
     assert other <= 70001 * 6 * 1e-4  # borders are met by chance only
 
 
+def test_longest_rows(fp8):
+    """K = 2^21 through the quantizers and the norm (whose lanes sum 2,048 squares one after another)."""
+    K = 1 << 21
+    x = torch.randn(3, K, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV)
+    v = x.double().cpu().numpy()
+    codes = torch.empty(3, K, dtype=torch.uint8, device=DEV)
+    scales = torch.empty(_blocks(K), 16, dtype=torch.uint8, device=DEV)
+    fp8.quantize_device(x.data_ptr(), 0, 3, K, codes.data_ptr(), scales.data_ptr(), _stream())
+    byte = _byte_of(np.abs(v).reshape(3, -1, 128).max(2))
+    assert np.array_equal(scales[:, :3].cpu().numpy(), byte.T)
+    assert _same_codes(codes.cpu().numpy(), _round_e4m3(v * 2.0 ** (127.0 - np.repeat(byte, 128, 1))))
+    blocks = torch.empty(1, _blocks(K), dtype=torch.uint8, device=DEV)
+    fp8.quantize_weights_device(x.data_ptr(), 0, 3, K, E8M0, codes.data_ptr(), blocks.data_ptr(), _stream())
+    byte = byte.max(0)
+    assert np.array_equal(blocks.cpu().numpy()[0], byte)
+    assert _same_codes(codes.cpu().numpy(), _round_e4m3(v * 2.0 ** (127.0 - np.repeat(byte, 128)[None])))
+    got = _norm_case(fp8, "bf16", "f16", 2, K)
+    _check_codes(*got, ((2048 + 22) / 2 + 8) * U)
+
+
+def test_most_workgroups(fp8):
+    """More rows and blocks than a launch has workgroups: the last ones are reached."""
+    M = (4 << 20) + 5
+    x = torch.zeros(M, 16, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = torch.randn(3, 16, device=DEV).to(torch.bfloat16)
+    g = torch.ones(16, device=DEV)
+    codes = torch.full((M, 16), 77, dtype=torch.uint8, device=DEV)
+    scales = torch.full((1, _rows16(M)), 77, dtype=torch.uint8, device=DEV)
+    fp8.rmsnorm_device(x.data_ptr(), 2, 0, 0, M, 16, g.data_ptr(), 1e-6, 0, codes.data_ptr(), scales.data_ptr(), _stream())
+    assert int(codes[:-3].max()) == 0 and bool((scales[:, :M - 3] == 1).all()) and bool((scales[:, M:] == 77).all())
+    v = x[-3:].double().cpu().numpy()
+    y = v / np.sqrt((v * v).mean(1, keepdims=True) + 1e-6)
+    _check_codes(codes[-3:].cpu().numpy(), scales[:, M - 3:M].cpu().numpy(), y, NORM_REL)
+    del x, codes
+    N = (128 << 20) + 200
+    w = torch.zeros(N, 16, dtype=torch.bfloat16, device=DEV)
+    w[-1] = torch.randn(16, device=DEV).to(torch.bfloat16)
+    codes = torch.full((N, 16), 77, dtype=torch.uint8, device=DEV)
+    scales = torch.full((_blocks(N),), 77, dtype=torch.uint8, device=DEV)
+    fp8.quantize_weights_device(w.data_ptr(), 2, N, 16, E8M0, codes.data_ptr(), scales.data_ptr(), _stream())
+    v = w[-1].double().cpu().numpy()
+    byte = _byte_of(np.abs(v).max())
+    assert bool((scales[:-1] == 1).all()) and int(scales[-1]) == byte
+    assert not bool(codes[:-1].any()) and _same_codes(codes[-1].cpu().numpy(), _round_e4m3(v * 2.0 ** (127.0 - byte)))
+
+
 # ---- products --------------------------------------------------------------------------------
 
 def _operand(values, scale_bytes, M, K):

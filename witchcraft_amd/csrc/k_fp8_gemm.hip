@@ -113,60 +113,57 @@ __device__ __forceinline__ void store_out(const Fp8GemmArgs& p, int m, int n, f4
 // meet in LDS and are added in wave order.  What bounds it is memory: 1 x 8,192 x 4,096 takes 6.8 us in bf16, its
 // 33.6 MB of weights at 5.0 TB/s, a large copy's rate; 32 x 2,304 x 768 3.6, where a launch alone is 2.7.
 template <int OUT, int ST, int MB, int NB, int KS>
-__global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int tiles_n, int64_t tiles) {
+__global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int tiles_n) {
   __shared__ f4 red[KS][MB * NB][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int kbs = (p.K + FP8_BLOCK - 1) / FP8_BLOCK;
   const size_t m16 = fp8_scale_rows(p.M);
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int m0 = (int)(tile / tiles_n) * 16 * MB, n0 = (int)(tile % tiles_n) * 16 * NB;
-    const uint8_t *arow[MB], *wrow[NB], *sa[MB];
+  const int m0 = (int)(blockIdx.x / tiles_n) * 16 * MB, n0 = (int)(blockIdx.x % tiles_n) * 16 * NB;
+  const uint8_t *arow[MB], *wrow[NB], *sa[MB];
+#pragma unroll
+  for (int i = 0; i < MB; i++) {
+    const int m = min(m0 + 16 * i + r, p.M - 1);
+    arow[i] = p.a + (size_t)m * p.K;
+    sa[i] = p.a_scales + m;
+  }
+#pragma unroll
+  for (int j = 0; j < NB; j++) wrow[j] = p.w + (size_t)min(n0 + 16 * j + r, p.N - 1) * p.K;
+  f4 acc[MB][NB];
+#pragma unroll
+  for (int i = 0; i < MB; i++)
+#pragma unroll
+    for (int j = 0; j < NB; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+  for (int kb = wave; kb < kbs; kb += KS) {
+    i8v a[MB], w[NB];
+    uint32_t as[MB], wb[NB];
+    float wf[NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+      w[j] = load_row(wrow[j], kb, g, p.K);
+      const size_t at = (size_t)(min(n0 + 16 * j, p.N - 1) / FP8_BLOCK) * kbs + kb;
+      wb[j] = ST == FP8_E8M0 ? ((const uint8_t*)p.w_scales)[at] : 0;
+      wf[j] = ST == FP8_F32 ? ((const float*)p.w_scales)[at] : 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < MB; i++) {
-      const int m = min(m0 + 16 * i + r, p.M - 1);
-      arow[i] = p.a + (size_t)m * p.K;
-      sa[i] = p.a_scales + m;
-    }
-#pragma unroll
-    for (int j = 0; j < NB; j++) wrow[j] = p.w + (size_t)min(n0 + 16 * j + r, p.N - 1) * p.K;
-    f4 acc[MB][NB];
-#pragma unroll
-    for (int i = 0; i < MB; i++)
-#pragma unroll
-      for (int j = 0; j < NB; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < kbs; kb += KS) {
-      i8v a[MB], w[NB];
-      uint32_t as[MB], wb[NB];
-      float wf[NB];
-#pragma unroll
-      for (int j = 0; j < NB; j++) {
-        w[j] = load_row(wrow[j], kb, g, p.K);
-        const size_t at = (size_t)(min(n0 + 16 * j, p.N - 1) / FP8_BLOCK) * kbs + kb;
-        wb[j] = ST == FP8_E8M0 ? ((const uint8_t*)p.w_scales)[at] : 0;
-        wf[j] = ST == FP8_F32 ? ((const float*)p.w_scales)[at] : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < MB; i++) {
-        a[i] = load_row(arow[i], kb, g, p.K);
-        as[i] = sa[i][kb * m16];
-      }
-#pragma unroll
-      for (int i = 0; i < MB; i++)
-#pragma unroll
-        for (int j = 0; j < NB; j++) block_product<OUT == FP8_IO_F32, ST>(w[j], a[i], as[i], wb[j], wf[j], acc[i][j]);
+      a[i] = load_row(arow[i], kb, g, p.K);
+      as[i] = sa[i][kb * m16];
     }
 #pragma unroll
     for (int i = 0; i < MB; i++)
 #pragma unroll
-      for (int j = 0; j < NB; j++) red[wave][i * NB + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int t = wave; t < MB * NB; t += KS) {
-      f4 v = red[0][t][lane];
+      for (int j = 0; j < NB; j++) block_product<OUT == FP8_IO_F32, ST>(w[j], a[i], as[i], wb[j], wf[j], acc[i][j]);
+  }
 #pragma unroll
-      for (int k = 1; k < KS; k++) v += red[k][t][lane];
-      store_out<OUT>(p, m0 + 16 * (t / NB) + r, n0 + 16 * (t % NB) + 4 * g, v);
-    }
-    __syncthreads();  // red is written again for the next tile
+  for (int i = 0; i < MB; i++)
+#pragma unroll
+    for (int j = 0; j < NB; j++) red[wave][i * NB + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int t = wave; t < MB * NB; t += KS) {
+    f4 v = red[0][t][lane];
+#pragma unroll
+    for (int k = 1; k < KS; k++) v += red[k][t][lane];
+    store_out<OUT>(p, m0 + 16 * (t / NB) + r, n0 + 16 * (t % NB) + 4 * g, v);
   }
 }
 
@@ -636,7 +633,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
 // library product of 8,192 cubed reaches 2.6); 74,640 x 2,048 x 768 115 us; gated 229 to 240 us, 2.0 PFLOP/s, the
 // rest its gelu and codes on the vector unit, which adds to the matrix unit's time.  f32 results from 9,232 x 768 x
 // 2,048 34 us, 0.85 PFLOP/s: widening and scaling take the vector unit as long as the products take theirs.
-// RING, for launches that leave each compute unit one workgroup (or two small ones): as many waves again do
+// RING, for launches that leave each compute unit one workgroup, with one tile each: as many waves again do
 // nothing but copy, through a ring of that many K blocks, weights and rows.  A copy holds its wave up for some 36
 // clocks, and a compute unit receives 64 bytes per clock: in waves that also multiply, copies and products of one
 // workgroup add up (0.52 us a K block of the gated product's 64 x 256), with copying waves a step takes 0.33, near
@@ -752,20 +749,16 @@ __global__ __launch_bounds__(64 * NW * (RING ? 2 : 1), 2) void fp8_strip_kernel(
     __builtin_amdgcn_s_waitcnt(WAIT);
     asm volatile("s_barrier" ::: "memory");
     uint32_t fill = STAGES - 1;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-      for (int kb = 0; kb < kbs; kb++) {
-        next_block();
+    for (int kb = 0; kb < kbs; kb++) {  // the last STAGES - 1 fill stages that nothing reads or uses for its end
+      next_block();
 #pragma unroll
-        for (int j = 0; j < OPS; j++) copy(j, fill);
-        fill = fill == STAGES - 1 ? 0 : fill + 1;
-        __builtin_amdgcn_s_waitcnt(WAIT);
-        asm volatile("s_barrier" ::: "memory");
-      }
-      if (GATED)  // those of the tile's end
-        for (int n = 0; n < 3; n++) asm volatile("s_barrier" ::: "memory");
+      for (int j = 0; j < OPS; j++) copy(j, fill);
+      fill = fill == STAGES - 1 ? 0 : fill + 1;
+      __builtin_amdgcn_s_waitcnt(WAIT);
+      asm volatile("s_barrier" ::: "memory");
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    return;
+    return;  // barriers of the tile's end do not count waves that have ended
   }
 
   if (RING) tile_place(tiles, tiles_m, tiles_n, ctile, tm, tn);
@@ -854,14 +847,11 @@ __global__ __launch_bounds__(64 * NW * (RING ? 2 : 1), 2) void fp8_strip_kernel(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed
 }
 
-constexpr int64_t kMostGroups = 1 << 20;  // workgroups of a launch; the kernels walk what is left
-
 template <int OUT, int ST, int MB, int NB, int KS>
 hipError_t launch_small(const Fp8GemmArgs& p, hipStream_t s) {
   const int tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
-  const int64_t tiles = (int64_t)((p.M + 16 * MB - 1) / (16 * MB)) * tiles_n;
-  T5K_LAUNCH((fp8_small_kernel<OUT, ST, MB, NB, KS>), dim3((unsigned)std::min(tiles, kMostGroups)), dim3(64 * KS), 0,
-             s, p, tiles_n, tiles);
+  const int64_t tiles = (int64_t)((p.M + 16 * MB - 1) / (16 * MB)) * tiles_n;  // few: see launch_product
+  T5K_LAUNCH((fp8_small_kernel<OUT, ST, MB, NB, KS>), dim3((unsigned)tiles), dim3(64 * KS), 0, s, p, tiles_n);
   return hipGetLastError();
 }
 
@@ -881,8 +871,8 @@ hipError_t launch_strip(const Fp8GemmArgs& p, int cus, hipStream_t s) {
   const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + COLS - 1) / COLS;
   const int64_t tiles = (int64_t)tiles_m * tiles_n;
   if (tiles >> 30) return hipErrorInvalidValue;
-  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, RING>),
-             dim3((unsigned)std::min<int64_t>(tiles, cus * ((RING ? 4 : 8) / NW))), dim3(64 * NW * (RING ? 2 : 1)), 0, s, p,
+  const int64_t groups = RING ? tiles : std::min<int64_t>(tiles, cus * (8 / NW));
+  T5K_LAUNCH((fp8_strip_kernel<OUT, ST, GATED, MT, NW, RING>), dim3((unsigned)groups), dim3(64 * NW * (RING ? 2 : 1)), 0, s, p,
              tiles_m, tiles_n);
   return hipGetLastError();
 }
