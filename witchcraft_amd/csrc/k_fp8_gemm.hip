@@ -373,17 +373,21 @@ __device__ __forceinline__ void gated_stripes(const Fp8GemmArgs& p, uint32_t* to
                                               int n0, int m16, f4 (&acc)[MT][4]) {
   const int r = lane & 15, g = lane >> 4;
   const int left = p.N - n0 - wave * 32;  // columns past N do not count (N % 16 == 0: whole 16s)
-  // Magnitudes are compared as their bits, which order alike and need no quieting of NaN.
+  // Largest magnitude of a lane's values of stripe i, NaN left out, as bits, which order alike.  The instruction
+  // takes two more values at a time; fmaxf would first quiet each (they are products, so they are quiet).
   auto largest = [&](int i, bool finite) {
-    uint32_t t[2] = {0, 0};
+    float t[2];
 #pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float y = acc[i][j][e];
-        t[j] = max(t[j], __float_as_uint(finite ? finite_abs(y) : fmaxf(0.f, fabsf(y))));  // fmaxf leaves NaN out
+    for (int j = 0; j < 2; j++) {
+      const f4 y = acc[i][j];
+      if (finite) {
+        t[j] = fmaxf(fmaxf(finite_abs(y[0]), finite_abs(y[1])), fmaxf(finite_abs(y[2]), finite_abs(y[3])));
+      } else {
+        asm("v_max3_f32 %0, |%1|, |%2|, 0" : "=v"(t[j]) : "v"(y[0]), "v"(y[1]));
+        asm("v_max3_f32 %0, |%1|, |%2|, %3" : "=v"(t[j]) : "v"(y[2]), "v"(y[3]), "v"(t[j]));
       }
-    return max(left > 0 ? t[0] : 0u, left > 16 ? t[1] : 0u);
+    }
+    return max(left > 0 ? __float_as_uint(t[0]) : 0u, left > 16 ? __float_as_uint(t[1]) : 0u);
   };
   uint32_t top[MT], all = 0;
 #pragma unroll
