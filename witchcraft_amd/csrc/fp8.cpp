@@ -149,7 +149,10 @@ struct HostCall {
     int ndev = 0;
     if (hipGetDeviceCount(&ndev) != hipSuccess || ndev <= 0) return fail(T5H_ERR_NODEVICE, "no HIP device");
     HIP_OK(hipSetDevice(dev < 0 ? 0 : dev));
-    if (hipMalloc((void**)&p, used) != hipSuccess) return fail(T5H_ERR_NOMEM, "fp8 buffers");
+    if (hipMalloc((void**)&p, used) != hipSuccess) {
+      p = nullptr;
+      return fail(T5H_ERR_NOMEM, "fp8 buffers");
+    }
     HIP_OK(hipMemset(p, 0, used));
     return T5H_OK;
   }

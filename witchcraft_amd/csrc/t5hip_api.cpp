@@ -25,7 +25,10 @@ namespace {
 
 thread_local std::string g_err;
 
+// Every entry point's failures.  A HIP call that failed also set the thread's last HIP error, which no
+// successful call resets: it is taken here, or the launches of a later call would report it as theirs.
 int fail(int code, const std::string& msg) {
+  if (code == T5H_ERR_HIP || code == T5H_ERR_NOMEM || code == T5H_ERR_NODEVICE) (void)hipGetLastError();
   g_err = msg;
   return code;
 }
@@ -629,7 +632,6 @@ int build_tiled(t5h_model* m, const std::vector<Linear*>& ls, void** buf) {
   for (const Linear* L : ls) need += align256((size_t)L->N * L->K * 2);
   if (hipMalloc(buf, need) != hipSuccess) {
     *buf = nullptr;
-    (void)hipGetLastError();  // or the next launch would report it
     return fail(T5H_ERR_NOMEM, "weight operand allocation of " + std::to_string(need) + " bytes failed");
   }
   size_t off = 0;
@@ -1956,7 +1958,6 @@ int build_bf16_layers(t5h_model* m) {
     if (L->fmt == WF_Q4K) need += align256((size_t)L->N * L->K * 2);
   if (need && hipMalloc(&o.w, need) != hipSuccess) {
     o.w = nullptr;
-    (void)hipGetLastError();  // or the next launch would report it
     return fail(T5H_ERR_NOMEM, "bf16 weight allocation of " + std::to_string(need) + " bytes failed");
   }
   size_t off = 0;
