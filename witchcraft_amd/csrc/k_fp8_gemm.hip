@@ -194,13 +194,17 @@ __device__ __forceinline__ i4v buffer_at(const void* base, uint32_t bytes) {
 }
 // Global -> LDS copies as inline asm, so that the compiler adds no waits for them at LDS reads: the
 // kernel's own vmcnt waits and barriers order them.  Lane l's bytes land at m0 + 16 l (4 l).
+// A vector-memory read of a scalar register needs five wait states after the vector unit has written it, as
+// buffer_at does and the restoring of a spilled descriptor; the compiler does not look for that in here.
+// The write of m0 and s_nop 3 are five whatever stands in front; over s_nop 0 they cost 0 to 2% (gated product of
+// 4,616 x 2,048 x 768 20.7 and 21.0 us in turn, 16,391 x 8,192 x 4,096 in bf16 428 and 424).
 __device__ __forceinline__ void lds_copy16(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                "s"(m0)
                : "memory");
 }
 __device__ __forceinline__ void lds_copy4(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                "s"(m0)
                : "memory");
 }
@@ -209,7 +213,7 @@ template <int ST>
 __device__ __forceinline__ void lds_copy_scale(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
   if constexpr (ST == FP8_F32) lds_copy4(rsrc, voff, soff, m0);
   else
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_ubyte %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_ubyte %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                  "s"(m0)
                  : "memory");
 }
