@@ -201,12 +201,12 @@ __device__ __forceinline__ i4v buffer_at(const void* base, uint32_t bytes) {
 __device__ __forceinline__ void lds_copy16(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                "s"(m0)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void lds_copy4(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                "s"(m0)
-               : "memory");
+               : "memory", "m0");
 }
 // One scale per lane, a byte or a dword of memory, a dword in LDS either way.
 template <int ST>
@@ -215,7 +215,7 @@ __device__ __forceinline__ void lds_copy_scale(i4v rsrc, uint32_t voff, uint32_t
   else
     asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_ubyte %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                  "s"(m0)
-                 : "memory");
+                 : "memory", "m0");
 }
 constexpr uint32_t kOutside = 0x7fffffffu;  // past every descriptor's range
 
