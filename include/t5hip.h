@@ -278,12 +278,10 @@ int t5h_embeddings_from_packed(int32_t hip_device, const uint8_t* buf, const siz
  * scales e4m3(x r), r = 448 / max|x| rounded to f32).  Values that are not finite get a NaN code
  * and do not count towards the maximum.
  * Row lengths K, D are multiples of 16 up to 2^21, N of the gated product is a multiple of 16; any M,
- * N >= 0 up to 2^30 (0: nothing to do), with fewer than 2^31 blocks to a matrix and, for a product's
- * activations, fewer than 2^31 scales (M16 a block column).  Rows are contiguous.  Buffers of the device
- * forms start on 16 bytes (weight scales on their own size), lie on the current device, and do not
- * overlap outputs except where said; calls are enqueued on `stream` (a hipStream_t; NULL = the default
- * stream) and return without waiting.  They allocate nothing and keep no state, so they may be captured
- * into a graph and run concurrently.
+ * N >= 0 up to 2^30 (0: nothing to do).  Rows are contiguous.  Buffers of the device forms start on 16 bytes (weight scales on their
+ * own size), lie on the current device, and do not overlap outputs except where said; calls are
+ * enqueued on `stream` (a hipStream_t; NULL = the default stream) and return without waiting.  They
+ * allocate nothing and keep no state, so they may be captured into a graph and run concurrently.
  * The host forms are synchronous, on HIP device hip_device. */
 #define T5H_TYPE_F32 0
 #define T5H_TYPE_F16 1

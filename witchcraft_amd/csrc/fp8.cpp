@@ -40,22 +40,11 @@ size_t weight_scale_bytes(int32_t N, int32_t K, int32_t scale_type) {
 
 int bad(const char* what) { return fail(T5H_ERR_INVALID, std::string("fp8: ") + what); }
 
-#define TRY(expr)                   \
-  do {                              \
-    if (int rc_ = (expr)) return rc_; \
-  } while (0)
-
 // Rows and the summed length of a call; the kernels index blocks of 128 in 31 bits.
 int check_shape(int32_t rows, int32_t K) {
   if (rows < 0 || rows > kMostRows) return bad("rows must lie in 0 .. 2^30");
   if (K < 16 || K % 16 || K > t5k::FP8_MAX_K) return bad("row length must be a multiple of 16 in 16 .. 2^21");
   if (((uint64_t)rows * blocks_of(K)) >> 31) return bad("2^31 blocks or more");
-  return T5H_OK;
-}
-// A product's activations: the kernels read their scales in one descriptor, whose outside begins at 2^31 - 1.
-int check_activations(int32_t M, int32_t K) {
-  TRY(check_shape(M, K));
-  if (act_scale_bytes(M, K) >> 31) return bad("2^31 activation scales or more, rows rounded up to 16");
   return T5H_OK;
 }
 int check_buffer(const void* p, const char* name, size_t align = 16) {
@@ -68,6 +57,11 @@ bool same_or_apart(const void* a, size_t an, const void* b, size_t bn) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return x == y || x + an <= y || y + bn <= x;
 }
+
+#define TRY(expr)                   \
+  do {                              \
+    if (int rc_ = (expr)) return rc_; \
+  } while (0)
 
 int check_quantize(const void* x, int32_t type, int32_t M, int32_t K, const void* codes, const void* scales) {
   TRY(check_shape(M, K));
@@ -113,7 +107,7 @@ int check_rmsnorm(const void* x, int32_t x_type, const void* delta, int32_t delt
 
 int check_product(const void* a, const void* a_scales, int32_t M, const void* w, const void* w_scales, int32_t N,
                   int32_t K, int32_t scale_type, const void* out) {
-  TRY(check_activations(M, K));
+  TRY(check_shape(M, K));
   TRY(check_shape(N, K));
   if (!known_scale(scale_type)) return bad("unknown scale type");
   if (M == 0 || N == 0) return T5H_OK;
@@ -285,7 +279,7 @@ int t5h_fp8_matmul_device(const uint8_t* d_a, const uint8_t* d_a_scales, int32_t
 
 int t5h_fp8_matmul(int32_t hip_device, const uint8_t* a, const uint8_t* a_scales, int32_t M, const uint8_t* w,
                    const void* w_scales, int32_t N, int32_t K, int32_t scale_type, void* c, int32_t c_type) {
-  TRY(check_activations(M, K));
+  TRY(check_shape(M, K));
   TRY(check_shape(N, K));
   if (!known_scale(scale_type)) return bad("unknown scale type");
   if (!known_type(c_type)) return bad("unknown type");
@@ -322,7 +316,7 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
 int t5h_fp8_gated_gelu(int32_t hip_device, const uint8_t* a, const uint8_t* a_scales, int32_t M, const uint8_t* w0,
                        const void* w0_scales, const uint8_t* w1, const void* w1_scales, int32_t N, int32_t K,
                        int32_t scale_type, uint8_t* codes, uint8_t* scales) {
-  TRY(check_activations(M, K));
+  TRY(check_shape(M, K));
   TRY(check_shape(N, K));
   if (N % 16) return bad("the gated product's columns must be a multiple of 16");
   if (((uint64_t)M * blocks_of(N)) >> 31) return bad("2^31 blocks or more");
