@@ -36,6 +36,13 @@ def _blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
 
 
+def _fits(bits: int) -> None:
+    """`bits`, sizes and type codes or-ed together, is what the library's 32-bit arguments hold: ctypes
+    would pass the low bits of a larger number."""
+    if bits >> 31:
+        raise ValueError("sizes and type codes must lie in 0 .. 2^31 - 1")
+
+
 def _input(x: np.ndarray, name: str) -> tuple[np.ndarray, int]:
     x = np.ascontiguousarray(x)
     if x.ndim != 2:
@@ -72,6 +79,7 @@ def quantize(x: np.ndarray, hip_device: int = 0) -> tuple[np.ndarray, np.ndarray
     """f32 or f16 activations [M, K] -> (codes [M, K], scales [ceil(K/128), M16])."""
     x, t = _input(x, "x")
     m, k = x.shape
+    _fits(m | k)
     codes, scales = np.empty((m, k), np.uint8), np.zeros((_blocks(k), scale_rows(m)), np.uint8)
     check(lib.t5h_fp8_quantize(hip_device, x.ctypes.data, t, m, k, codes.ctypes.data, scales.ctypes.data))
     return codes, scales
@@ -81,6 +89,7 @@ def quantize_weights(w: np.ndarray, scale_type: int = E8M0, hip_device: int = 0)
     """f32 or f16 weights [N, K] -> (codes [N, K], scales [ceil(N/128), ceil(K/128)])."""
     w, t = _input(w, "w")
     n, k = w.shape
+    _fits(n | k | scale_type)
     codes = np.empty((n, k), np.uint8)
     scales = np.empty((_blocks(n), _blocks(k)), np.float32 if scale_type == F32_SCALES else np.uint8)
     check(lib.t5h_fp8_quantize_weights(hip_device, w.ctypes.data, t, n, k, scale_type, codes.ctypes.data,
@@ -94,6 +103,7 @@ def rmsnorm(x: np.ndarray, gamma: np.ndarray, eps: float = 1e-6, delta: np.ndarr
     where sum is x + delta in x's type."""
     x, xt = _input(x, "x")
     m, d = x.shape
+    _fits(m | d)
     gamma = np.ascontiguousarray(gamma, np.float32)
     if gamma.shape != (d,):
         raise ValueError(f"gamma is {gamma.shape}, rows have {d} values")
@@ -114,6 +124,7 @@ def matmul(a, w, dtype=np.float32, hip_device: int = 0) -> np.ndarray:
     ac, asc = _activations(a)
     wc, wsc, st = _weights(w)
     (m, k), (n, k2) = ac.shape, wc.shape
+    _fits(m | n | k)
     if k != k2:
         raise ValueError(f"matmul dimension mismatch: a is [{m},{k}], w is [{n},{k2}]")
     types = [c for c, t in _NUMPY.items() if np.dtype(t) == np.dtype(dtype)]
@@ -131,6 +142,7 @@ def gated_gelu(a, w0, w1, hip_device: int = 0) -> tuple[np.ndarray, np.ndarray]:
     c0, s0, st = _weights(w0)
     c1, s1, st1 = _weights(w1)
     (m, k), (n, k2) = ac.shape, c0.shape
+    _fits(m | n | k)
     if k != k2 or c1.shape != c0.shape or st1 != st:
         raise ValueError(f"gated_gelu mismatch: a is [{m},{k}], w0 {c0.shape} {s0.dtype}, w1 {c1.shape} {s1.dtype}")
     codes, scales = np.empty((m, n), np.uint8), np.zeros((_blocks(n), scale_rows(m)), np.uint8)
@@ -141,12 +153,14 @@ def gated_gelu(a, w0, w1, hip_device: int = 0) -> tuple[np.ndarray, np.ndarray]:
 
 def quantize_device(d_x: int, type: int, m: int, k: int, d_codes: int, d_scales: int, stream: int = 0) -> None:
     """Activations of `type` (F32, F16, BF16) -> codes and scales, asynchronous on `stream`."""
+    _fits(type | m | k)
     check(lib.t5h_fp8_quantize_device(d_x, type, m, k, d_codes, d_scales, stream))
 
 
 def quantize_weights_device(d_w: int, type: int, n: int, k: int, scale_type: int, d_codes: int, d_scales: int,
                             stream: int = 0) -> None:
     """Weights of `type` -> codes and scales of `scale_type` (E8M0, F32_SCALES), on `stream`."""
+    _fits(type | n | k | scale_type)
     check(lib.t5h_fp8_quantize_weights_device(d_w, type, n, k, scale_type, d_codes, d_scales, stream))
 
 
@@ -154,6 +168,7 @@ def rmsnorm_device(d_x: int, x_type: int, d_delta: int, delta_type: int, m: int,
                    d_sum: int, d_codes: int, d_scales: int, stream: int = 0) -> None:
     """Residual's addition, T5LayerNorm and codes on `stream`; d_delta and d_sum may be 0 (none), and
     d_sum may be d_x."""
+    _fits(x_type | delta_type | m | d)
     check(lib.t5h_fp8_rmsnorm_device(d_x, x_type, d_delta, delta_type, m, d, d_gamma, eps, d_sum, d_codes, d_scales,
                                      stream))
 
@@ -161,11 +176,13 @@ def rmsnorm_device(d_x: int, x_type: int, d_delta: int, delta_type: int, m: int,
 def matmul_device(d_a: int, d_a_scales: int, m: int, d_w: int, d_w_scales: int, n: int, k: int, scale_type: int,
                   d_c: int, c_type: int, stream: int = 0) -> None:
     """C [m, n] of `c_type` = A . W^T on `stream`."""
+    _fits(m | n | k | scale_type | c_type)
     check(lib.t5h_fp8_matmul_device(d_a, d_a_scales, m, d_w, d_w_scales, n, k, scale_type, d_c, c_type, stream))
 
 
 def gated_gelu_device(d_a: int, d_a_scales: int, m: int, d_w0: int, d_w0_scales: int, d_w1: int, d_w1_scales: int,
                       n: int, k: int, scale_type: int, d_codes: int, d_scales: int, stream: int = 0) -> None:
     """gelu(A . W0^T) * (A . W1^T) -> codes [m, n] and scales on `stream`."""
+    _fits(m | n | k | scale_type)
     check(lib.t5h_fp8_gated_gelu_device(d_a, d_a_scales, m, d_w0, d_w0_scales, d_w1, d_w1_scales, n, k, scale_type,
                                         d_codes, d_scales, stream))
