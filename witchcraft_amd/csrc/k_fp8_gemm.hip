@@ -220,35 +220,38 @@ __device__ __forceinline__ void lds_copy_scale(i4v rsrc, uint32_t voff, uint32_t
                  "s"(m0)
                  : "memory", "m0");
 }
-// Copies in a run, each 1024 bytes of LDS behind the last: one wait for all of their descriptors.  Eight of
-// weights, four from each of two matrices (or of one), at their own scalar offsets, and a stage's rows with
-// their scales behind them.  For waves that only copy, whose issue can be what a step takes: 65 x 2,048 x 4,096
-// in bf16 8.3 us, with a wait in front of each copy 10.1.
-#define T5K_RUN_FIRST(rsrc, voff, soff) "s_mov_b32 m0, %[at]\n\ts_nop 3\n\tbuffer_load_dwordx4 %[" voff "], %[" rsrc "], %[" soff "] offen lds\n\t"
-#define T5K_RUN_NEXT(rsrc, voff, soff) "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %[" voff "], %[" rsrc "], %[" soff "] offen lds\n\t"
-#define T5K_RUN_SCALES "s_mov_b32 m0, %[sat]\n\ts_nop 0\n\tbuffer_load_dword %[sv], %[sr], %[ss] offen lds"
-__device__ __forceinline__ void lds_copy_weights(i4v a, i4v b, uint32_t voff, const uint32_t (&s)[8], uint32_t m0) {
-  asm volatile(T5K_RUN_FIRST("a", "v", "s0") T5K_RUN_NEXT("a", "v", "s1") T5K_RUN_NEXT("a", "v", "s2") T5K_RUN_NEXT("a", "v", "s3")
-               T5K_RUN_NEXT("b", "v", "s4") T5K_RUN_NEXT("b", "v", "s5") T5K_RUN_NEXT("b", "v", "s6") T5K_RUN_NEXT("b", "v", "s7")
-               ::[v] "v"(voff), [a] "s"(a), [b] "s"(b), [s0] "s"(s[0]), [s1] "s"(s[1]), [s2] "s"(s[2]), [s3] "s"(s[3]),
-               [s4] "s"(s[4]), [s5] "s"(s[5]), [s6] "s"(s[6]), [s7] "s"(s[7]), [at] "s"(m0)
+// Copies in a run, each 1024 bytes of LDS behind the last, with one wait for all of their descriptors: eight of
+// weights at their own scalar offsets, and a stage's rows with their scales behind them.  For workgroups with two
+// waves that only copy, whose issue can be what a step takes: 65 x 2,048 x 4,096 in bf16 8.3 us, with a wait in
+// front of each copy 10.1.  Four such waves are faster with single copies, between which the compiler forms
+// the next one's offset: gated 135 x 2,032 x 2,976 11.2 us, in runs 11.5.
+#define T5K_RUN_FIRST(rsrc, soff) "s_mov_b32 m0, %[at]\n\ts_nop 3\n\tbuffer_load_dwordx4 %[v], %[" rsrc "], %[" soff "] offen lds\n\t"
+#define T5K_RUN_NEXT(rsrc, soff) "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %[v], %[" rsrc "], %[" soff "] offen lds\n\t"
+__device__ __forceinline__ void lds_copy_weights(i4v r, uint32_t voff, const uint32_t (&s)[8], uint32_t m0) {
+  asm volatile(T5K_RUN_FIRST("r", "s0") T5K_RUN_NEXT("r", "s1") T5K_RUN_NEXT("r", "s2") T5K_RUN_NEXT("r", "s3")
+               T5K_RUN_NEXT("r", "s4") T5K_RUN_NEXT("r", "s5") T5K_RUN_NEXT("r", "s6") T5K_RUN_NEXT("r", "s7")
+               ::[v] "v"(voff), [r] "s"(r), [s0] "s"(s[0]), [s1] "s"(s[1]), [s2] "s"(s[2]), [s3] "s"(s[3]), [s4] "s"(s[4]),
+               [s5] "s"(s[5]), [s6] "s"(s[6]), [s7] "s"(s[7]), [at] "s"(m0)
                : "memory", "m0", "scc");
 }
 template <int N>
 __device__ __forceinline__ void lds_copy_rows(const i4v (&r)[N], uint32_t voff, uint32_t soff, uint32_t m0, i4v scales, uint32_t scale_voff,
                                               uint32_t scale_soff, uint32_t scale_m0) {
-  static_assert(N == 1 || N == 2 || N == 4, "a stage's rows");
+  static_assert(N == 2 || N == 4, "a stage's rows");
+#define T5K_RUN_SCALES "s_mov_b32 m0, %[sat]\n\ts_nop 0\n\tbuffer_load_dword %[sv], %[sr], %[ss] offen lds"
 #define T5K_RUN_IN [v] "v"(voff), [s] "s"(soff), [at] "s"(m0), [sr] "s"(scales), [sv] "v"(scale_voff), [ss] "s"(scale_soff), [sat] "s"(scale_m0)
-  if constexpr (N == 1)
-    asm volatile(T5K_RUN_FIRST("a", "v", "s") T5K_RUN_SCALES ::T5K_RUN_IN, [a] "s"(r[0]) : "memory", "m0");
-  else if constexpr (N == 2)
-    asm volatile(T5K_RUN_FIRST("a", "v", "s") T5K_RUN_NEXT("b", "v", "s") T5K_RUN_SCALES ::T5K_RUN_IN, [a] "s"(r[0]), [b] "s"(r[1])
+  if constexpr (N == 2)
+    asm volatile(T5K_RUN_FIRST("a", "s") T5K_RUN_NEXT("b", "s") T5K_RUN_SCALES ::T5K_RUN_IN, [a] "s"(r[0]), [b] "s"(r[1])
                  : "memory", "m0", "scc");
   else
-    asm volatile(T5K_RUN_FIRST("a", "v", "s") T5K_RUN_NEXT("b", "v", "s") T5K_RUN_NEXT("c", "v", "s") T5K_RUN_NEXT("d", "v", "s") T5K_RUN_SCALES
+    asm volatile(T5K_RUN_FIRST("a", "s") T5K_RUN_NEXT("b", "s") T5K_RUN_NEXT("c", "s") T5K_RUN_NEXT("d", "s") T5K_RUN_SCALES
                  ::T5K_RUN_IN, [a] "s"(r[0]), [b] "s"(r[1]), [c] "s"(r[2]), [d] "s"(r[3])
                  : "memory", "m0", "scc");
+#undef T5K_RUN_SCALES
+#undef T5K_RUN_IN
 }
+#undef T5K_RUN_FIRST
+#undef T5K_RUN_NEXT
 constexpr uint32_t kOutside = 0x7fffffffu;  // past every descriptor's range
 
 // c + one K block of a 16 x 16 tile; sa4: four rows' scale bytes, sel the one; swb: the weights' byte.
@@ -743,13 +746,17 @@ __global__ __launch_bounds__(64 * NW * (RING ? 2 : 1), 2) void fp8_strip_kernel(
   };
   // RING: all copies of a step, by a copying wave
   auto copy_stage = [&](uint32_t slot) {
-    uint32_t at[8];
+    if constexpr (NW == 2) {
+      uint32_t at[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      at[j] = min(ckb * 128u + (uint32_t)((GATED ? j % 4 : j) * 8) * (uint32_t)p.K, (uint32_t)rw[GATED ? j / 4 : 0][2]);
-    lds_copy_weights(rw[0], rw[NM - 1], cvw, at, lds0 + slot * STAGE + WEIGHTS + wave * 8192);
-    lds_copy_rows<CA>(ra, cva, ckb * 128, lds0 + slot * STAGE + wave * CA * 1024, rsa, vsa, ckb * (uint32_t)m16,
-                      lds0 + SCALES + 256 * slot);
+      for (int j = 0; j < 8; j++) at[j] = min(ckb * 128u + (uint32_t)(j * 8) * (uint32_t)p.K, (uint32_t)rw[0][2]);
+      lds_copy_weights(rw[0], cvw, at, lds0 + slot * STAGE + WEIGHTS + wave * 8192);
+      lds_copy_rows<CA>(ra, cva, ckb * 128, lds0 + slot * STAGE + wave * CA * 1024, rsa, vsa, ckb * (uint32_t)m16,
+                        lds0 + SCALES + 256 * slot);
+    } else {
+#pragma unroll
+      for (int j = 0; j < OPS; j++) copy(j, slot);
+    }
   };
   auto lane_offsets = [&]() {
     const bool in = ckb * 128 + (int)fx < climit;
