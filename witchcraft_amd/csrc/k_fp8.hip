@@ -44,8 +44,8 @@ __device__ __forceinline__ void load8(const void* p, size_t i, float (&v)[8]) {
 
 // ---- activations: 16 threads per block of 128, 8 values each --------------------------------
 // 8 values are one 16-byte load of a 16-bit type and one 8-byte store, and 16 threads are a row of the wave's
-// lanes, whose maximum takes four lane moves and no LDS.  74,640 x 768 takes 42 us from f32 (6.8 TB/s, some of it
-// from the last-level cache), 29 from f16; 30,000 x 8,192 from bf16 140 us (5.3 TB/s, a large copy's rate).
+// lanes, whose maximum takes four lane moves and no LDS.  74,640 x 768 takes 42 us from f32 (6.9 TB/s, some of it
+// from the last-level cache), 28.5 from f16; 30,000 x 8,192 from bf16 128 us (5.8 TB/s).  A large copy has 5.0.
 template <int T>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* x, int K, int kb, uint32_t blocks,
                                                            size_t m16, uint8_t* codes, uint8_t* scales) {
@@ -74,7 +74,8 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const void* x, int K,
 
 // ---- weights: one workgroup per 128 x 128 block, all of it in registers ----------------------
 // A block's scale needs all of it, so it is held (64 values a thread) rather than read twice.  8,192 x 4,096 from
-// f32: 31.3 us (5.4 TB/s).
+// f32: 31.3 us (5.4 TB/s), from the same matrix again 25.8, as the last-level cache holds part of its 134 MB; byte
+// scales 26.3.
 template <int T>
 __global__ __launch_bounds__(256) void fp8_quantize_weights_kernel(const void* w, int N, int K, int kb,
                                                                    uint32_t blocks, int f32_scales, uint8_t* codes, void* scales) {
@@ -167,8 +168,10 @@ __device__ __forceinline__ void norm_codes(const Fp8NormArgs& a, size_t row, int
 
 // A row stays in registers between its sum of squares and its codes: one wave for up to 1,024 values (four rows
 // a workgroup, no barrier), 4 or 16 waves past that, so that a lane holds at most 16 values and a lone row of
-// 8,192 takes 3.9 us, most of it the launch.  74,640 x 768, f32 with an f16 delta: 114 us, 5.5 TB/s; 4,616 x 768:
-// 8.7 us, 4.5 TB/s.
+// 8,192 takes 3.7 us, half of it the launch.  74,640 x 768, f32 with an f16 delta: 114 us, 5.5 TB/s; 4,616 x 768:
+// 7.7 us, 5.1 TB/s; 74,640 x 768 all in bf16 77 us, 5.2 TB/s.  Four waves a row: 20,000 x 2,048 in bf16 54 us, 5.3
+// TB/s.  Sixteen: 5,000 x 8,192 in f32 with an f16 delta 87 us, 5.2 TB/s, in bf16 73 to 77 us, 3.7 to 3.9 TB/s (two
+// rows of 16 waves fill a compute unit, and each waits twice for its slowest wave).
 // W waves per row, C chunks of 256 W values in registers; C = 0: a row of any length, read twice
 // (the second time from the stored sum, where there is one: it may have replaced x or delta).
 template <int XT, int DT, int W, int C>

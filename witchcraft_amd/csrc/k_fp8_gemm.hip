@@ -113,8 +113,9 @@ __device__ __forceinline__ void store_out(const Fp8GemmArgs& p, int m, int n, f4
 
 // ---- few rows: 16 MB rows x 16 NB columns per workgroup, its waves on the K blocks in turn ---
 // Each operand goes from memory straight to the wave that multiplies it; the waves' partial sums
-// meet in LDS and are added in wave order.  What bounds it is memory: 1 x 8,192 x 4,096 takes 6.8 us in bf16, its
-// 33.6 MB of weights at 5.0 TB/s, a large copy's rate; 32 x 2,304 x 768 3.6, where a launch alone is 2.7.
+// meet in LDS and are added in wave order.  What bounds it is memory: 1 x 8,192 x 4,096 takes 6.5 us in bf16, its
+// 33.6 MB of weights at 5.1 TB/s; 32 x 2,304 x 768 3.1, a launch (1.7) and two trips to memory.  A wave has one K
+// block on its way at a time, so with a long K and several rows the trips add up: 65 x 2,048 x 4,096 in f32 10.7 us.
 template <int OUT, int ST, int MB, int NB, int KS>
 __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int tiles_n) {
   __shared__ f4 red[KS][MB * NB][64];
@@ -183,13 +184,14 @@ __global__ __launch_bounds__(64 * KS) void fp8_small_kernel(Fp8GemmArgs p, int t
 //    in registers by then, so the first operands of step kb + 1 are read behind those MFMAs.
 // Out-of-range rows and K chunks past K read as zero through the buffer descriptors' range.
 // For 16-bit results of launches between one and one and a half strips of 128 x 256 per compute unit, whose
-// last round these smaller tiles fill better.  4,616 x 2,048 x 768: 11.6 us, 1.25 PFLOP/s; what bounds it is the
+// last round these smaller tiles fill better.  4,616 x 2,048 x 768: 12 us, 1.2 PFLOP/s; what bounds it is the
 // last round, and LDS (64 KiB read and 32 written for 16 products of a wave).
 
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
-// Raw buffer of `bytes` bytes at a wave-uniform base; reads past it give zero.
+// Raw buffer of `bytes` bytes at a wave-uniform base; reads past it give zero.  The lane's and the scalar offset
+// count together (measured: a scalar offset at the end or past it leaves no lane in range).
 __device__ __forceinline__ i4v buffer_at(const void* base, uint32_t bytes) {
   const uint64_t b = (uint64_t)(uintptr_t)base;
   return i4v{__builtin_amdgcn_readfirstlane((int)(uint32_t)b), __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff),
@@ -199,8 +201,8 @@ __device__ __forceinline__ i4v buffer_at(const void* base, uint32_t bytes) {
 // kernel's own vmcnt waits and barriers order them.  Lane l's bytes land at m0 + 16 l (4 l).
 // A vector-memory read of a scalar register needs five wait states after the vector unit has written it, as
 // buffer_at does and the restoring of a spilled descriptor; the compiler does not look for that in here.
-// The write of m0 and s_nop 3 are five whatever stands in front; over s_nop 0 they cost 0 to 2% (gated product of
-// 4,616 x 2,048 x 768 20.7 and 21.0 us in turn, 16,391 x 8,192 x 4,096 in bf16 428 and 424).
+// The write of m0 and s_nop 3 are five whatever stands in front.  Over s_nop 0 they cost 0 to 3%, in turn: gated
+// 4,616 x 2,048 x 768 20.7 to 21.0 us, 24,288 x 113 x 3,936 in f32 57.9 to 59.4, 16,391 x 8,192 x 4,096 in bf16 nothing.
 __device__ __forceinline__ void lds_copy16(i4v rsrc, uint32_t voff, uint32_t soff, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff),
                "s"(m0)
@@ -672,10 +674,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8GemmArgs p
 // columns).  Rows' codes are double-buffered in LDS; the weights have one buffer, a wave's own share:
 // their operands are in registers from a step's start, when the next step's are requested.  The two
 // workgroups run apart, so that one's results are formed and stored behind the other's products.  The large
-// sizes: 16,391 x 8,192 x 4,096 in bf16 takes 440 to 470 us, 2.3 to 2.5 PFLOP/s, at the clock that power leaves (a
-// library product of 8,192 cubed reaches 2.6); 74,640 x 2,048 x 768 115 us; gated 229 to 240 us, 2.0 PFLOP/s, the
-// rest its gelu and codes on the vector unit, which adds to the matrix unit's time.  f32 results from 9,232 x 768 x
-// 2,048 34 us, 0.85 PFLOP/s: widening and scaling take the vector unit as long as the products take theirs.
+// sizes: 16,391 x 8,192 x 4,096 in bf16 takes 424 to 456 us, 2.4 to 2.6 PFLOP/s, at the clock that power leaves (a
+// library product of 8,192 cubed reaches 2.6), with float scales 476 to 510, for the multiply-add per result and K
+// block; 74,640 x 2,048 x 768 115 to 122 us, float scales 126 to 135; gated 226 to 247 us, 1.9 to 2.1 PFLOP/s, the
+// rest its gelu and codes on the vector unit, which adds to the matrix unit's time, float scales 261 to 284.  f32
+// results from 9,232 x 768 x 2,048 33 us, 0.87 PFLOP/s: widening and scaling take the vector unit as long as the
+// products take theirs.
 // RING, for launches that leave each compute unit one workgroup, with one tile each: as many waves again do
 // nothing but copy, through a ring of that many K blocks, weights and rows.  A copy holds its wave up for some 36
 // clocks, and a compute unit receives 64 bytes per clock: in waves that also multiply, copies and products of one
@@ -967,15 +971,16 @@ hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
     if (groups(32, 128) <= cus) return launch_strip<OUT, ST, false, 2, 2, 3>(p, cus, s);
     if (groups(32, 256) <= cus) return launch_strip<OUT, ST, false, 2, 4, 3>(p, cus, s);
     if (groups(64, 256) <= cus) return launch_strip<OUT, ST, false, 4, 4, 3>(p, cus, s);
-    return launch_strip<OUT, ST, false, 4, 4, 0>(p, cus, s);  // 9,232 x 768 x 2,048: 34.3, through the ring 37
+    return launch_strip<OUT, ST, false, 4, 4, 0>(p, cus, s);  // 9,232 x 768 x 2,048: 32.6, through the ring 35
   } else {
     if (groups(32, 128) <= cus) return launch_strip<OUT, ST, false, 2, 2, 3>(p, cus, s);
     if (groups(64, 128) <= cus) return launch_strip<OUT, ST, false, 4, 2, 3>(p, cus, s);
     if (groups(64, 256) <= cus) return launch_strip<OUT, ST, false, 4, 4, 3>(p, cus, s);
     if (groups(128, 256) <= cus) return launch_strip<OUT, ST, false, 8, 4, 3>(p, cus, s);
-    // us of 128 x 256 strips, two workgroups on a compute unit / through the ring / tiles of 128 x 128: 12.0 / 13.1 / 11.6
-    // for 4,616 x 2,048 x 768 (296 strips), 50 / 48 / 45 for 1,500 x 8,192 x 4,096 (384); 12.5 / 13.5 / 14.6 for 6,500 x
-    // 2,304 x 768 (459), 117 / 123 / 136 for 74,640 x 2,048 x 768, 468 / 463 / 530 for 16,391 x 8,192 x 4,096
+    // us of 128 x 256 strips, two workgroups on a compute unit / through the ring / tiles of 128 x 128: 12.2 / 14.9 / 12.2
+    // for 4,616 x 2,048 x 768 (296 strips), 48.7 / 48.2 / 47.5 for 1,500 x 8,192 x 4,096 (384); 13.3 / 15.1 / 15.8 for
+    // 6,500 x 2,304 x 768 (459), 115 / 146 / 135 for 74,640 x 2,048 x 768, 427 / 441 / 497 for 16,391 x 8,192 x 4,096.
+    // Over 34 sizes of 257 to 384 strips the tiles take 0.95 of the strips' time with byte scales, 0.97 with float ones.
     if (2 * groups(128, 256) > 3 * cus) return launch_strip<OUT, ST, false, 8, 4, 0>(p, cus, s);
     return launch_tile<OUT, ST, 128, 128, 2, 2>(p, cus, s);
   }
@@ -984,8 +989,8 @@ hipError_t launch_product(const Fp8GemmArgs& p, hipStream_t s) {
 // A scale needs all of its 128 columns in one workgroup.  Up to one strip per compute unit, as few rows each as that
 // allows, through the ring: us of 32 / 64 / 128 rows / 128 without the ring, 5.2 / 6.2 / 8.9 / 9.4 for 32 x 2,048 x 768,
 // 16 / 17 / 24 / 35 for 32 x 8,192 x 4,096, 30 / 19 / 27 / - for 200 x 8,192 x 4,096, 30 / 19 / 16 / 21 for 4,616 x 768 x
-// 2,048 (222 of 128).  Beyond that two workgroups on a compute unit: 20.2 against 21.9 for 4,616 x 2,048 x 768, 239
-// against 261 for 74,640 x 2,048 x 768.  Few rows leave most compute units without work, and a strip's time is that of
+// 2,048 (222 of 128).  Beyond that two workgroups on a compute unit: 21 against 24 for 4,616 x 2,048 x 768, 230
+// against 300 for 74,640 x 2,048 x 768.  Few rows leave most compute units without work, and a strip's time is that of
 // its weights through one of them, at 64 bytes per clock; operands straight to registers take 9.0 for 32 x 2,048 x 768.
 template <int ST>
 hipError_t launch_gated(const Fp8GemmArgs& p, hipStream_t s) {
