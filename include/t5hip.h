@@ -334,6 +334,40 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
                               const void* d_w0_scales, const uint8_t* d_w1, const void* d_w1_scales, int32_t N,
                               int32_t K, int32_t scale_type, uint8_t* d_codes, uint8_t* d_scales, void* stream);
 
+/* ---- Queries and keys between the projection and attention ----
+ * No counterpart in the reference, whose attention has a bias by distance instead.  For encoders whose
+ * queries and keys are normed head by head and rotated by their positions, in one pass:
+ *   z = x / sqrt(mean over the head of x^2 + eps) * gamma       (x itself where gamma is NULL)
+ *   (a, b) -> (a cos t - b sin t, b cos t + a sin t)            for each pair of the first `rot` values
+ * in f32, rounded once to the type.  Pair i holds values i and i + rot / 2 (T5H_ROTARY_HALVES) or 2i and
+ * 2i + 1 (T5H_ROTARY_NEIGHBOURS); the other D - rot values are not turned.  t = position * frequency, pair
+ * i's frequency and the axis whose position it follows (text has one axis; images and video have row and
+ * column, or time, height and width) as the table of t5h_rotary_table holds them. */
+#define T5H_ROTARY_HALVES 0
+#define T5H_ROTARY_NEIGHBOURS 1
+/* Host only: the table of `pairs` frequencies, in radians per step, finite; axis[i] in 0 .. 7, or axis NULL:
+ * all 0.  An entry is the frequency in turns modulo 1, in 61 bits, and the axis in 3, so that angles stay
+ * within 2^-29 radians of position * frequency for every 32-bit position. */
+int t5h_rotary_table(const double* frequency, const int32_t* axis, int32_t pairs, uint64_t* table);
+/* d_q: T rows of q_heads heads of D values each, ldq values from row to row; d_k likewise; so q and k may
+ * be columns of one projection's rows, of which nothing else is read.  Results go to d_q_out and d_k_out,
+ * which may be d_q and d_k themselves with their row lengths, and otherwise share no byte with either.
+ * d_table[rot / 2] as above; d_pos[axes][T] int32, negative ones too, pairs of an axis >= axes are not
+ * turned.  D and rot <= D are multiples of 8, D <= 512, rot may be 0 (no table, no positions needed); axes
+ * 1 .. 8, T <= 2^30, heads of each up to 65,535, 0 for none (its pointers and row lengths are not looked
+ * at).  Rows start on multiples of 16 bytes, gammas on 4.  All buffers lie on the current device; the call
+ * is enqueued on `stream` (a hipStream_t; NULL = the default stream) and returns without waiting.  It
+ * allocates nothing and keeps no state. */
+int t5h_rotary_device(const void* d_q, int64_t ldq, int32_t q_heads, const void* d_k, int64_t ldk, int32_t k_heads,
+                      int32_t type, int32_t T, int32_t D, const float* d_q_gamma, const float* d_k_gamma, float eps,
+                      const uint64_t* d_table, int32_t rot, int32_t pairing, const int32_t* d_pos, int32_t axes,
+                      void* d_q_out, int64_t ldq_out, void* d_k_out, int64_t ldk_out, void* stream);
+/* The same on host buffers, rows without gaps (q[T][q_heads][D], k[T][k_heads][D]), synchronous, on HIP
+ * device hip_device. */
+int t5h_rotary(int32_t hip_device, const void* q, int32_t q_heads, const void* k, int32_t k_heads, int32_t type,
+               int32_t T, int32_t D, const float* q_gamma, const float* k_gamma, float eps, const uint64_t* table,
+               int32_t rot, int32_t pairing, const int32_t* pos, int32_t axes, void* q_out, void* k_out);
+
 /* One T5Block (src/quantized_t5.rs:598-627) on packed sequences: x_in/x_out are
  * host [T, d_model] f32. */
 int t5h_layer_forward(t5h_model* model, int32_t layer, const float* x_in,

@@ -28,6 +28,8 @@ T5H_TYPE_F16 = 1
 T5H_TYPE_BF16 = 2
 T5H_SCALE_E8M0 = 0
 T5H_SCALE_F32 = 1
+T5H_ROTARY_HALVES = 0
+T5H_ROTARY_NEIGHBOURS = 1
 
 
 class T5HConfig(C.Structure):
@@ -106,6 +108,12 @@ SIGNATURES = {
                                      _vp, _vp]),
     "t5h_fp8_gated_gelu_device": (C.c_int, [_vp, _vp, C.c_int32, _vp, _vp, _vp, _vp, C.c_int32, C.c_int32, C.c_int32, _vp,
                                             _vp, _vp]),
+    "t5h_rotary_table": (C.c_int, [_vp, _vp, C.c_int32, _vp]),
+    "t5h_rotary_device": (C.c_int, [_vp, C.c_int64, C.c_int32, _vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                    _vp, _vp, C.c_float, _vp, C.c_int32, C.c_int32, _vp, C.c_int32, _vp, C.c_int64, _vp,
+                                    C.c_int64, _vp]),
+    "t5h_rotary": (C.c_int, [C.c_int32, _vp, C.c_int32, _vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp,
+                             C.c_float, _vp, C.c_int32, C.c_int32, _vp, C.c_int32, _vp, _vp]),
     "t5h_layer_forward": (C.c_int, [_vp, C.c_int32, _f32p, _i32p, C.c_int32, _f32p]),
     "t5h_ffn_block": (C.c_int, [_vp, C.c_int32, _f32p, C.c_int32, _f32p, C.c_int32]),
     "t5h_set_profiling": (C.c_int, [_vp, C.c_int32]),

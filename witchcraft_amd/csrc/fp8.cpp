@@ -1,27 +1,16 @@
 // fp8.cpp -- the C ABI entry points of the 8-bit operators: argument checks, and the host-buffer forms
 // around the launches of k_fp8.hip and k_fp8_gemm.hip.
-#include <hip/hip_runtime.h>
 #include <math.h>
 
-#include <string>
-
-#include "../../include/t5hip.h"
+#include "abi.hpp"
 #include "fp8.hpp"
-
-namespace t5h_detail {
-int fail(int code, const std::string& msg);
-}
 
 namespace {
 
 using t5h_detail::fail;
-
-#define HIP_OK(expr)                                                                   \
-  do {                                                                                 \
-    hipError_t e_ = (expr);                                                            \
-    if (e_ != hipSuccess)                                                              \
-      return fail(T5H_ERR_HIP, std::string(#expr ": ") + hipGetErrorString(e_));       \
-  } while (0)
+using t5h_detail::HostCall;
+using t5h_detail::known_type;
+using t5h_detail::type_bytes;
 
 static_assert(T5H_TYPE_F32 == t5k::FP8_IO_F32 && T5H_TYPE_F16 == t5k::FP8_IO_F16 && T5H_TYPE_BF16 == t5k::FP8_IO_BF16,
               "the kernels take the ABI's type codes");
@@ -29,8 +18,6 @@ static_assert(T5H_SCALE_E8M0 == t5k::FP8_E8M0 && T5H_SCALE_F32 == t5k::FP8_F32, 
 
 constexpr int32_t kMostRows = 1 << 30;
 
-size_t type_bytes(int32_t t) { return t == T5H_TYPE_F32 ? 4 : 2; }
-bool known_type(int32_t t) { return t == T5H_TYPE_F32 || t == T5H_TYPE_F16 || t == T5H_TYPE_BF16; }
 bool known_scale(int32_t t) { return t == T5H_SCALE_E8M0 || t == T5H_SCALE_F32; }
 size_t blocks_of(int32_t n) { return ((size_t)n + t5k::FP8_BLOCK - 1) / t5k::FP8_BLOCK; }
 size_t act_scale_bytes(int32_t M, int32_t K) { return blocks_of(K) * t5k::fp8_scale_rows(M); }
@@ -57,11 +44,6 @@ bool same_or_apart(const void* a, size_t an, const void* b, size_t bn) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return x == y || x + an <= y || y + bn <= x;
 }
-
-#define TRY(expr)                   \
-  do {                              \
-    if (int rc_ = (expr)) return rc_; \
-  } while (0)
 
 int check_quantize(const void* x, int32_t type, int32_t M, int32_t K, const void* codes, const void* scales) {
   TRY(check_shape(M, K));
@@ -128,43 +110,6 @@ int check_gated(const void* a, const void* a_scales, int32_t M, const void* w0, 
   TRY(check_buffer(w1_scales, "up weight scales", scale_type == T5H_SCALE_F32 ? 4 : 1));
   return check_buffer(scales, "scales");
 }
-
-// Device copies of a host call's buffers: one allocation, parts on 256-byte boundaries, freed on every
-// path.  Outputs are cleared first, so that the scales' unused rows come back as zeros.
-struct HostCall {
-  char* p = nullptr;
-  size_t used = 0;
-  HostCall() = default;
-  HostCall(const HostCall&) = delete;
-  HostCall& operator=(const HostCall&) = delete;
-  ~HostCall() {
-    if (p) (void)hipFree(p);
-  }
-  size_t part(size_t bytes) {
-    const size_t at = used;
-    used += (bytes + 255) & ~(size_t)255;
-    return at;
-  }
-  int open(int32_t dev) {
-    int ndev = 0;
-    if (hipGetDeviceCount(&ndev) != hipSuccess || ndev <= 0) return fail(T5H_ERR_NODEVICE, "no HIP device");
-    HIP_OK(hipSetDevice(dev < 0 ? 0 : dev));
-    if (hipMalloc((void**)&p, used) != hipSuccess) {
-      p = nullptr;
-      return fail(T5H_ERR_NOMEM, "fp8 buffers");
-    }
-    HIP_OK(hipMemset(p, 0, used));
-    return T5H_OK;
-  }
-  int up(size_t at, const void* from, size_t bytes) {
-    HIP_OK(hipMemcpy(p + at, from, bytes, hipMemcpyHostToDevice));
-    return T5H_OK;
-  }
-  int down(void* to, size_t at, size_t bytes) {
-    HIP_OK(hipMemcpy(to, p + at, bytes, hipMemcpyDeviceToHost));
-    return T5H_OK;
-  }
-};
 
 t5k::Fp8GemmArgs gemm_args(const void* a, const void* a_scales, int32_t M, const void* w, const void* w_scales, int32_t N,
                            int32_t K, int32_t scale_type, void* out) {
