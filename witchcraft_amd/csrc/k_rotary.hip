@@ -87,112 +87,192 @@ __device__ __forceinline__ float sum_group(float v) {
   return v;
 }
 
-struct Shape {
-  int tokens, heads;  // a workgroup's
-  int step_tokens, step_heads;  // of 256 / L heads, in whole rows of `heads`
+// Queries or keys alone: rows of `heads` heads, and how workgroups share them.
+struct Part {
+  const char* from;
+  char* to;
+  int64_t ld, ld_to;  // bytes from row to row
+  const float* gamma;
+  int heads;
+  int tokens, group;        // rows and heads of a workgroup's share, 256 heads at most in all
+  unsigned per_group;       // 2^16 / group, rounded up: i * per_group >> 16 is i / group for i < 256
+  unsigned groups, blocks;  // groups of heads, workgroups for this part
 };
 
-// A lane holds two chunks of V values of a head, those whose values make pairs: c and c + rot / 2 / V for
-// halves, neighbouring ones otherwise and behind the rotated part; L lanes (a power of two) hold the head.
-// A workgroup walks the heads of some tokens, and computes each token's sines and cosines once, into LDS.
-// What bounds it is memory; a value takes about 10 vector instructions, a third of the memory's time.
-template <int T, int V, int L, bool HALVES>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, Shape w) {
+// Of both parts.
+struct Shared {
+  float inverse;       // 1 / D
+  unsigned per_pairs;  // 2^20 / pairs, rounded up: i * per_pairs >> 20 is i / pairs for i < 2,048
+};
+
+// x1 of the lower four lanes of each eight and x0 of the upper four change places.
+template <int WORDS>
+__device__ __forceinline__ void swap_quads(uint32_t* x0, uint32_t* x1) {
+#pragma unroll
+  for (int i = 0; i < WORDS; i++) {
+    const int a = (int)x0[i], b = (int)x1[i];
+    x1[i] = (uint32_t)__builtin_amdgcn_update_dpp(b, a, 0x104, 0xf, 0x5, false);  // lane + 4 to the lower four
+    x0[i] = (uint32_t)__builtin_amdgcn_update_dpp(a, b, 0x114, 0xf, 0xa, false);  // lane - 4 to the upper four
+  }
+}
+
+// Workgroups [0, q.blocks) take the queries, the others the keys.  A lane holds two chunks of V values of a head,
+// c and c + rot / 2 / V, which are pairs in the one form and contain them in the other, and neighbouring chunks
+// behind the rotated part; L lanes (a power of two) hold the head.  A workgroup walks the heads of some rows, the next
+// head's values on their way while one is turned, and computes each row's sines and cosines once, into LDS.
+// What bounds it is memory, and for few rows a launch and two trips to it: 16,391 x (32 + 8) heads of 128 in bf16, three
+// axes, norms: 71 us, 4.7 TB/s; one row of it 3.8 us.  Stores go past the caches: 20.9 instead of 27.1 us for 10,007 x
+// (16 + 16) heads of 80 whose input the last-level cache does not hold.
+// EIGHT: heads of eight chunks, all turned, would be loaded and stored in halves of 64 bytes (74,640 x (12 + 12) heads of
+// 64 in f16 with norms: 106 us, 4.3 TB/s); there eight lanes load a head's chunks into x0 and the next head's into x1,
+// and the quads of lanes swap (93 us, 4.9 TB/s).
+template <int T, int V, int L, bool HALVES, bool EIGHT>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, Shared u, Part q, Part k) {
   extern __shared__ f4 lds[];
   float* turns = (float*)lds;  // [tokens][2][pairs]: cosines, sines
+  typedef Chunk<T, V> C;
+  constexpr int SIZE = T == FP8_IO_F32 ? 4 : 2, PIECE = V * SIZE, STEP = 256 / L, WORDS = PIECE / 4;
+  const bool is_q = blockIdx.x < q.blocks;
+  const Part& w = is_q ? q : k;
+  const unsigned block = is_q ? blockIdx.x : blockIdx.x - q.blocks, stride = w.blocks / w.groups;
   const int pairs = a.rot / 2, unit = threadIdx.x & (L - 1), slot = threadIdx.x / L;
   const int n = a.D / V, m = pairs / V;  // chunks of a head, chunks of a half of its rotated part
-  const bool turned = unit < m, first_ok = 2 * unit < n;
-  const int c0 = HALVES && turned ? unit : 2 * unit, c1 = HALVES && turned ? unit + m : 2 * unit + 1;
-  const bool second_ok = c1 < n && first_ok;
-  const int h_first = blockIdx.y * w.heads, h_last = min(h_first + w.heads, a.q_heads + a.k_heads);
-  const size_t size = T == FP8_IO_F32 ? 4 : 2;
-  float gq[2 * V], gk[2 * V];
+  const bool turned = unit < m, first_ok = EIGHT || 2 * unit < n;
+  const int c0 = turned ? unit : 2 * unit, c1 = turned ? unit + m : 2 * unit + 1;
+  const bool second_ok = EIGHT || (c1 < n && first_ok);
+  const int h0 = (int)(block % w.groups) * w.group, group = min(w.group, w.heads - h0);
+  const int head = a.D * SIZE;
+  // what a lane loads and stores: chunk l0 of item i + d0 and chunk l1 of item i + d1
+  const int l0 = (EIGHT ? (int)(threadIdx.x & 7) : c0) * PIECE, l1 = (EIGHT ? (int)(threadIdx.x & 7) : c1) * PIECE;
+  const int d0 = EIGHT ? -(slot & 1) : 0, d1 = EIGHT ? 1 - (slot & 1) : 0;
+  for (int64_t t0 = (int64_t)(block / w.groups) * w.tokens; t0 < a.T; t0 += (int64_t)stride * w.tokens) {
+    const int tokens = (int)min((int64_t)w.tokens, a.T - t0), items = tokens * w.group;
+    const char* from = w.from + t0 * w.ld + (int64_t)h0 * head;
+    char* to = w.to + t0 * w.ld_to + (int64_t)h0 * head;
+    const auto place = [&](int i, int64_t ld, int64_t& at) {  // of item i; whether there is one
+      const int t = (int)((unsigned)i * w.per_group >> 16), h = i - t * w.group;
+      at = t * ld + h * head;
+      return i < items && h < group;
+    };
+    const auto load = [&](int i, C& x0, C& x1) {
+      int64_t at;
+      const bool ok = place(i + d0, w.ld, at);
+      if (ok && first_ok) x0 = *(const C*)(from + at + l0);
+      const bool ok1 = EIGHT ? place(i + d1, w.ld, at) : ok;
+      if (ok1 && second_ok) x1 = *(const C*)(from + at + l1);
+    };
+    C x0{}, x1{};
+    load(slot, x0, x1);
+    float g[2 * V];
+    if (w.gamma) {
 #pragma unroll
-  for (int e = 0; e < 2 * V; e++) {
-    const bool ok = e < V ? first_ok : second_ok;
-    const int at = (e < V ? c0 * V + e : c1 * V + e - V);
-    gq[e] = ok && a.q_gamma ? a.q_gamma[at] : 1.f;
-    gk[e] = ok && a.k_gamma ? a.k_gamma[at] : 1.f;
-  }
-  for (int64_t t0 = (int64_t)blockIdx.x * w.tokens; t0 < a.T; t0 += (int64_t)gridDim.x * w.tokens) {
-    const int tokens = (int)min((int64_t)w.tokens, a.T - t0);
+      for (int e = 0; e < 2 * V; e++) g[e] = (e < V ? first_ok : second_ok) ? w.gamma[(e < V ? c0 : c1 - 1) * V + e] : 0.f;
+    }
     for (int i = threadIdx.x; i < tokens * pairs; i += 256) {
-      const int t = i / pairs, p = i - t * pairs;
+      const int r = (int)((unsigned)i * u.per_pairs >> 20), p = i - r * pairs;
       const uint64_t entry = a.table[p];
       const int axis = (int)(entry & (ROTARY_MAX_AXES - 1));
-      const int32_t at = axis < a.axes ? a.pos[(size_t)axis * a.T + t0 + t] : 0;
-      const uint64_t turn = (uint64_t)(int64_t)at * (entry & ~(uint64_t)(ROTARY_MAX_AXES - 1));
+      int32_t pos;
+      if (a.axes == 1) {  // on its way together with the table's entry
+        pos = a.pos[t0 + r];
+        if (axis) pos = 0;
+      } else {
+        pos = axis < a.axes ? a.pos[(size_t)axis * a.T + t0 + r] : 0;
+      }
+      const uint64_t turn = (uint64_t)(int64_t)pos * (entry & ~(uint64_t)(ROTARY_MAX_AXES - 1));
       float s, c;
       sincos_turn((uint32_t)(turn >> 32), s, c);
-      turns[2 * t * pairs + p] = c;
-      turns[(2 * t + 1) * pairs + p] = s;
+      turns[2 * r * pairs + p] = c;
+      turns[(2 * r + 1) * pairs + p] = s;
     }
     __syncthreads();
-    int t = slot / w.heads, h = h_first + slot - t * w.heads;
-    while (t < tokens) {
-      if (h < h_last) {
-        const bool is_q = h < a.q_heads;
-        const int hh = is_q ? h : h - a.q_heads;
-        const char* from = (const char*)(is_q ? a.q : a.k) + ((size_t)(t0 + t) * (is_q ? a.ldq : a.ldk) + (size_t)hh * a.D) * size;
-        char* to = (char*)(is_q ? a.q_out : a.k_out) + ((size_t)(t0 + t) * (is_q ? a.ldq_out : a.ldk_out) + (size_t)hh * a.D) * size;
-        Chunk<T, V> x0{}, x1{};
-        if (first_ok) x0 = *(const Chunk<T, V>*)(from + c0 * V * size);
-        if (second_ok) x1 = *(const Chunk<T, V>*)(from + c1 * V * size);
-        float v[2 * V];
-        x0.get(v), x1.get(v + V);
-        if (is_q ? a.q_gamma != nullptr : a.k_gamma != nullptr) {
-          float ss = 0.f;
+    for (int i0 = 0; i0 < items; i0 += STEP) {
+      C y0{}, y1{};
+      load(i0 + STEP + slot, y0, y1);
+      if constexpr (EIGHT) swap_quads<WORDS>((uint32_t*)&x0.raw, (uint32_t*)&x1.raw);
+      float v[2 * V];
+      x0.get(v), x1.get(v + V);
+      if (w.gamma) {
+        float ss = 0.f;
 #pragma unroll
-          for (int e = 0; e < 2 * V; e++) ss = __builtin_fmaf(v[e], v[e], ss);
-          const float rs = rsqrtf(sum_group<L>(ss) / (float)a.D + a.eps);
+        for (int e = 0; e < 2 * V; e++) ss = __builtin_fmaf(v[e], v[e], ss);
+        const float rs = rsqrtf(__builtin_fmaf(sum_group<L>(ss), u.inverse, a.eps));
 #pragma unroll
-          for (int e = 0; e < 2 * V; e++) v[e] *= rs * (is_q ? gq[e] : gk[e]);
-        }
-        if (turned) {
-          float cs[V], sn[V];
+        for (int e = 0; e < 2 * V; e++) v[e] *= rs * g[e];
+      }
+      if (turned) {
+        // halves: pair e is (c0's, c1's) value e; neighbours: two values of c0, then of c1
+        const int t = min((int)((unsigned)(i0 + slot) * w.per_group >> 16), tokens - 1);
+        const float* cs = turns + 2 * t * pairs;
+        constexpr int W = HALVES ? 4 : V / 2;
+        typedef float fw __attribute__((ext_vector_type(W)));
 #pragma unroll
-          for (int e = 0; e < V; e += 4) {
-            *(f4*)(cs + e) = *(const f4*)(turns + 2 * t * pairs + unit * V + e);
-            *(f4*)(sn + e) = *(const f4*)(turns + (2 * t + 1) * pairs + unit * V + e);
-          }
+        for (int i = 0; i < V; i += W) {
+          const int p = HALVES ? c0 * V + i : (i == 0 ? c0 : c1) * W;
+          const fw cw = *(const fw*)(cs + p), sw = *(const fw*)(cs + pairs + p);
 #pragma unroll
-          for (int e = 0; e < V; e++) {
+          for (int e = i; e < i + W; e++) {
             float& x = v[HALVES ? e : 2 * e];
             float& y = v[HALVES ? e + V : 2 * e + 1];
-            const float c = cs[e], s = sn[e], r = x * c - y * s;
+            const float c = cw[e - i], s = sw[e - i], r = x * c - y * s;
             y = y * c + x * s;
             x = r;
           }
         }
-        x0.set(v), x1.set(v + V);
-        if (first_ok) *(Chunk<T, V>*)(to + c0 * V * size) = x0;
-        if (second_ok) *(Chunk<T, V>*)(to + c1 * V * size) = x1;
       }
-      t += w.step_tokens, h += w.step_heads;
-      if (h - h_first >= w.heads) h -= w.heads, t++;
+      x0.set(v), x1.set(v + V);
+      if constexpr (EIGHT) swap_quads<WORDS>((uint32_t*)&x0.raw, (uint32_t*)&x1.raw);
+      int64_t at;
+      const bool ok = place(i0 + slot + d0, w.ld_to, at);
+      if (ok && first_ok) __builtin_nontemporal_store(x0.raw, &((C*)(to + at + l0))->raw);
+      const bool ok1 = EIGHT ? place(i0 + slot + d1, w.ld_to, at) : ok;
+      if (ok1 && second_ok) __builtin_nontemporal_store(x1.raw, &((C*)(to + at + l1))->raw);
+      x0 = y0, x1 = y1;
     }
-    __syncthreads();  // the next tokens' sines take this one's place
+    __syncthreads();  // the next rows' sines take this one's place
   }
+}
+
+// How the workgroups share `heads` heads of T rows, `step` heads at a time.
+Part share(const RotaryArgs& a, const void* from, int64_t ld, void* to, int64_t ld_to, const float* gamma, int heads, int step) {
+  const int size = a.type == FP8_IO_F32 ? 4 : 2, pairs = a.rot / 2;
+  Part w{};
+  w.from = (const char*)from, w.to = (char*)to;
+  w.ld = ld * size, w.ld_to = ld_to * size;
+  w.gamma = gamma;
+  w.heads = heads;
+  w.group = w.groups = 1;
+  if (heads == 0) return w;
+  // Up to four rounds of a workgroup's lanes while that leaves 400 workgroups a part.  4,616 x (12 + 12) heads of 64 in
+  // f16: 7.8 us at two rounds, 8.7 at one; 10,007 x (16 + 16) heads of 80 in bf16 21.7 at four, 20.9 at two.
+  const int want = step * (int)std::min<int64_t>(4, std::max<int64_t>(1, (int64_t)a.T * heads / (400 * step)));
+  w.group = std::min(heads, want);
+  w.tokens = std::max(1, want / w.group);
+  if (pairs > 0) w.tokens = std::min(w.tokens, std::max(1, 4096 / (2 * pairs)));  // 16 KiB of sines
+  w.tokens = std::min(w.tokens, a.T);
+  w.per_group = (65536 + w.group - 1) / w.group;
+  w.groups = (unsigned)((heads + w.group - 1) / w.group);
+  const unsigned most = std::max(1u, (1u << 20) / w.groups);  // workgroups for a group; they walk what is left
+  w.blocks = w.groups * std::min((unsigned)(((int64_t)a.T + w.tokens - 1) / w.tokens), most);
+  return w;
 }
 
 template <int T, int V, int L>
 hipError_t launch(const RotaryArgs& a, int pairing, hipStream_t s) {
-  const int heads = a.q_heads + a.k_heads, pairs = a.rot / 2, step = 256 / L;
-  // Heads per workgroup: four rounds of its lanes, one where that leaves workgroups for every compute unit.
-  const int64_t all = (int64_t)a.T * heads;
-  const int want = all < (int64_t)1024 * step ? step : 4 * step;
-  Shape w{};
-  w.heads = std::min(heads, want);
-  w.tokens = std::max(1, want / heads);
-  if (pairs > 0) w.tokens = std::min(w.tokens, std::max(1, 4096 / (2 * pairs)));  // 16 KiB of sines
-  w.tokens = (int)std::min<int64_t>(w.tokens, a.T);
-  w.step_tokens = step / w.heads;
-  w.step_heads = step % w.heads;
-  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.T + w.tokens - 1) / w.tokens, 1 << 20), (heads + w.heads - 1) / w.heads);
-  const size_t lds = (size_t)w.tokens * 2 * pairs * 4;
-  if (pairing == ROTARY_HALVES) T5K_LAUNCH((rotary_kernel<T, V, L, true>), grid, dim3(256), lds, s, a, w);
-  else T5K_LAUNCH((rotary_kernel<T, V, L, false>), grid, dim3(256), lds, s, a, w);
+  const Part q = share(a, a.q, a.ldq, a.q_out, a.ldq_out, a.q_gamma, a.q_heads, 256 / L);
+  const Part k = share(a, a.k, a.ldk, a.k_out, a.ldk_out, a.k_gamma, a.k_heads, 256 / L);
+  const Shared u{1.f / (float)a.D, a.rot ? (unsigned)((1 << 20) + a.rot / 2 - 1) / (unsigned)(a.rot / 2) : 0u};
+  const dim3 grid(q.blocks + k.blocks);
+  const size_t lds = (size_t)std::max(q.tokens, k.tokens) * a.rot * 4;
+  if constexpr (L == 4) {
+    if (a.D == 8 * V && a.rot == a.D) {
+      if (pairing == ROTARY_HALVES) T5K_LAUNCH((rotary_kernel<T, V, L, true, true>), grid, dim3(256), lds, s, a, u, q, k);
+      else T5K_LAUNCH((rotary_kernel<T, V, L, false, true>), grid, dim3(256), lds, s, a, u, q, k);
+      return hipGetLastError();
+    }
+  }
+  if (pairing == ROTARY_HALVES) T5K_LAUNCH((rotary_kernel<T, V, L, true, false>), grid, dim3(256), lds, s, a, u, q, k);
+  else T5K_LAUNCH((rotary_kernel<T, V, L, false, false>), grid, dim3(256), lds, s, a, u, q, k);
   return hipGetLastError();
 }
 template <int T, int V>
