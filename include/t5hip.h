@@ -334,6 +334,44 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
                               const void* d_w0_scales, const uint8_t* d_w1, const void* d_w1_scales, int32_t N,
                               int32_t K, int32_t scale_type, uint8_t* d_codes, uint8_t* d_scales, void* stream);
 
+/* ---- Low-rank adapters beside a shared projection ----
+ * No counterpart in the reference, whose encoder has one set of weights.  The rows of a packed batch belong
+ * to requests of which each has an adapter of its own, or none; the shared product y = x W^T (t5h_fp8_matmul
+ * or any other) is the same for all, and these calls add what the adapters say, for all of them at once:
+ *   out[t][n] = y[t][n] + scale_g sum_r (sum_k x[t][k] A_g[s R + r][k]) B_g[n][r],    g = ids[t]
+ * ids[t] outside 0 .. G - 1 (-1, say): the row has no adapter, out[t] is y[t], bit for bit.  Rows of one adapter are fastest
+ * where they follow each other.  Columns come in `slices` (1 .. 4, as q, k and v of a fused projection), each
+ * with its own A: column n of slice s takes ranks s R .. s R + R - 1 of A.
+ *   x: [T] rows of K values, ldx from row to row, of the adapters' type, or e4m3 codes (T5H_TYPE_E4M3) with
+ *      scales as t5h_fp8_quantize and t5h_fp8_rmsnorm write them (what the shared product takes).
+ *   a: [G][slices][R][K], b: [G][N][R], f16 or bf16, N = the sum of cols[slices] (a HOST array).
+ *   ranks: [G] or NULL (all R): adapter g has ranks[g] <= R ranks; past those, up to a multiple of 8, its a
+ *      and b hold zeros, and what lies behind is not read.  Values outside 0 .. R count as the nearer of both.
+ *   scales: [G] f32, or NULL (all 1).
+ *   y, out: [T] rows of N values in f32, f16 or bf16; out may be y itself with its row length, or share no
+ *      byte with it.  Rows without an adapter are then not touched.
+ * Sums are f32, and so is the inner product, which goes to the matrix units in two or three 16-bit parts
+ * (within 2^-17 of it for bf16 adapters under 16-bit results, 2^-22 otherwise); results are rounded once.
+ * Adapters are finite; an infinity or NaN in a row stays in that row.
+ * K is a multiple of 16 up to 2^21, R one of 8 up to 128, columns of a slice one of 16 up to 2^24; T up to
+ * 2^30, G up to 2^24.  Rows of x, y and out start on multiples of 16 bytes and are up to 2^30 values apart; a,
+ * b and the workspace start on 16 bytes.  Device buffers lie on the current device; the call is enqueued on `stream`
+ * (a hipStream_t; NULL = the default stream) and returns without waiting.  It allocates nothing and keeps no
+ * state: intermediate sums live in d_work, of at least t5h_adapter_workspace's bytes, which serves one call
+ * (or replay of a graph that holds one) at a time. */
+#define T5H_TYPE_E4M3 3
+int t5h_adapter_workspace(int32_t T, int32_t K, int32_t slices, int32_t R, size_t* bytes);
+int t5h_adapter_add_device(const void* d_x, int32_t x_type, const uint8_t* d_x_scales, int64_t ldx, int32_t T, int32_t K,
+                           const int32_t* d_ids, int32_t G, const void* d_a, const void* d_b, int32_t w_type,
+                           const int32_t* d_ranks, const float* d_scales, int32_t R, const int32_t* cols, int32_t slices,
+                           const void* d_y, int64_t ldy, void* d_out, int64_t ldo, int32_t y_type, void* d_work,
+                           size_t work_bytes, void* stream);
+/* The same on host buffers, rows without gaps, synchronous, on HIP device hip_device. */
+int t5h_adapter_add(int32_t hip_device, const void* x, int32_t x_type, const uint8_t* x_scales, int32_t T, int32_t K,
+                    const int32_t* ids, int32_t G, const void* a, const void* b, int32_t w_type, const int32_t* ranks,
+                    const float* scales, int32_t R, const int32_t* cols, int32_t slices, const void* y, void* out,
+                    int32_t y_type);
+
 /* ---- Queries and keys between the projection and attention ----
  * No counterpart in the reference, whose attention has a bias by distance instead.  For encoders whose
  * queries and keys are normed head by head and rotated by their positions, in one pass:

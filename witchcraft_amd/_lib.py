@@ -26,6 +26,7 @@ T5H_NUMERICS_HYBRID_BF16 = 2
 T5H_TYPE_F32 = 0
 T5H_TYPE_F16 = 1
 T5H_TYPE_BF16 = 2
+T5H_TYPE_E4M3 = 3
 T5H_SCALE_E8M0 = 0
 T5H_SCALE_F32 = 1
 T5H_ROTARY_HALVES = 0
@@ -108,6 +109,12 @@ SIGNATURES = {
                                      _vp, _vp]),
     "t5h_fp8_gated_gelu_device": (C.c_int, [_vp, _vp, C.c_int32, _vp, _vp, _vp, _vp, C.c_int32, C.c_int32, C.c_int32, _vp,
                                             _vp, _vp]),
+    "t5h_adapter_workspace": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
+    "t5h_adapter_add_device": (C.c_int, [_vp, C.c_int32, _vp, C.c_int64, C.c_int32, C.c_int32, _vp, C.c_int32, _vp, _vp,
+                                         C.c_int32, _vp, _vp, C.c_int32, _vp, C.c_int32, _vp, C.c_int64, _vp, C.c_int64,
+                                         C.c_int32, _vp, C.c_size_t, _vp]),
+    "t5h_adapter_add": (C.c_int, [C.c_int32, _vp, C.c_int32, _vp, C.c_int32, C.c_int32, _vp, C.c_int32, _vp, _vp, C.c_int32,
+                                  _vp, _vp, C.c_int32, _vp, C.c_int32, _vp, _vp, C.c_int32]),
     "t5h_rotary_table": (C.c_int, [_vp, _vp, C.c_int32, _vp]),
     "t5h_rotary_device": (C.c_int, [_vp, C.c_int64, C.c_int32, _vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                     _vp, _vp, C.c_float, _vp, C.c_int32, C.c_int32, _vp, C.c_int32, _vp, C.c_int64, _vp,

@@ -26,6 +26,23 @@ int fail(int code, const std::string& msg);
 inline size_t type_bytes(int32_t t) { return t == T5H_TYPE_F32 ? 4 : 2; }
 inline bool known_type(int32_t t) { return t == T5H_TYPE_F32 || t == T5H_TYPE_F16 || t == T5H_TYPE_BF16; }
 
+// Rows of `width` bytes, `stride` bytes apart.
+struct Rows {
+  uintptr_t at;
+  uint64_t width, stride;
+  const char* name;
+};
+// Whether some row of a shares a byte with some row of b: rows of one stride, by where the second's lie
+// between the first's; otherwise by all that the rows span.
+inline bool overlap(const Rows& a, const Rows& b, uint64_t rows) {
+  const uintptr_t a_end = a.at + (rows - 1) * a.stride + a.width, b_end = b.at + (rows - 1) * b.stride + b.width;
+  if (a_end <= b.at || b_end <= a.at) return false;
+  if (rows == 1 || a.stride != b.stride) return true;
+  const uint64_t d = a.at <= b.at ? (b.at - a.at) % a.stride : (a.stride - (a.at - b.at) % a.stride) % a.stride;
+  return d < a.width || d + b.width > a.stride;
+}
+
+
 // Device copies of a host call's buffers: one allocation, parts on 256-byte boundaries, freed on every
 // path.  Outputs are cleared first, so that the scales' unused rows come back as zeros.
 struct HostCall {

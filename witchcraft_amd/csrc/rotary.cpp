@@ -11,6 +11,8 @@ namespace {
 using t5h_detail::fail;
 using t5h_detail::HostCall;
 using t5h_detail::known_type;
+using t5h_detail::overlap;
+using t5h_detail::Rows;
 using t5h_detail::type_bytes;
 
 static_assert(T5H_ROTARY_HALVES == t5k::ROTARY_HALVES && T5H_ROTARY_NEIGHBOURS == t5k::ROTARY_NEIGHBOURS,
@@ -34,28 +36,12 @@ int check_shape(int32_t q_heads, int32_t k_heads, int32_t type, int32_t T, int32
   return T5H_OK;
 }
 
-// `rows` rows of `width` bytes, `stride` bytes apart.
-struct Rows {
-  uintptr_t at;
-  uint64_t width, stride;
-  const char* name;
-};
 int check_rows(const Rows& r, int64_t ld, int64_t heads_width) {
   if (!r.at) return bad(std::string("NULL ") + r.name);
   if (r.at % 16 || r.stride % 16) return bad(std::string(r.name) + "'s rows must start on 16 bytes");
   if (ld < heads_width || ld > kMostStride) return bad(std::string(r.name) + "'s rows must be as long as its heads, up to 2^30 apart");
   return T5H_OK;
 }
-// Whether some row of a shares a byte with some row of b: rows of one stride, by where the second's lie
-// between the first's; otherwise by all that the rows span.
-bool overlap(const Rows& a, const Rows& b, uint64_t rows) {
-  const uintptr_t a_end = a.at + (rows - 1) * a.stride + a.width, b_end = b.at + (rows - 1) * b.stride + b.width;
-  if (a_end <= b.at || b_end <= a.at) return false;
-  if (rows == 1 || a.stride != b.stride) return true;
-  const uint64_t d = a.at <= b.at ? (b.at - a.at) % a.stride : (a.stride - (a.at - b.at) % a.stride) % a.stride;
-  return d < a.width || d + b.width > a.stride;
-}
-
 }  // namespace
 
 extern "C" {
