@@ -25,9 +25,8 @@ struct AdapterArgs {
   void* out;
   int64_t ldy, ldo;  // values
   int y_type;
-  float* h;  // [splits][T][S R]
+  void* h;  // bf16 [T][S][2 or 3 parts][R], or for few rows f32 [splits][T][S R]
 };
-// Parts of K that separate workgroups sum, each into its own part of h.
-int adapter_splits(int T, int K, int SR);
+size_t adapter_work_bytes(int T, int K, int SR);
 hipError_t launch_adapter(const AdapterArgs& a, hipStream_t s);
 }  // namespace t5k
