@@ -24,11 +24,13 @@ namespace {
 using namespace t5k;
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int ROWS = 16;        // of a matrix instruction
-constexpr int STEP = 64;        // K values of a step
-constexpr int DOWN_WAVES = 8;   // waves of a workgroup of the first product, at most
+constexpr int STEP = 128;       // K values of a step of the first product
+constexpr int FEW_STEP = 64;    // of the one for few rows
+constexpr int FEW_WAVES = 8;    // its waves, at most
 constexpr int COLS = 64;        // columns of a wave in the second product
 constexpr int UP_WAVES = 4;     // its waves, on columns beside each other
 
@@ -70,10 +72,15 @@ struct Adapters {
 #pragma unroll
     for (int i = 0; i < NT; i++) {
       const int64_t row = row0 + ROWS * i + (threadIdx.x & 15);
-      const int v = row < p.T ? p.ids[row] : -1;
-      id[i] = (unsigned)v < (unsigned)p.G ? v : -1;
+      const int v = p.ids[min(row, (int64_t)p.T - 1)];
+      id[i] = row < p.T && (unsigned)v < (unsigned)p.G ? v : -1;
       pending[i] = id[i] >= 0;
     }
+  }
+  // from the lane's id of row l % 16
+  __device__ __forceinline__ Adapters(const AdapterArgs& p, int64_t first, int v) : row0(first) {
+    id[0] = row0 + (threadIdx.x & 15) < p.T && (unsigned)v < (unsigned)p.G ? v : -1;
+    pending[0] = id[0] >= 0;
   }
   __device__ __forceinline__ void only(int row) {
     const int first = __builtin_amdgcn_readlane(id[0], row);
@@ -118,144 +125,200 @@ __device__ __forceinline__ uint32_t next_part(float& v, bool last_of_two) {
   return part;
 }
 
-// ---- h = scale x A^T: 16 NT rows x 16 RT ranks per workgroup, its waves on 64 K values in turn ----
-// Lane (r = lane % 16, g = lane / 16) holds row r's K values 16 g .. + 15 of a step, so that four lanes read a whole
-// line of 16-bit values or half of one of codes; the next step's are on their way while one is multiplied.  The waves'
-// sums meet in LDS and are added in wave order.  With JOIN, for few rows, workgroups split K further, and leave their
-// sums in f32 for the second product to add.
-template <bool CODES, bool BF, int NT, int RT>
-struct DownStep {
-  u4 w[RT][2], x[NT][CODES ? 1 : 2];
-  uint32_t scale[NT];
+// ---- h = scale x A^T, few rows: 16 rows x 16 ranks per workgroup, its waves on 64 K values in turn ----
+// Lane (r = lane % 16, g = lane / 16) holds row r's K values 16 g .. + 15 of a step, the next step's are on their way
+// while one is multiplied.  The waves' sums meet in LDS and are added in wave order.  Workgroups split K further, and
+// leave their sums in f32 for the second product to add; each takes one adapter of the sixteen rows.
+template <bool CODES>
+struct FewStep {
+  u4 w[2], x[CODES ? 1 : 2];
+  uint32_t scale;
   bool ok;
 };
-constexpr int down_occupancy(int NT, int RT) { return NT * RT <= 2 ? 4 : (NT * RT <= 8 ? 3 : 2); }  // waves a SIMD
-
-template <bool CODES, bool BF, int NT, int RT, bool JOIN>
-__global__ __launch_bounds__(64 * DOWN_WAVES, down_occupancy(NT, RT)) void adapter_down_kernel(AdapterArgs p, int splits, int parts) {
-  extern __shared__ f4 red[];  // [waves][NT * RT][64], where there is more than one
+template <bool CODES, bool BF>
+__global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(AdapterArgs p, int splits) {
+  __shared__ f4 red[FEW_WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int SR = p.S * p.R, steps = (p.K + STEP - 1) / STEP, waves = (int)(blockDim.x >> 6);
-  const int split = JOIN ? (int)blockIdx.y % splits : 0, group = JOIN ? (int)blockIdx.y / splits : (int)blockIdx.y;
-  const int first = split * waves + wave, stride = splits * waves;
+  const int SR = p.S * p.R, steps = (p.K + FEW_STEP - 1) / FEW_STEP, waves = (int)(blockDim.x >> 6);
+  const int split = (int)blockIdx.y % splits, group = (int)blockIdx.y / splits;
   const size_t m16 = fp8_scale_rows(p.T);
-  const int64_t tiles = ((int64_t)p.T + ROWS * NT - 1) / (ROWS * NT);
+  const int64_t row0 = (int64_t)blockIdx.x * ROWS;
+  Adapters<1> ad(p, row0);
+  ad.only((int)blockIdx.z);
+  if (!ad.next()) return;
+  const float scale = p.scales ? p.scales[ad.current] : 1.f;
+  const int j0 = ROWS * group, rank = rank_of(p, ad.current);
+  const int64_t at = ad.source(0);
+  const uint16_t* arow = (const uint16_t*)p.a + ((size_t)ad.current * SR + min(j0 + r, SR - 1)) * p.K;
+  // loads are unconditional, past the rows' end from their start
+  const auto load = [&](FewStep<CODES>& v, int n) {
+    const int k0 = n * FEW_STEP + 16 * g, k = k0 < p.K ? k0 : 0;
+    const int block = min(n, steps - 1) / (FP8_BLOCK / FEW_STEP);  // of the scales: the same for all lanes
+    if constexpr (CODES) {
+      v.x[0] = *(const u4*)((const uint8_t*)p.x + at * p.ldx + k);
+      v.scale = p.x_scales[(size_t)block * m16 + at];
+    } else {
+      const uint16_t* from = (const uint16_t*)p.x + at * p.ldx + k;
+      v.x[0] = *(const u4*)from;
+      v.x[1] = *(const u4*)(from + 8);
+    }
+    v.w[0] = *(const u4*)(arow + k);
+    v.w[1] = *(const u4*)(arow + k + 8);
+    v.ok = k0 < p.K;
+  };
+  f4 acc = f4{0.f, 0.f, 0.f, 0.f};
+  FewStep<CODES> u;
+  load(u, split * waves + wave);
+#pragma unroll 2
+  for (int n = split * waves + wave; n < steps; n += splits * waves) {
+    FewStep<CODES> v;
+    load(v, n + splits * waves);
+    const u4 zero = u4{0, 0, 0, 0};
+    const u4 x = u.ok ? u.x[0] : zero;
+    if constexpr (CODES) {
+      f4 t = mfma<BF>(u.w[0], widen8<BF>(x[0], x[1]), f4{0.f, 0.f, 0.f, 0.f});
+      t = mfma<BF>(u.w[1], widen8<BF>(x[2], x[3]), t);
+      const float f = e8m0_value(u.scale);
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(t[e], f, acc[e]);
+    } else {
+      acc = mfma<BF>(u.w[0], x, acc);
+      acc = mfma<BF>(u.w[1], u.ok ? u.x[CODES ? 0 : 1] : zero, acc);
+    }
+    u = v;
+  }
+  red[wave][lane] = acc;
+  __syncthreads();
+  const int j = j0 + 4 * g;
+  if (wave != 0 || ad.id[0] != ad.current || j >= SR) return;
+  for (int k = 1; k < waves; k++) acc += red[k][lane];
+  // ranks past the adapter's own may come from anything
+#pragma unroll
+  for (int e = 0; e < 4; e++) acc[e] = j % p.R < rank ? acc[e] * scale : 0.f;
+  *(f4*)((float*)p.h + ((size_t)split * p.T + row0 + r) * SR + j) = acc;
+}
+
+// ---- h = scale x A^T, many rows: 64 rows x 16 RT ranks per workgroup --------------------------------
+// 4 KG waves: four of sixteen rows each, KG times over, on steps of 128 K in turn.  A goes through LDS, loaded in whole
+// rows by the four waves that share it and read in the operand's order; a row's sixteen 16-byte chunks are stored
+// rotated (xor) by its number, so that sixteen rows at once spread over all banks.  x goes straight to registers,
+// where the lanes of a load lie in sixteen rows: that costs the address unit a quarter of its rate, which x alone can
+// bear.  The next step's loads are on their way while one is multiplied.  The KG sums meet in LDS and are added in order.
+template <bool CODES, bool BF, int RT, int KG>
+__global__ __launch_bounds__(256 * KG, KG == 1 ? 3 : 4) void adapter_down_kernel(AdapterArgs p, int parts) {
+  constexpr int BUFFER = RT * ROWS * STEP * 2;  // bytes of A's ranks of a step
+  extern __shared__ char lds[];                 // [KG][2][BUFFER]; the sums: [KG][4][RT][64] f4, no more
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int rw = wave & 3, kg = wave >> 2, tid = threadIdx.x & 255;
+  const int SR = p.S * p.R, steps = (p.K + STEP - 1) / STEP, group = (int)blockIdx.y;
+  const size_t m16 = fp8_scale_rows(p.T);
+  const int64_t tiles = ((int64_t)p.T + 4 * ROWS - 1) / (4 * ROWS);
+  char* mine = lds + kg * 2 * BUFFER;
+  const u4 zero = u4{0, 0, 0, 0};
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t row0 = tile * ROWS * NT;
-    Adapters<NT> ad(p, row0);
-    if (JOIN) ad.only((int)blockIdx.z);
-    while (ad.next()) {
-      int64_t at[NT];  // the lane's rows of x
-#pragma unroll
-      for (int i = 0; i < NT; i++) at[i] = ad.source(i);
+    const int64_t row0 = tile * 4 * ROWS;
+    Adapters<4> ad(p, row0);
+    for (unsigned seen = 0; ad.next(); seen++) {
+      if (seen % gridDim.z != blockIdx.z) continue;
       const float scale = p.scales ? p.scales[ad.current] : 1.f;
-      // ranks past the adapter's own give results that nothing keeps
       const int rank = rank_of(p, ad.current);
-      const uint16_t* arow[RT];
-#pragma unroll
-      for (int q = 0; q < RT; q++) {
-        const int j = ROWS * (group * RT + q) + r;
-        arow[q] = (const uint16_t*)p.a + ((size_t)ad.current * SR + min(j, SR - 1)) * p.K;
-      }
-      f4 acc[NT][RT];
-#pragma unroll
-      for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int q = 0; q < RT; q++) acc[i][q] = f4{0.f, 0.f, 0.f, 0.f};
-      typedef DownStep<CODES, BF, NT, RT> Step;
-      // loads are unconditional, past the rows' end from their start: a branch around each would cost registers, and
-      // the addresses of results are left to be computed behind the loop for the same reason
+      const int id = rw == 0 ? ad.id[0] : (rw == 1 ? ad.id[1] : (rw == 2 ? ad.id[2] : ad.id[3]));
+      const int64_t row = row0 + ROWS * rw + r;
+      const int64_t at = id == ad.current ? row : ad.row;  // of rows whose result nothing keeps, one that is read anyway
+      const uint16_t* a = (const uint16_t*)p.a + (size_t)ad.current * SR * p.K;
+      struct Step {
+        u4 a[RT], x[CODES ? 2 : 4];
+        uint32_t scale;
+      };
+      // loads are unconditional, past the rows' end from their start: a branch around each would cost registers
       const auto load = [&](Step& v, int n) {
-        const int k0 = n * STEP + 16 * g, k = k0 < p.K ? k0 : 0;
-        const int block = min(n, steps - 1) / (FP8_BLOCK / STEP);  // of the scales: the same for all lanes
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-          if constexpr (CODES) {
-            v.x[i][0] = *(const u4*)((const uint8_t*)p.x + at[i] * p.ldx + k);
-            v.scale[i] = p.x_scales[(size_t)block * m16 + at[i]];
-          } else {
-            const uint16_t* from = (const uint16_t*)p.x + at[i] * p.ldx + k;
-            v.x[i][0] = *(const u4*)from;
-            v.x[i][1] = *(const u4*)(from + 8);
-          }
+        for (int i = 0; i < RT; i++) {
+          const int c = tid + 256 * i, k = n * STEP + 8 * (c & 15);
+          v.a[i] = *(const u4*)(a + (size_t)min(ROWS * RT * group + c / 16, SR - 1) * p.K + (k < p.K ? k : 0));
         }
+#pragma unroll
+        for (int e = 0; e < (CODES ? 2 : 4); e++) {
+          const int k = n * STEP + (CODES ? 16 * (g + 4 * e) : 8 * (g + 4 * e));
+          v.x[e] = *(const u4*)((const char*)p.x + (at * p.ldx + (k < p.K ? k : 0)) * (CODES ? 1 : 2));
+        }
+        if constexpr (CODES) v.scale = p.x_scales[(size_t)min(n, steps - 1) * m16 + at];
+      };
+      f4 acc[RT];
+#pragma unroll
+      for (int q = 0; q < RT; q++) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
+      Step u;
+      load(u, kg);
+#pragma unroll 2
+      for (int i = 0; i * KG < steps; i++) {
+        const int n = i * KG + kg;
+        char* buffer = mine + (i & 1) * BUFFER;
+#pragma unroll
+        for (int k = 0; k < RT; k++) {
+          const int c = tid + 256 * k, j = c / 16;
+          *(u4*)(buffer + j * 256 + ((c ^ j) & 15) * 16) = u.a[k];
+        }
+        Step v;
+        load(v, n + KG);
+        __syncthreads();  // the buffer is whole; it is written again past the next one's barrier
+        u4 x[4];
+#pragma unroll
+        for (int e = 0; e < (CODES ? 2 : 4); e++) {
+          const u4 c = n * STEP + (CODES ? 16 * (g + 4 * e) : 8 * (g + 4 * e)) < p.K ? u.x[e] : zero;
+          if constexpr (CODES) x[2 * e] = widen8<BF>(c[0], c[1]), x[2 * e + 1] = widen8<BF>(c[2], c[3]);
+          else x[e] = c;
+        }
+        const float f = CODES ? e8m0_value(u.scale) : 1.f;
 #pragma unroll
         for (int q = 0; q < RT; q++) {
-          v.w[q][0] = *(const u4*)(arow[q] + k);
-          v.w[q][1] = *(const u4*)(arow[q] + k + 8);
-        }
-        v.ok = k0 < p.K;
-      };
-      const auto multiply = [&](const Step& v) {
+          f4 t = CODES ? f4{0.f, 0.f, 0.f, 0.f} : acc[q];
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-          const u4 zero = u4{0, 0, 0, 0};
-          u4 x0 = v.ok ? v.x[i][0] : zero, x1 = CODES ? zero : (v.ok ? v.x[i][CODES ? 0 : 1] : zero);
-          if constexpr (CODES) x1 = widen8<BF>(x0[2], x0[3]), x0 = widen8<BF>(x0[0], x0[1]);
+          for (int e = 0; e < 4; e++) {
+            const int c = CODES ? 2 * (g + 4 * (e / 2)) + e % 2 : g + 4 * e;  // the chunk with the same K values
+            t = mfma<BF>(*(const u4*)(buffer + (ROWS * q + r) * 256 + ((c ^ r) & 15) * 16), x[e], t);
+          }
+          if constexpr (CODES) {
 #pragma unroll
-          for (int q = 0; q < RT; q++) {
-            f4 t = mfma<BF>(v.w[q][0], x0, CODES ? f4{0.f, 0.f, 0.f, 0.f} : acc[i][q]);
-            t = mfma<BF>(v.w[q][1], x1, t);
-            if constexpr (CODES) {
-              const float f = e8m0_value(v.scale[i]);
-#pragma unroll
-              for (int e = 0; e < 4; e++) acc[i][q][e] = __builtin_fmaf(t[e], f, acc[i][q][e]);
-            } else {
-              acc[i][q] = t;
-            }
+            for (int e = 0; e < 4; e++) acc[q][e] = __builtin_fmaf(t[e], f, acc[q][e]);
+          } else {
+            acc[q] = t;
           }
         }
-      };
-      Step u;
-      load(u, first);
-#pragma unroll 2
-      for (int n = first; n < steps; n += stride) {
-        Step v;
-        load(v, n + stride);
-        multiply(u);
         u = v;
       }
-      if (waves > 1) {
+      __syncthreads();  // the buffers are free
+      if constexpr (KG > 1) {
 #pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-          for (int q = 0; q < RT; q++) red[(wave * NT * RT + i * RT + q) * 64 + lane] = acc[i][q];
+        for (int q = 0; q < RT; q++) ((f4*)lds)[(wave * RT + q) * 64 + lane] = acc[q];
         __syncthreads();
       }
       int gg = g;
-      asm volatile("" : "+v"(gg));
-#pragma unroll
-      for (int i = 0; i < NT; i++) {
-        if (ad.id[i] != ad.current) continue;  // -1 behind the last row
+      asm volatile("" : "+v"(gg));  // the addresses of results are left to be computed here
+      if (id == ad.current) {       // -1 behind the last row
 #pragma unroll
         for (int q = 0; q < RT; q++) {
-          const int t = i * RT + q, j = ROWS * (group * RT + q) + 4 * gg;
-          if (t % waves != wave || j >= SR || j % p.R >= rank) continue;
-          f4 v = acc[i][q];
-          if (waves > 1) {
-            v = red[t * 64 + lane];
-            for (int k = 1; k < waves; k++) v += red[(k * NT * RT + t) * 64 + lane];
+          const int j = ROWS * (group * RT + q) + 4 * gg;
+          if (q % KG != kg || j >= SR) continue;
+          f4 v = acc[q];
+          if constexpr (KG > 1) {
+            v = ((f4*)lds)[(rw * RT + q) * 64 + lane];
+#pragma unroll
+            for (int k = 1; k < KG; k++) v += ((f4*)lds)[((4 * k + rw) * RT + q) * 64 + lane];
           }
+          const int slice = j / p.R, at_rank = j - slice * p.R;
+          float rest[4];  // ranks past the adapter's own may come from anything
 #pragma unroll
-          for (int e = 0; e < 4; e++) v[e] *= scale;
-          const int64_t row = row0 + ROWS * i + r;
-          if constexpr (JOIN) {
-            *(f4*)((float*)p.h + ((size_t)split * p.T + row) * SR + j) = v;
-          } else {
-            float rest[4] = {v[0], v[1], v[2], v[3]};
-            const int slice = j / p.R;
-            uint16_t* to = (uint16_t*)p.h + ((size_t)row * p.S + slice) * parts * p.R + (j - slice * p.R);
-            for (int k = 0; k < parts; k++) {
-              uint32_t w[4];
+          for (int e = 0; e < 4; e++) rest[e] = at_rank < rank ? v[e] * scale : 0.f;
+          uint16_t* to = (uint16_t*)p.h + ((size_t)row * p.S + slice) * parts * p.R + at_rank;
+          for (int k = 0; k < parts; k++) {
+            uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; e++) w[e] = next_part(rest[e], k == 1 && parts == 2);
-              typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-              *(u2*)(to + k * p.R) = u2{w[0] | w[1] << 16, w[2] | w[3] << 16};
-            }
+            for (int e = 0; e < 4; e++) w[e] = next_part(rest[e], k == 1 && parts == 2);
+            *(u2*)(to + k * p.R) = u2{w[0] | w[1] << 16, w[2] | w[3] << 16};
           }
         }
       }
-      if (waves > 1) __syncthreads();
+      if constexpr (KG > 1) __syncthreads();  // the sums are read
     }
   }
 }
@@ -309,6 +372,11 @@ __device__ __forceinline__ void split8(const u4& w, u4& hi, u4& lo) {
   }
 }
 
+// Waves a SIMD that the second product's registers leave room for.
+constexpr int up_occupancy(int YT, bool BF, int STEPS, bool JOIN) {
+  return JOIN || (STEPS == 1 && (BF || YT != FP8_IO_F32)) || (STEPS == 2 && BF && YT != FP8_IO_F32) ? 3 : 2;
+}
+
 // Eight ranks of a row's part, from parts of K that the first product left in f32.
 template <int PARTS>
 __device__ __forceinline__ void join8(const float* from, int splits, size_t stride, u4 (&part)[PARTS]) {
@@ -328,10 +396,14 @@ __device__ __forceinline__ void join8(const float* from, int splits, size_t stri
     }
 }
 
-template <int YT, bool BF, int NT, bool JOIN>
-__global__ __launch_bounds__(64 * UP_WAVES, (NT == 1) == (YT == FP8_IO_F32) ? 3 : (NT == 1 ? 4 : 2)) void adapter_up_kernel(AdapterArgs p, int splits) {
+// A wave walks sixteens of rows, the next two on their way while one is taken, and keeps the weights of the adapter that
+// it met last: STEPS times 32 ranks of its columns, f16 ones as their two parts where registers hold them.  JOIN: few
+// rows, one sixteen and one of its adapters.
+template <int YT, bool BF, int STEPS, bool JOIN>
+__global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, STEPS, JOIN)) void adapter_up_kernel(AdapterArgs p, int splits, int run) {
   constexpr int PARTS = YT == FP8_IO_F32 ? 3 : 2, SIZE = YT == FP8_IO_F32 ? 4 : 2, PAIRS = YT == FP8_IO_F32 ? 2 : 1;
   constexpr int PIECE = 64 / SIZE, COUNT = 16 / SIZE;  // values of a piece, and of a lane in it
+  constexpr bool EARLY = STEPS == 1 && !JOIN;          // h of a sixteen comes with its y
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   // this wave's columns
   int s = 0, n0 = 0, c = (int)blockIdx.x;
@@ -343,112 +415,159 @@ __global__ __launch_bounds__(64 * UP_WAVES, (NT == 1) == (YT == FP8_IO_F32) ? 3 
   const int end = n0 + p.cols[s];
   n0 += (c * UP_WAVES + wave) * COLS;
   if (n0 >= end) return;
-  const int64_t tiles = ((int64_t)p.T + ROWS * NT - 1) / (ROWS * NT);
+  const int64_t tiles = ((int64_t)p.T + ROWS - 1) / ROWS;
   const bool in_place = p.y == p.out, upper = r >= 8;
   const int nm = n0 + (upper ? PIECE : 0) + COUNT * g;  // the first column that the lane loads and stores, pairs 32 apart
-  for (int64_t tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
-    const int64_t row0 = tile * ROWS * NT;
-    Adapters<NT> ad(p, row0);
-    u4 y[NT][PAIRS][2];
+  const u4 zero = u4{0, 0, 0, 0};
+  struct Tile {
+    u4 y[PAIRS][2], v[EARLY ? PARTS : 1];
+    int id;
+  };
+  // loads are unconditional, behind the last row from it
+  const auto load = [&](Tile& x, int64_t tile) {
+    const int64_t row0 = tile * ROWS, last = p.T - 1;
 #pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-      for (int m = 0; m < PAIRS; m++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-          const int64_t row = row0 + ROWS * i + (r & 7) + 8 * k;
-          const int n = nm + 32 * m < end ? nm + 32 * m : n0;
-          y[i][m][k] = *(const u4*)((const char*)p.y + (min(row, (int64_t)p.T - 1) * p.ldy + n) * SIZE);
-        }
-    // stores the rows of adapter `which`, -1: those of none
-    const auto store = [&](int i, int which) {
-      int column = nm;  // opaque, so that no address is held from before
-      asm volatile("" : "+v"(column));
-      const int other = __builtin_amdgcn_update_dpp(0, ad.id[i], 0x128, 0xf, 0xf, false);
+    for (int m = 0; m < PAIRS; m++)
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const int64_t row = row0 + ROWS * i + (r & 7) + 8 * k;
-        if (((k == 1) == upper ? ad.id[i] : other) != which || row >= p.T) continue;
+        const int n = nm + 32 * m < end ? nm + 32 * m : n0;
+        x.y[m][k] = *(const u4*)((const char*)p.y + (min(row0 + (r & 7) + 8 * k, last) * p.ldy + n) * SIZE);
+      }
+    const int64_t row = min(row0 + r, last);
+    x.id = p.ids[row];
+    if constexpr (EARLY) {
+      const uint16_t* from = (const uint16_t*)p.h + (row * p.S + s) * PARTS * p.R + (8 * g < p.R ? 8 * g : 0);
+#pragma unroll
+      for (int k = 0; k < PARTS; k++) x.v[k] = *(const u4*)(from + k * p.R);
+    }
+  };
+  constexpr bool APART = !BF && STEPS < 4 && !JOIN;  // f16 weights are kept as their parts
+  int held = -1, rank = 0;
+  u4 w[JOIN ? 1 : STEPS][4], lo[APART ? STEPS : 1][4];
+  const auto weights = [&](u4 (&v)[4], int t) {  // of ranks 32 t + 8 g .. + 7
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int n = min(n0 + column<YT>(j, r / 4, r % 4), end - 1), at = 32 * t + 8 * g;
+      v[j] = *(const u4*)((const uint16_t*)p.b + ((size_t)held * p.N + n) * p.R + (at < p.R ? at : 0));
+    }
+  };
+  const auto take = [&](const Tile& x, int64_t tile) {
+    const int64_t row0 = tile * ROWS;
+    Adapters<1> ad(p, row0, x.id);
+    const int id = ad.id[0], other = __builtin_amdgcn_update_dpp(0, id, 0x128, 0xf, 0xf, false);
+    // stores the rows of adapter `which`, -1: those of none
+    const auto store = [&](const u4 (&y)[PAIRS][2], int which) {
+      int column = nm;
+      asm volatile("" : "+v"(column));  // no address is held from before
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int64_t row = row0 + (r & 7) + 8 * k;
+        if (((k == 1) == upper ? id : other) != which || row >= p.T) continue;
 #pragma unroll
         for (int m = 0; m < PAIRS; m++)
-          if (column + 32 * m < end) *(u4*)((char*)p.out + (row * p.ldo + column + 32 * m) * SIZE) = y[i][m][k];
+          if (column + 32 * m < end) *(u4*)((char*)p.out + (row * p.ldo + column + 32 * m) * SIZE) = y[m][k];
       }
     };
-    if (!in_place && (!JOIN || blockIdx.z == 0)) {
-#pragma unroll
-      for (int i = 0; i < NT; i++) store(i, -1);
-    }
+    if (!in_place && (!JOIN || blockIdx.z == 0)) store(x.y, -1);
     if (JOIN) ad.only((int)blockIdx.z);
     while (ad.next()) {
-      const int rank = rank_of(p, ad.current);
-      const uint16_t* brow[4];
+      if (ad.current != held) {
+        held = ad.current;
+        rank = rank_of(p, held);
+        if constexpr (!JOIN) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int n = min(n0 + column<YT>(j, r / 4, r % 4), end - 1);
-        brow[j] = (const uint16_t*)p.b + ((size_t)ad.current * p.N + n) * p.R;
-      }
-      f4 acc[NT][4];
+          for (int t = 0; t < STEPS; t++) weights(w[t], t);
 #pragma unroll
-      for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int r0 = 0; r0 < p.R; r0 += 32) {
-        // this lane's eight ranks, loaded where they are the matrix's and counted where they are the adapter's: the
-        // loads do not wait for its rank
-        const int at = r0 + 8 * g < p.R ? r0 + 8 * g : 0;
-        const u4 zero = u4{0, 0, 0, 0};
-        u4 w[4], lo[4], v[NT][PARTS];
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = *(const u4*)(brow[j] + at);
-#pragma unroll
-        for (int i = 0; i < NT; i++) {
-          const size_t row = ad.source(i);
-          if constexpr (JOIN) {
-            join8<PARTS>((const float*)p.h + row * p.S * p.R + s * p.R + at, splits, (size_t)p.T * p.S * p.R, v[i]);
-          } else {
-            const uint16_t* from = (const uint16_t*)p.h + (row * p.S + s) * PARTS * p.R + at;
-#pragma unroll
-            for (int k = 0; k < PARTS; k++) v[i][k] = *(const u4*)(from + k * p.R);
-          }
-        }
-        if (r0 >= rank) break;
-        const bool ok = r0 + 8 * g < rank;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          w[j] = ok ? w[j] : zero;
-          if constexpr (!BF) {
-            const u4 x = w[j];
-            split8(x, w[j], lo[j]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-          for (int k = 0; k < PARTS; k++) {
-            const u4 x = ok ? v[i][k] : zero;
+          for (int t = 0; t < STEPS; t++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              acc[i][j] = mfma<true>(w[j], x, acc[i][j]);
-              if constexpr (!BF) acc[i][j] = mfma<true>(lo[j], x, acc[i][j]);
+              w[t][j] = 32 * t + 8 * g < rank ? w[t][j] : zero;
+              if constexpr (APART) {
+                const u4 f = w[t][j];
+                split8(f, w[t][j], lo[t][j]);
+              }
             }
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < NT; i++) {
-        const int other = __builtin_amdgcn_update_dpp(0, ad.id[i], 0x128, 0xf, 0xf, false);
-#pragma unroll
-        for (int m = 0; m < PAIRS; m++) {
-          u4 a = y[i][m][0], b = y[i][m][1];
-          swap_eights(a, b);
-          add_to<YT>(a, &acc[i][YT == FP8_IO_F32 ? 2 * m : 0]);
-          add_to<YT>(b, &acc[i][YT == FP8_IO_F32 ? 2 * m + 1 : 2]);
-          swap_eights(a, b);
-          // another adapter's rows keep theirs
-          if ((upper ? other : ad.id[i]) == ad.current) y[i][m][0] = a;
-          if ((upper ? ad.id[i] : other) == ad.current) y[i][m][1] = b;
         }
-        store(i, ad.current);
+      }
+      f4 acc[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+      const int64_t row = ad.source(0);
+      const auto multiply = [&](const u4 (&hi)[4], const u4 (&low)[4], u4 (&v)[PARTS], int t) {
+#pragma unroll
+        for (int k = 0; k < PARTS; k++) {
+          v[k] = 32 * t + 8 * g < rank ? v[k] : zero;  // an infinity times the weights' zeros would be NaN
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            acc[j] = mfma<true>(hi[j], v[k], acc[j]);
+            if constexpr (!BF) acc[j] = mfma<true>(low[j], v[k], acc[j]);
+          }
+        }
+      };
+      const auto apart = [&](const u4 (&f)[4], u4 (&hi)[4], u4 (&low)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if constexpr (BF) hi[j] = f[j];
+          else split8(f[j], hi[j], low[j]);
+        }
+      };
+      if constexpr (JOIN) {
+#pragma unroll 1
+        for (int t = 0; 32 * t < p.R; t++) {
+          const int at = 32 * t + 8 * g;
+          weights(w[0], t);
+          u4 v[PARTS], hi[4], low[4];
+          join8<PARTS>((const float*)p.h + (size_t)row * p.S * p.R + s * p.R + (at < p.R ? at : 0), splits, (size_t)p.T * p.S * p.R, v);
+#pragma unroll
+          for (int j = 0; j < 4; j++) w[0][j] = at < rank ? w[0][j] : zero;
+          apart(w[0], hi, low);
+          multiply(hi, low, v, t);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < STEPS; t++) {
+          const int at = 32 * t + 8 * g;
+          u4 v[PARTS];
+          const uint16_t* from = (const uint16_t*)p.h + (row * p.S + s) * PARTS * p.R + (at < p.R ? at : 0);
+#pragma unroll
+          for (int k = 0; k < PARTS; k++) v[k] = EARLY ? x.v[EARLY ? k : 0] : *(const u4*)(from + k * p.R);
+          if constexpr (BF || APART) {
+            multiply(w[t], lo[APART ? t : 0], v, t);
+          } else {
+            u4 hi[4], low[4];
+            apart(w[t], hi, low);
+            multiply(hi, low, v, t);
+          }
+        }
+      }
+      u4 y[PAIRS][2];
+#pragma unroll
+      for (int m = 0; m < PAIRS; m++) {
+        y[m][0] = x.y[m][0], y[m][1] = x.y[m][1];
+        swap_eights(y[m][0], y[m][1]);
+        add_to<YT>(y[m][0], &acc[YT == FP8_IO_F32 ? 2 * m : 0]);
+        add_to<YT>(y[m][1], &acc[YT == FP8_IO_F32 ? 2 * m + 1 : 2]);
+        swap_eights(y[m][0], y[m][1]);
+      }
+      store(y, ad.current);
+    }
+  };
+  for (int64_t first = (int64_t)blockIdx.y * run; first < tiles; first += (int64_t)gridDim.y * run) {
+    const int64_t stop = min(first + run, tiles);
+    if constexpr (JOIN) {
+      Tile x;
+      load(x, first);
+      take(x, first);
+    } else {
+      Tile x, x1;
+      load(x, first);
+      load(x1, min(first + 1, stop - 1));
+#pragma unroll 1
+      for (int64_t tile = first; tile < stop; tile++) {
+        Tile x2;
+        load(x2, min(tile + 2, stop - 1));
+        take(x, tile);
+        x = x1, x1 = x2;
       }
     }
   }
@@ -456,71 +575,89 @@ __global__ __launch_bounds__(64 * UP_WAVES, (NT == 1) == (YT == FP8_IO_F32) ? 3 
 
 // How a call is cut up.
 struct Plan {
-  bool join;       // few rows: one of a sixteen's adapters to a workgroup, K split over workgroups
-  int splits;      // parts of K of different workgroups
-  int waves;       // of a workgroup, on parts of K
-  int down, up;    // sixteens of rows of a workgroup
-  int ranks;       // sixteens of ranks of a workgroup
+  bool few;     // rows: one of a sixteen's adapters to a workgroup, K split over workgroups
+  int splits;   // their parts of K
+  int waves;    // of a workgroup, on parts of K: few rows; times four otherwise
+  int ranks;    // sixteens of ranks of a workgroup
 };
-Plan plan_of(int T, int K, int SR, int up_blocks) {
+Plan plan_of(int T, int K, int SR) {
   Plan q{};
-  const int steps = (K + STEP - 1) / STEP, tiles = (SR + ROWS - 1) / ROWS;
-  const int64_t sixteens = ((int64_t)T + ROWS - 1) / ROWS;
-  q.join = T <= 256;
-  if (q.join) {
-    q.waves = std::min(8, steps);
+  const int tiles = (SR + ROWS - 1) / ROWS;
+  q.few = T <= 256;
+  q.splits = 1;
+  if (q.few) {
+    const int steps = (K + FEW_STEP - 1) / FEW_STEP;
+    q.waves = std::min(FEW_WAVES, steps);
     q.splits = std::min((steps + q.waves - 1) / q.waves, 8);
-    q.down = q.up = q.ranks = 1;
+    q.ranks = 1;
     return q;
   }
-  q.splits = 1;
-  q.ranks = std::min(tiles, 4);
-  const int groups = (tiles + q.ranks - 1) / q.ranks;
-  q.down = sixteens >= 4 * 1024 ? 4 : 2;
-  q.waves = 1;
-  while (q.waves < DOWN_WAVES && 2 * q.waves <= steps && sixteens / q.down * groups * q.waves < 4096) q.waves *= 2;
-  q.up = sixteens * up_blocks >= 2 * 1024 ? 2 : 1;
+  const int steps = (K + STEP - 1) / STEP;
+  q.ranks = tiles <= 4 ? tiles : (tiles % 3 == 0 ? 3 : 4);
+  const int64_t blocks = ((int64_t)T + 4 * ROWS - 1) / (4 * ROWS) * ((tiles + q.ranks - 1) / q.ranks);
+  q.waves = blocks >= 768 || steps < 2 ? 1 : (blocks >= 192 || steps < 4 ? 2 : 4);
   return q;
 }
 
-template <bool CODES, bool BF, int NT, int RT, bool JOIN>
-hipError_t launch_down(const AdapterArgs& a, const Plan& q, hipStream_t s) {
+template <bool CODES, bool BF, int RT, int KG>
+hipError_t launch_down(const AdapterArgs& a, hipStream_t s) {
   const int tiles = (a.S * a.R + ROWS - 1) / ROWS, groups = (tiles + RT - 1) / RT;
-  const int64_t rows = ((int64_t)a.T + ROWS * NT - 1) / (ROWS * NT);
-  const dim3 grid((unsigned)std::min<int64_t>(rows, 1 << 20), (unsigned)(groups * q.splits), JOIN ? std::min(ROWS, a.T) : 1);
-  const size_t lds = q.waves > 1 ? (size_t)q.waves * NT * RT * 64 * sizeof(f4) : 0;
-  T5K_LAUNCH((adapter_down_kernel<CODES, BF, NT, RT, JOIN>), grid, dim3(64 * q.waves), lds, s, a, q.splits, a.y_type == FP8_IO_F32 ? 3 : 2);
+  const int64_t rows = ((int64_t)a.T + 4 * ROWS - 1) / (4 * ROWS);
+  // a tile with the rows of several short requests would take as many turns: workgroups share them while there is room
+  const dim3 grid((unsigned)std::min<int64_t>(rows, 1 << 20), (unsigned)groups, rows * groups < 768 ? 4 : 1);
+  const size_t lds = (size_t)KG * 2 * RT * ROWS * STEP * 2;
+  T5K_LAUNCH((adapter_down_kernel<CODES, BF, RT, KG>), grid, dim3(256 * KG), lds, s, a, a.y_type == FP8_IO_F32 ? 3 : 2);
   return hipGetLastError();
 }
-template <bool CODES, bool BF, int NT>
+template <bool CODES, bool BF, int KG>
 hipError_t launch_down_ranks(const AdapterArgs& a, const Plan& q, hipStream_t s) {
   switch (q.ranks) {
-    case 1: return launch_down<CODES, BF, NT, 1, false>(a, q, s);
-    case 2: return launch_down<CODES, BF, NT, 2, false>(a, q, s);
-    case 3: return launch_down<CODES, BF, NT, 3, false>(a, q, s);
+    case 1: return launch_down<CODES, BF, 1, KG>(a, s);
+    case 2: return launch_down<CODES, BF, 2, KG>(a, s);
+    case 3: return launch_down<CODES, BF, 3, KG>(a, s);
   }
-  return launch_down<CODES, BF, NT, 4, false>(a, q, s);
+  return launch_down<CODES, BF, 4, KG>(a, s);
 }
 template <bool CODES, bool BF>
 hipError_t launch_down_plan(const AdapterArgs& a, const Plan& q, hipStream_t s) {
-  if (q.join) return launch_down<CODES, BF, 1, 1, true>(a, q, s);
-  return q.down == 4 ? launch_down_ranks<CODES, BF, 4>(a, q, s) : launch_down_ranks<CODES, BF, 2>(a, q, s);
+  if (q.few) {
+    const int groups = (a.S * a.R + ROWS - 1) / ROWS;
+    const dim3 grid((unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)(groups * q.splits), (unsigned)std::min(ROWS, a.T));
+    T5K_LAUNCH((adapter_down_few_kernel<CODES, BF>), grid, dim3(64 * q.waves), 0, s, a, q.splits);
+    return hipGetLastError();
+  }
+  switch (q.waves) {
+    case 1: return launch_down_ranks<CODES, BF, 1>(a, q, s);
+    case 2: return launch_down_ranks<CODES, BF, 2>(a, q, s);
+  }
+  return launch_down_ranks<CODES, BF, 4>(a, q, s);
 }
 
+template <int YT, bool BF, int STEPS>
+hipError_t launch_up_steps(const AdapterArgs& a, int blocks, hipStream_t s) {
+  const int64_t sixteens = ((int64_t)a.T + ROWS - 1) / ROWS;
+  // sixteens of rows of a workgroup, so that there are workgroups for every place twice
+  const int run = (int)std::max<int64_t>(1, std::min<int64_t>(32, sixteens * blocks / 2048));
+  const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>((sixteens + run - 1) / run, 65535));
+  T5K_LAUNCH((adapter_up_kernel<YT, BF, STEPS, false>), grid, dim3(64 * UP_WAVES), 0, s, a, 1, run);
+  return hipGetLastError();
+}
 template <int YT, bool BF>
 hipError_t launch_up(const AdapterArgs& a, const Plan& q, int blocks, hipStream_t s) {
-  const int64_t sixteens = ((int64_t)a.T + ROWS - 1) / ROWS;
-  const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>((sixteens + q.up - 1) / q.up, 65535), q.join ? std::min(ROWS, a.T) : 1);
-  if (q.join) T5K_LAUNCH((adapter_up_kernel<YT, BF, 1, true>), grid, dim3(64 * UP_WAVES), 0, s, a, q.splits);
-  else if (q.up == 2) T5K_LAUNCH((adapter_up_kernel<YT, BF, 2, false>), grid, dim3(64 * UP_WAVES), 0, s, a, 1);
-  else T5K_LAUNCH((adapter_up_kernel<YT, BF, 1, false>), grid, dim3(64 * UP_WAVES), 0, s, a, 1);
-  return hipGetLastError();
+  if (q.few) {
+    const dim3 grid((unsigned)blocks, (unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)std::min(ROWS, a.T));
+    T5K_LAUNCH((adapter_up_kernel<YT, BF, 1, true>), grid, dim3(64 * UP_WAVES), 0, s, a, q.splits, 1);
+    return hipGetLastError();
+  }
+  if (a.R <= 32) return launch_up_steps<YT, BF, 1>(a, blocks, s);
+  if (a.R <= 64) return launch_up_steps<YT, BF, 2>(a, blocks, s);
+  return launch_up_steps<YT, BF, 4>(a, blocks, s);
 }
 template <bool BF>
 hipError_t launch(const AdapterArgs& a, hipStream_t s) {
   int blocks = 0;
   for (int i = 0; i < a.S; i++) blocks += (a.cols[i] + UP_WAVES * COLS - 1) / (UP_WAVES * COLS);
-  const Plan q = plan_of(a.T, a.K, a.S * a.R, blocks);
+  const Plan q = plan_of(a.T, a.K, a.S * a.R);
   const hipError_t e = a.x_type == ADAPTER_E4M3 ? launch_down_plan<true, BF>(a, q, s) : launch_down_plan<false, BF>(a, q, s);
   if (e != hipSuccess) return e;
   switch (a.y_type) {
@@ -534,8 +671,8 @@ hipError_t launch(const AdapterArgs& a, hipStream_t s) {
 
 namespace t5k {
 size_t adapter_work_bytes(int T, int K, int SR) {
-  const Plan q = plan_of(T, K, SR, 1);
-  return (size_t)T * SR * (q.join ? 4 * (size_t)q.splits : 6);
+  const Plan q = plan_of(T, K, SR);
+  return (size_t)T * SR * (q.few ? 4 * (size_t)q.splits : 6);
 }
 
 hipError_t launch_adapter(const AdapterArgs& a, hipStream_t s) {
