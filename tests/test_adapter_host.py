@@ -44,8 +44,8 @@ def _call(x=P, xt=1, xs=None, ldx=128, T=5, K=128, ids=P, G=3, a=P, b=P, wt=1, r
     (dict(y=P + FAR + 4), "y is not aligned"), (dict(out=P + 2), "out is not aligned"), (dict(a=P + 8), "a is not aligned"),
     (dict(b=P + 8), "b is not aligned"), (dict(ids=P + 2), "ids is not aligned"), (dict(ranks=P + 1), "ranks is not aligned"),
     (dict(scales=P + 2), "scales is not aligned"), (dict(work=P + 4), "workspace is not aligned"), (dict(ldx=120), "x's rows"),
-    (dict(ldx=132), "x's rows"), (dict(ldx=-128), "x's rows"), (dict(ldx=(1 << 30) + 8), "x's rows"), (dict(ldy=48), "y's rows"),
-    (dict(ldo=68), "out's rows"), (dict(ldo=0), "out's rows"), (dict(bytes_=5 * 16 * 4 - 1), "workspace is smaller"), (dict(bytes_=0), "workspace"),
+    (dict(ldx=132), "x's rows"), (dict(ldx=-128), "x's rows"), (dict(ldx=(1 << 24) + 8), "x's rows"), (dict(ldy=48), "y's rows"),
+    (dict(ldo=68), "out's rows"), (dict(ldo=0), "out's rows"), (dict(ldo=(1 << 24) + 8), "out's rows"), (dict(bytes_=5 * 16 * 4 - 1), "workspace is smaller"), (dict(bytes_=0), "workspace"),
     (dict(out=P + FAR + 16), "overlaps"), (dict(out=P + FAR, ldo=128), "overlaps"), (dict(out=P + FAR, ldy=128, ldo=64), "overlaps"),
     # columns of the same rows, which run into the next row's
     (dict(ldy=128, out=P + FAR + 192, ldo=128), "overlaps"), (dict(ldy=128, out=P + FAR + 64, ldo=128), "overlaps"),
@@ -66,7 +66,7 @@ def test_workspace():
         for k in (16, 128, 768, 4096):
             for slices, r in ((1, 8), (3, 16), (4, 128)):
                 n = adapters.workspace_bytes(t, k, slices, r)
-                assert n >= t * slices * r * 4 and n % (t * slices * r) == 0
+                assert n >= t * slices * r * 4
     big = adapters.workspace_bytes(1 << 30, 1 << 21, 4, 128)
     assert big == (1 << 30) * 512 * 6
     _refused(lib.t5h_adapter_workspace, 1, 128, 1, 16, None, says="NULL")

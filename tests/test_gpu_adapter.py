@@ -288,18 +288,22 @@ def test_infinities_and_nan_stay_in_their_row(adapters, w):
             assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0, 1, -1), want.nan_to_num(0, 1, -1))
 
 
-def test_rows_past_32_bits(adapters):
-    """Rows whose values lie past 2^32, of x, y and out."""
-    T, K, n, ld = 6, 64, 32, 1 << 30
-    c = Case(T, K, (n,), 8, 2, ids=[0, 1, -1, 1, 0, 1])
+@pytest.mark.parametrize("y", ["f16", "f32"])
+@pytest.mark.parametrize("T", [150, 400])
+def test_rows_past_32_bits(adapters, T, y):
+    """Rows as far apart as may be, whose bytes (and with 400 of them values) lie past 2^32, of x, y and out."""
+    K, n, ld = 64, 32, 1 << 24
+    if y == "f32" and T > 200:
+        ld = 1 << 23
+    c = Case(T, K, (n,), 8, 2, y=y, ids=[0, 1, -1, 1, 0] * (T // 5))
     x = torch.empty((T - 1) * ld + K, dtype=torch.float16, device=DEV)
-    y = torch.empty((T - 1) * ld + n, dtype=torch.float16, device=DEV)
+    big = torch.empty((T - 1) * ld + n, dtype=c.y.dtype, device=DEV)
     for t in range(T):
-        x[t * ld:t * ld + K], y[t * ld:t * ld + n] = c.x[t, :K], c.y[t, :n]
+        x[t * ld:t * ld + K], big[t * ld:t * ld + n] = c.x[t, :K], c.y[t, :n]
     work = torch.empty(adapters.workspace_bytes(T, K, 1, 8), dtype=torch.uint8, device=DEV)
     adapters.add_device(x.data_ptr(), 1, 0, ld, T, K, c.ids.data_ptr(), 2, c.a.data_ptr(), c.b.data_ptr(), 1, 0, c.scales.data_ptr(), 8, (n,),
-                        y.data_ptr(), ld, y.data_ptr(), ld, 1, work.data_ptr(), work.numel(), _stream())
-    c.check(torch.stack([y[t * ld:t * ld + n] for t in range(T)]))
+                        big.data_ptr(), ld, big.data_ptr(), ld, CODE[y], work.data_ptr(), work.numel(), _stream())
+    c.check(torch.stack([big[t * ld:t * ld + n] for t in range(T)]))
 
 
 def test_adapters_past_32_bits(adapters):

@@ -16,7 +16,7 @@ using t5h_detail::type_bytes;
 static_assert(T5H_TYPE_E4M3 == t5k::ADAPTER_E4M3, "the kernels take the ABI's type codes");
 
 constexpr int32_t kMostRows = 1 << 30, kMostAdapters = 1 << 24, kMostCols = 1 << 24;
-constexpr int64_t kMostStride = (int64_t)1 << 30;
+constexpr int64_t kMostStride = (int64_t)1 << 24;  // the kernels' offsets between a tile's rows have 32 bits
 
 int bad(const std::string& what) { return fail(T5H_ERR_INVALID, "adapter: " + what); }
 
@@ -49,7 +49,7 @@ int check_buffer(const void* p, const char* name, size_t align) {
 }
 int check_rows(const Rows& r, int64_t ld, int64_t least) {
   TRY(check_buffer((const void*)r.at, r.name, 16));
-  if (ld < least || ld > kMostStride) return bad(std::string(r.name) + "'s rows must be as long as its values, up to 2^30 apart");
+  if (ld < least || ld > kMostStride) return bad(std::string(r.name) + "'s rows must be as long as its values, up to 2^24 apart");
   if (r.stride % 16) return bad(std::string(r.name) + "'s rows must start on 16 bytes");
   return T5H_OK;
 }

@@ -25,7 +25,7 @@ struct AdapterArgs {
   void* out;
   int64_t ldy, ldo;  // values
   int y_type;
-  void* h;  // bf16 [T][S][2 or 3 parts][R], or for few rows f32 [splits][T][S R]
+  void* h;  // bf16 parts in operand order, or for few rows f32 [splits][T][S R]: the kernels' own
 };
 size_t adapter_work_bytes(int T, int K, int SR);
 hipError_t launch_adapter(const AdapterArgs& a, hipStream_t s);

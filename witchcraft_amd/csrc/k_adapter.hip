@@ -77,11 +77,6 @@ struct Adapters {
       pending[i] = id[i] >= 0;
     }
   }
-  // from the lane's id of row l % 16
-  __device__ __forceinline__ Adapters(const AdapterArgs& p, int64_t first, int v) : row0(first) {
-    id[0] = row0 + (threadIdx.x & 15) < p.T && (unsigned)v < (unsigned)p.G ? v : -1;
-    pending[0] = id[0] >= 0;
-  }
   __device__ __forceinline__ void only(int row) {
     const int first = __builtin_amdgcn_readlane(id[0], row);
     const uint64_t m = __ballot(id[0] == first);
@@ -109,10 +104,10 @@ struct Adapters {
   }
 };
 
-// The adapter's rank, rounded up to whole eights: what its weights are read up to.
-__device__ __forceinline__ int rank_of(const AdapterArgs& p, int g) {
-  if (!p.ranks) return p.R;
-  const int r = __builtin_amdgcn_readfirstlane(p.ranks[g]);
+// The adapter's rank as it is given, and (the same in all lanes) rounded up to whole eights: what of its weights counts.
+__device__ __forceinline__ int given_rank(const AdapterArgs& p, int g) { return p.ranks ? p.ranks[g] : p.R; }
+__device__ __forceinline__ int whole_rank(const AdapterArgs& p, int given) {
+  const int r = __builtin_amdgcn_readfirstlane(given);
   return r <= 0 ? 0 : (r >= p.R ? p.R : (r + 7) & ~7);
 }
 
@@ -123,6 +118,12 @@ __device__ __forceinline__ uint32_t next_part(float& v, bool last_of_two) {
   const uint32_t part = last_of_two ? (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v) : u >> 16;
   v = (u & 0x7f800000u) != 0x7f800000u ? v - __uint_as_float(u & 0xffff0000u) : 0.f;
   return part;
+}
+
+// Where the parts of h lie, in the second product's operand order: for each sixteen of rows, slice, part and eight of
+// ranks 16 rows of 16 bytes, so that its lanes read consecutive ones.  Behind the last row up to a sixteen.
+__device__ __forceinline__ size_t h_index(int64_t row, int slice, int part, int rank, int S, int parts, int R) {
+  return ((((size_t)(row / ROWS) * S + slice) * parts + part) * (R / 8) + rank / 8) * (ROWS * 8) + (row % ROWS) * 8 + rank % 8;
 }
 
 // ---- h = scale x A^T, few rows: 16 rows x 16 ranks per workgroup, its waves on 64 K values in turn ----
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(Adapte
   ad.only((int)blockIdx.z);
   if (!ad.next()) return;
   const float scale = p.scales ? p.scales[ad.current] : 1.f;
-  const int j0 = ROWS * group, rank = rank_of(p, ad.current);
+  const int j0 = ROWS * group, given = given_rank(p, ad.current);
   const int64_t at = ad.source(0);
   const uint16_t* arow = (const uint16_t*)p.a + ((size_t)ad.current * SR + min(j0 + r, SR - 1)) * p.K;
   // loads are unconditional, past the rows' end from their start
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(Adapte
   const int j = j0 + 4 * g;
   if (wave != 0 || ad.id[0] != ad.current || j >= SR) return;
   for (int k = 1; k < waves; k++) acc += red[k][lane];
-  // ranks past the adapter's own may come from anything
+  const int rank = whole_rank(p, given);  // values past it may come from anything
 #pragma unroll
   for (int e = 0; e < 4; e++) acc[e] = j % p.R < rank ? acc[e] * scale : 0.f;
   *(f4*)((float*)p.h + ((size_t)split * p.T + row0 + r) * SR + j) = acc;
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(Adapte
 // where the lanes of a load lie in sixteen rows: that costs the address unit a quarter of its rate, which x alone can
 // bear.  The next step's loads are on their way while one is multiplied.  The KG sums meet in LDS and are added in order.
 template <bool CODES, bool BF, int RT, int KG>
-__global__ __launch_bounds__(256 * KG, KG == 1 ? 3 : 4) void adapter_down_kernel(AdapterArgs p, int parts) {
+__global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : 3) void adapter_down_kernel(AdapterArgs p, int parts) {
   constexpr int BUFFER = RT * ROWS * STEP * 2;  // bytes of A's ranks of a step
   extern __shared__ char lds[];                 // [KG][2][BUFFER]; the sums: [KG][4][RT][64] f4, no more
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
@@ -221,7 +222,6 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 3 : 4) void adapter_down_kernel
     for (unsigned seen = 0; ad.next(); seen++) {
       if (seen % gridDim.z != blockIdx.z) continue;
       const float scale = p.scales ? p.scales[ad.current] : 1.f;
-      const int rank = rank_of(p, ad.current);
       const int id = rw == 0 ? ad.id[0] : (rw == 1 ? ad.id[1] : (rw == 2 ? ad.id[2] : ad.id[3]));
       const int64_t row = row0 + ROWS * rw + r;
       const int64_t at = id == ad.current ? row : ad.row;  // of rows whose result nothing keeps, one that is read anyway
@@ -249,6 +249,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 3 : 4) void adapter_down_kernel
       for (int q = 0; q < RT; q++) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
       Step u;
       load(u, kg);
+      const int given = given_rank(p, ad.current);
 #pragma unroll 2
       for (int i = 0; i * KG < steps; i++) {
         const int n = i * KG + kg;
@@ -292,6 +293,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 3 : 4) void adapter_down_kernel
         for (int q = 0; q < RT; q++) ((f4*)lds)[(wave * RT + q) * 64 + lane] = acc[q];
         __syncthreads();
       }
+      const int rank = whole_rank(p, given);
       int gg = g;
       asm volatile("" : "+v"(gg));  // the addresses of results are left to be computed here
       if (id == ad.current) {       // -1 behind the last row
@@ -306,15 +308,15 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 3 : 4) void adapter_down_kernel
             for (int k = 1; k < KG; k++) v += ((f4*)lds)[((4 * k + rw) * RT + q) * 64 + lane];
           }
           const int slice = j / p.R, at_rank = j - slice * p.R;
-          float rest[4];  // ranks past the adapter's own may come from anything
+          float rest[4];  // values past the adapter's rank may come from anything
 #pragma unroll
           for (int e = 0; e < 4; e++) rest[e] = at_rank < rank ? v[e] * scale : 0.f;
-          uint16_t* to = (uint16_t*)p.h + ((size_t)row * p.S + slice) * parts * p.R + at_rank;
+          uint16_t* to = (uint16_t*)p.h + h_index(row, slice, 0, at_rank, p.S, parts, p.R);
           for (int k = 0; k < parts; k++) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) w[e] = next_part(rest[e], k == 1 && parts == 2);
-            *(u2*)(to + k * p.R) = u2{w[0] | w[1] << 16, w[2] | w[3] << 16};
+            *(u2*)(to + k * p.R * ROWS) = u2{w[0] | w[1] << 16, w[2] | w[3] << 16};
           }
         }
       }
@@ -323,42 +325,33 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 3 : 4) void adapter_down_kernel
   }
 }
 
-// ---- out = y + h B^T: 16 NT rows x 256 columns of one slice per workgroup, 64 columns a wave -------
-// A wave's columns of a row are two pieces of 64 bytes in 16-bit types and four in f32.  Matrix tile j has columns such
-// that a lane's results are 16 bytes of each piece; the lanes of rows 0 .. 7 and 8 .. 15 of a sixteen then swap pieces,
-// so that eight lanes load and store whole lines.
+// ---- out = y + h B^T: 16 rows x 256 columns of one slice per workgroup and turn, 64 columns a wave -------
+// A wave loads and stores y in whole lines, eight rows of 128 bytes or four of 256 to an instruction, lane after lane:
+// with lanes in the matrix units' order, sixteen rows in turn, the address unit takes four times as long.  The
+// products therefore change lanes, through LDS: rows of 64 f32, 16 bytes apart in their banks.
+constexpr int PITCH = 64 + 4;
+// raw (16 bytes of y) += v (as many values as it has), rounded once.
 template <int YT>
-__device__ __forceinline__ int column(int j, int g, int e) {  // of value e of lane group g in tile j
-  return YT == FP8_IO_F32 ? 16 * j + 4 * g + e : 32 * (j / 2) + 8 * g + 4 * (j % 2) + e;
-}
-// x1 of the lower eight lanes of each sixteen and x0 of the upper eight change places.
-__device__ __forceinline__ void swap_eights(u4& x0, u4& x1) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int a = (int)x0[i], b = (int)x1[i];
-    x1[i] = (uint32_t)__builtin_amdgcn_update_dpp(b, a, 0x128, 0xf, 0x3, false);
-    x0[i] = (uint32_t)__builtin_amdgcn_update_dpp(a, b, 0x128, 0xf, 0xc, false);
-  }
-}
-template <int YT>
-__device__ __forceinline__ void add_to(u4& raw, const f4* v) {  // raw += v, rounded once
+__device__ __forceinline__ u4 add_to(const u4& raw, const f4& v0, const f4& v1) {
   if constexpr (YT == FP8_IO_F32) {
-    raw = __builtin_bit_cast(u4, __builtin_bit_cast(f4, raw) + v[0]);
+    return __builtin_bit_cast(u4, __builtin_bit_cast(f4, raw) + v0);
   } else {
     typedef _Float16 hh __attribute__((ext_vector_type(2)));
     typedef __bf16 bb __attribute__((ext_vector_type(2)));
     typedef float ff __attribute__((ext_vector_type(2)));
+    u4 out;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const uint32_t w = raw[e];
       ff x;
       if constexpr (YT == FP8_IO_F16) x = ff{f16_bits_to_f32(w & 0xffffu), f16_bits_to_f32(w >> 16)};
       else x = ff{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
-      x[0] += v[e / 2][2 * (e % 2)];
-      x[1] += v[e / 2][2 * (e % 2) + 1];
-      if constexpr (YT == FP8_IO_F16) raw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, hh));
-      else raw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bb));
+      x[0] += e < 2 ? v0[2 * e] : v1[2 * e - 4];
+      x[1] += e < 2 ? v0[2 * e + 1] : v1[2 * e - 3];
+      if constexpr (YT == FP8_IO_F16) out[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, hh));
+      else out[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bb));
     }
+    return out;
   }
 }
 // Eight f16 weights as two bf16 parts each.
@@ -370,11 +363,6 @@ __device__ __forceinline__ void split8(const u4& w, u4& hi, u4& lo) {
     hi[e] = ah >> 16 | bh;
     lo[e] = __float_as_uint(a - __uint_as_float(ah)) >> 16 | (__float_as_uint(b - __uint_as_float(bh)) & 0xffff0000u);
   }
-}
-
-// Waves a SIMD that the second product's registers leave room for.
-constexpr int up_occupancy(int YT, bool BF, int STEPS, bool JOIN) {
-  return JOIN || (STEPS == 1 && (BF || YT != FP8_IO_F32)) || (STEPS == 2 && BF && YT != FP8_IO_F32) ? 3 : 2;
 }
 
 // Eight ranks of a row's part, from parts of K that the first product left in f32.
@@ -396,15 +384,28 @@ __device__ __forceinline__ void join8(const float* from, int splits, size_t stri
     }
 }
 
-// A wave walks sixteens of rows, the next two on their way while one is taken, and keeps the weights of the adapter that
-// it met last: STEPS times 32 ranks of its columns, f16 ones as their two parts where registers hold them.  JOIN: few
-// rows, one sixteen and one of its adapters.
-template <int YT, bool BF, int STEPS, bool JOIN>
-__global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, STEPS, JOIN)) void adapter_up_kernel(AdapterArgs p, int splits, int run) {
-  constexpr int PARTS = YT == FP8_IO_F32 ? 3 : 2, SIZE = YT == FP8_IO_F32 ? 4 : 2, PAIRS = YT == FP8_IO_F32 ? 2 : 1;
-  constexpr int PIECE = 64 / SIZE, COUNT = 16 / SIZE;  // values of a piece, and of a lane in it
-  constexpr bool EARLY = STEPS == 1 && !JOIN;          // h of a sixteen comes with its y
+// Three forms: SHORT, ranks up to 16, where the matrix unit's 32 hold a row's parts one after the other; otherwise STEPS
+// times 32 ranks for each part (f16 weights kept as their two parts where registers hold them); JOIN, few rows, one
+// sixteen and one of its adapters.  Except there, a wave walks sixteens of rows, the next one or two on their way
+// while one is taken, and loads weights where the adapter changes.
+enum UpForm : int { SHORT = 0, JOIN = -1 };  // else STEPS
+constexpr int up_occupancy(int YT, bool BF, int FORM) {  // waves a SIMD
+  if (FORM == 4 && !BF) return 1;
+  if (YT == FP8_IO_F32) return FORM <= 0 || (FORM == 1 && BF) ? 3 : 2;
+  return FORM == JOIN || (FORM == SHORT && BF) ? 4 : (FORM <= 1 || BF ? 3 : 2);
+}
+template <int YT, bool BF, int FORM>
+__global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void adapter_up_kernel(AdapterArgs p, int splits, int run) {
+  constexpr int PARTS = YT == FP8_IO_F32 ? 3 : 2, SIZE = YT == FP8_IO_F32 ? 4 : 2;
+  constexpr int PIECES = YT == FP8_IO_F32 ? 4 : 2, COUNT = 16 / SIZE, LANES = COLS / COUNT, STRIDE = 64 / LANES;
+  constexpr int STEPS = FORM > 0 ? FORM : 1;
+  constexpr int TURNS = YT == FP8_IO_F32 ? 2 : 1;  // SHORT: of four eights of ranks
+  constexpr int EARLY = FORM == SHORT ? TURNS : (FORM == 1 || FORM == 2 ? FORM * PARTS : 0);  // pieces of h that come with y
+  constexpr bool APART = !BF && FORM >= 0 && FORM < 4;                                        // f16 weights are kept as their parts
+  constexpr int AHEAD = FORM == SHORT && YT != FP8_IO_F32 ? 2 : 1;                            // sixteens on their way
+  __shared__ f4 stage_all[UP_WAVES][ROWS * PITCH / 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  float* stage = (float*)stage_all[wave];
   // this wave's columns
   int s = 0, n0 = 0, c = (int)blockIdx.x;
   while (true) {
@@ -416,158 +417,228 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, STEPS, JOIN)) v
   n0 += (c * UP_WAVES + wave) * COLS;
   if (n0 >= end) return;
   const int64_t tiles = ((int64_t)p.T + ROWS - 1) / ROWS;
-  const bool in_place = p.y == p.out, upper = r >= 8;
-  const int nm = n0 + (upper ? PIECE : 0) + COUNT * g;  // the first column that the lane loads and stores, pairs 32 apart
+  const bool in_place = p.y == p.out;
+  // what the lane loads and stores: 16 bytes at column lc of rows lr, lr + STRIDE, ..; past the columns' end the first
+  // ones are loaded.  Rows of a sixteen lie within 2^30 bytes.
+  const int lr = lane / LANES, lc = COUNT * (lane % LANES);
+  const bool inside = n0 + lc < end;
+  const uint32_t column = (inside ? lc : 0) * SIZE, pitch_y = (uint32_t)p.ldy * SIZE, pitch_out = (uint32_t)p.ldo * SIZE;
   const u4 zero = u4{0, 0, 0, 0};
+  const int eights = p.R / 8;  // SHORT: 1 or 2
+  const int short_at = eights == 1 ? 0 : 8 * (g & 1);
   struct Tile {
-    u4 y[PAIRS][2], v[EARLY ? PARTS : 1];
-    int id;
+    u4 y[PIECES], v[EARLY ? EARLY : 1];
   };
+  const auto last_of = [&](int64_t tile) { return (int)min((int64_t)ROWS - 1, (int64_t)p.T - 1 - tile * ROWS); };  // its last row
   // loads are unconditional, behind the last row from it
   const auto load = [&](Tile& x, int64_t tile) {
-    const int64_t row0 = tile * ROWS, last = p.T - 1;
+    const int last = last_of(tile);
+    const char* y = (const char*)p.y + (tile * ROWS * p.ldy + n0) * SIZE;
 #pragma unroll
-    for (int m = 0; m < PAIRS; m++)
+    for (int k = 0; k < PIECES; k++) x.y[k] = *(const u4*)(y + ((uint32_t)min(lr + STRIDE * k, last) * pitch_y + column));
+    if constexpr (EARLY > 0) {
+      const char* h = (const char*)p.h + 2 * h_index(tile * ROWS, s, 0, 0, p.S, PARTS, p.R);
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const int n = nm + 32 * m < end ? nm + 32 * m : n0;
-        x.y[m][k] = *(const u4*)((const char*)p.y + (min(row0 + (r & 7) + 8 * k, last) * p.ldy + n) * SIZE);
+      for (int k = 0; k < EARLY; k++) {
+        // SHORT: piece 4 k + g of all; otherwise ranks 32 (k / PARTS) + 8 g of part k % PARTS
+        const int rank0 = FORM == SHORT ? 8 * (4 * k + g) : 32 * (k / PARTS) + 8 * g;
+        const int at = FORM == SHORT ? (rank0 < PARTS * p.R ? rank0 : 0) : (rank0 < p.R ? rank0 : 0) + k % PARTS * p.R;
+        x.v[k] = *(const u4*)(h + (uint32_t)(at * ROWS + r * 8) * 2);
       }
-    const int64_t row = min(row0 + r, last);
-    x.id = p.ids[row];
-    if constexpr (EARLY) {
-      const uint16_t* from = (const uint16_t*)p.h + (row * p.S + s) * PARTS * p.R + (8 * g < p.R ? 8 * g : 0);
-#pragma unroll
-      for (int k = 0; k < PARTS; k++) x.v[k] = *(const u4*)(from + k * p.R);
     }
   };
-  constexpr bool APART = !BF && STEPS < 4 && !JOIN;  // f16 weights are kept as their parts
-  int held = -1, rank = 0;
-  u4 w[JOIN ? 1 : STEPS][4], lo[APART ? STEPS : 1][4];
-  const auto weights = [&](u4 (&v)[4], int t) {  // of ranks 32 t + 8 g .. + 7
+  const auto id_of = [&](int64_t tile) {  // of row r, -1 without an adapter
+    const int last = last_of(tile), v = p.ids[tile * ROWS + min(r, last)];
+    return r <= last && (unsigned)v < (unsigned)p.G ? v : -1;
+  };
+  const auto store = [&](int64_t tile, int k, const u4& v) {
+    char* out = (char*)p.out + (tile * ROWS * p.ldo + n0) * SIZE;
+    if (lr + STRIDE * k <= last_of(tile) && inside) *(u4*)(out + ((uint32_t)(lr + STRIDE * k) * pitch_out + column)) = v;
+  };
+  const auto row_id = [&](int id, int k) { return __builtin_amdgcn_ds_bpermute(4 * (lr + STRIDE * k), id); };  // of a stored row
+  const auto store_none = [&](const Tile& x, int64_t tile, int id) {
+#pragma unroll
+    for (int k = 0; k < PIECES; k++)
+      if (row_id(id, k) == -1) store(tile, k, x.y[k]);
+  };
+  const auto weights = [&](u4 (&v)[4], int current, int at) {  // of ranks at .. + 7
+    int first = n0 + r;
+    asm volatile("" : "+v"(first));  // no address is held from before
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const int n = min(n0 + column<YT>(j, r / 4, r % 4), end - 1), at = 32 * t + 8 * g;
-      v[j] = *(const u4*)((const uint16_t*)p.b + ((size_t)held * p.N + n) * p.R + (at < p.R ? at : 0));
+      const int n = min(first + 16 * j, end - 1);
+      v[j] = *(const u4*)((const uint16_t*)p.b + ((size_t)current * p.N + n) * p.R + (at < p.R ? at : 0));
     }
   };
-  const auto take = [&](const Tile& x, int64_t tile) {
-    const int64_t row0 = tile * ROWS;
-    Adapters<1> ad(p, row0, x.id);
-    const int id = ad.id[0], other = __builtin_amdgcn_update_dpp(0, id, 0x128, 0xf, 0xf, false);
-    // stores the rows of adapter `which`, -1: those of none
-    const auto store = [&](const u4 (&y)[PAIRS][2], int which) {
-      int column = nm;
-      asm volatile("" : "+v"(column));  // no address is held from before
+  const auto apart = [&](const u4 (&f)[4], u4 (&hi)[4], u4 (&low)[4]) {
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const int64_t row = row0 + (r & 7) + 8 * k;
-        if (((k == 1) == upper ? id : other) != which || row >= p.T) continue;
+    for (int j = 0; j < 4; j++) {
+      if constexpr (BF) hi[j] = f[j];
+      else split8(f[j], hi[j], low[j]);
+    }
+  };
+  const auto multiply = [&](f4 (&acc)[4], const u4 (&hi)[4], const u4 (&low)[4], const u4& v) {
 #pragma unroll
-        for (int m = 0; m < PAIRS; m++)
-          if (column + 32 * m < end) *(u4*)((char*)p.out + (row * p.ldo + column + 32 * m) * SIZE) = y[m][k];
-      }
-    };
-    if (!in_place && (!JOIN || blockIdx.z == 0)) store(x.y, -1);
-    if (JOIN) ad.only((int)blockIdx.z);
-    while (ad.next()) {
-      if (ad.current != held) {
-        held = ad.current;
-        rank = rank_of(p, held);
-        if constexpr (!JOIN) {
+    for (int j = 0; j < 4; j++) {
+      acc[j] = mfma<true>(hi[j], v, acc[j]);
+      if constexpr (!BF) acc[j] = mfma<true>(low[j], v, acc[j]);
+    }
+  };
+  // y and the products, in the order of memory, and the rows of adapter `current`
+  const auto finish = [&](const f4 (&acc)[4], const Tile& x, int64_t tile, int id, int current) {
 #pragma unroll
-          for (int t = 0; t < STEPS; t++) weights(w[t], t);
+    for (int j = 0; j < 4; j++) *(f4*)(stage + r * PITCH + 16 * j + 4 * g) = acc[j];
+    // the wave's own region: its lanes' writes come before its reads, and these before the next writes
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int k = 0; k < PIECES; k++) {
+      const float* from = stage + (lr + STRIDE * k) * PITCH + lc;
+      const f4 v0 = *(const f4*)from, v1 = *(const f4*)(from + (COUNT > 4 ? 4 : 0));
+      if (row_id(id, k) == current) store(tile, k, add_to<YT>(x.y[k], v0, v1));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  // Values behind the last part or the adapter's rank count as zeros, like the weights' there: an infinity times zero
+  // would be NaN.
+  if constexpr (FORM == JOIN) {
+    const int64_t tile = blockIdx.y;
+    Tile x;
+    load(x, tile);
+    Adapters<1> ad(p, tile * ROWS);
+    if (!in_place && blockIdx.z == 0) store_none(x, tile, ad.id[0]);
+    ad.only((int)blockIdx.z);
+    if (!ad.next()) return;
+    const int rank = whole_rank(p, given_rank(p, ad.current));
+    const int64_t row = ad.source(0);
+    f4 acc[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int t = 0; 32 * t < p.R; t++) {
+      const int at = 32 * t + 8 * g;
+      u4 w[4], v[PARTS], hi[4], low[4];
+      weights(w, ad.current, at);
+      join8<PARTS>((const float*)p.h + (size_t)row * p.S * p.R + s * p.R + (at < p.R ? at : 0), splits, (size_t)p.T * p.S * p.R, v);
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = at < rank ? w[j] : zero;
+      apart(w, hi, low);
+#pragma unroll
+      for (int k = 0; k < PARTS; k++) multiply(acc, hi, low, at < rank ? v[k] : zero);
+    }
+    finish(acc, x, tile, ad.id[0], ad.current);
+  } else {
+    for (int64_t first = (int64_t)blockIdx.y * run; first < tiles; first += (int64_t)gridDim.y * run) {
+      const int64_t stop = min(first + run, tiles);
+      // the first adapter that rows of `id` wait for, -1: none
+      const auto waiting = [&](int id) {
+        const uint64_t m = __ballot(id >= 0);
+        return m ? __builtin_amdgcn_readlane(id, __builtin_ctzll(m)) : -1;
+      };
+      Tile x, x1, x2;
+      int64_t tile = first;
+      int id = id_of(tile), left = id, next_id = id_of(min(tile + 1, stop - 1));  // left: of rows not yet taken
+      load(x, tile);
+      if constexpr (AHEAD == 2) load(x1, min(tile + 1, stop - 1));
+      bool fresh = true;  // rows without an adapter are yet to come
+      while (tile < stop) {
+        const int current = waiting(left);
+        int rank = 0;
+        u4 w[STEPS][4], lo[APART ? STEPS : 1][4];
+        if (current >= 0) {
+#pragma unroll
+          for (int t = 0; t < STEPS; t++) weights(w[t], current, FORM == SHORT ? short_at : 32 * t + 8 * g);
+          rank = whole_rank(p, given_rank(p, current));
 #pragma unroll
           for (int t = 0; t < STEPS; t++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              w[t][j] = 32 * t + 8 * g < rank ? w[t][j] : zero;
+              w[t][j] = (FORM == SHORT ? short_at : 32 * t + 8 * g) < rank ? w[t][j] : zero;
               if constexpr (APART) {
                 const u4 f = w[t][j];
                 split8(f, w[t][j], lo[t][j]);
               }
             }
         }
-      }
-      f4 acc[4];
+        // Takes the sixteen in `now` for the current adapter, the next one on its way to `later`.  False: another
+        // adapter's turn, in the same sixteen (`same`) or in the next.
+        bool same = false;
+        const auto take = [&](const Tile& now, Tile& later) {
+          const int later_id = id_of(min(tile + 2, stop - 1));
+          load(later, min(tile + AHEAD, stop - 1));
+          if (!in_place && fresh) store_none(now, tile, id);
+          if (current >= 0) {
+            f4 acc[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
-      const int64_t row = ad.source(0);
-      const auto multiply = [&](const u4 (&hi)[4], const u4 (&low)[4], u4 (&v)[PARTS], int t) {
+            for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (FORM == SHORT) {
 #pragma unroll
-        for (int k = 0; k < PARTS; k++) {
-          v[k] = 32 * t + 8 * g < rank ? v[k] : zero;  // an infinity times the weights' zeros would be NaN
+              for (int t = 0; t < TURNS; t++)
+                multiply(acc, w[0], lo[0], 4 * t + g < PARTS * eights && short_at < rank ? now.v[t] : zero);
+            } else {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            acc[j] = mfma<true>(hi[j], v[k], acc[j]);
-            if constexpr (!BF) acc[j] = mfma<true>(low[j], v[k], acc[j]);
+              for (int t = 0; t < STEPS; t++) {
+                const int at = 32 * t + 8 * g;
+                u4 v[PARTS], hi[4], low[4];
+                const char* from = (const char*)p.h + 2 * h_index(tile * ROWS, s, 0, 0, p.S, PARTS, p.R);
+#pragma unroll
+                for (int k = 0; k < PARTS; k++)
+                  v[k] = EARLY ? now.v[EARLY ? PARTS * t + k : 0]
+                               : *(const u4*)(from + (uint32_t)(((at < p.R ? at : 0) + k * p.R) * ROWS + r * 8) * 2);
+                if constexpr (!APART) apart(w[t], hi, low);
+#pragma unroll
+                for (int k = 0; k < PARTS; k++) {
+                  const u4 u = at < rank ? v[k] : zero;
+                  if constexpr (APART) multiply(acc, w[t], lo[t], u);
+                  else multiply(acc, hi, low, u);
+                }
+                if constexpr (STEPS == 4) __builtin_amdgcn_sched_barrier(0);  // all steps' operands at once are too many
+              }
+            }
+            finish(acc, now, tile, id, current);
+            left = left == current ? -1 : left;
           }
-        }
-      };
-      const auto apart = [&](const u4 (&f)[4], u4 (&hi)[4], u4 (&low)[4]) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if constexpr (BF) hi[j] = f[j];
-          else split8(f[j], hi[j], low[j]);
-        }
-      };
-      if constexpr (JOIN) {
-#pragma unroll 1
-        for (int t = 0; 32 * t < p.R; t++) {
-          const int at = 32 * t + 8 * g;
-          weights(w[0], t);
-          u4 v[PARTS], hi[4], low[4];
-          join8<PARTS>((const float*)p.h + (size_t)row * p.S * p.R + s * p.R + (at < p.R ? at : 0), splits, (size_t)p.T * p.S * p.R, v);
-#pragma unroll
-          for (int j = 0; j < 4; j++) w[0][j] = at < rank ? w[0][j] : zero;
-          apart(w[0], hi, low);
-          multiply(hi, low, v, t);
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < STEPS; t++) {
-          const int at = 32 * t + 8 * g;
-          u4 v[PARTS];
-          const uint16_t* from = (const uint16_t*)p.h + (row * p.S + s) * PARTS * p.R + (at < p.R ? at : 0);
-#pragma unroll
-          for (int k = 0; k < PARTS; k++) v[k] = EARLY ? x.v[EARLY ? k : 0] : *(const u4*)(from + k * p.R);
-          if constexpr (BF || APART) {
-            multiply(w[t], lo[APART ? t : 0], v, t);
+          if (current >= 0 && waiting(left) >= 0) {
+            fresh = false;
+            same = true;
+            return false;
+          }
+          tile++;
+          id = left = next_id;
+          next_id = later_id;
+          fresh = true;
+          return tile < stop && waiting(left) == current;
+        };
+        // the sixteens' registers take turns: moved from one to the next, they would have to have arrived
+        while (true) {
+          if constexpr (AHEAD == 2) {
+            if (!take(x, x2)) {
+              if (!same) x = x1, x1 = x2;
+              break;
+            }
+            if (!take(x1, x)) {
+              if (same) x = x1, x1 = x2;
+              else x1 = x, x = x2;
+              break;
+            }
+            if (!take(x2, x1)) {
+              if (same) x1 = x, x = x2;
+              break;
+            }
           } else {
-            u4 hi[4], low[4];
-            apart(w[t], hi, low);
-            multiply(hi, low, v, t);
+            if (!take(x, x1)) {
+              if (!same) x = x1;
+              break;
+            }
+            if (!take(x1, x)) {
+              if (same) x = x1;
+              break;
+            }
           }
         }
-      }
-      u4 y[PAIRS][2];
-#pragma unroll
-      for (int m = 0; m < PAIRS; m++) {
-        y[m][0] = x.y[m][0], y[m][1] = x.y[m][1];
-        swap_eights(y[m][0], y[m][1]);
-        add_to<YT>(y[m][0], &acc[YT == FP8_IO_F32 ? 2 * m : 0]);
-        add_to<YT>(y[m][1], &acc[YT == FP8_IO_F32 ? 2 * m + 1 : 2]);
-        swap_eights(y[m][0], y[m][1]);
-      }
-      store(y, ad.current);
-    }
-  };
-  for (int64_t first = (int64_t)blockIdx.y * run; first < tiles; first += (int64_t)gridDim.y * run) {
-    const int64_t stop = min(first + run, tiles);
-    if constexpr (JOIN) {
-      Tile x;
-      load(x, first);
-      take(x, first);
-    } else {
-      Tile x, x1;
-      load(x, first);
-      load(x1, min(first + 1, stop - 1));
-#pragma unroll 1
-      for (int64_t tile = first; tile < stop; tile++) {
-        Tile x2;
-        load(x2, min(tile + 2, stop - 1));
-        take(x, tile);
-        x = x1, x1 = x2;
       }
     }
   }
@@ -633,25 +704,27 @@ hipError_t launch_down_plan(const AdapterArgs& a, const Plan& q, hipStream_t s) 
   return launch_down_ranks<CODES, BF, 4>(a, q, s);
 }
 
-template <int YT, bool BF, int STEPS>
-hipError_t launch_up_steps(const AdapterArgs& a, int blocks, hipStream_t s) {
+template <int YT, bool BF, int FORM>
+hipError_t launch_up_form(const AdapterArgs& a, int blocks, hipStream_t s) {
   const int64_t sixteens = ((int64_t)a.T + ROWS - 1) / ROWS;
-  // sixteens of rows of a workgroup, so that there are workgroups for every place twice
-  const int run = (int)std::max<int64_t>(1, std::min<int64_t>(32, sixteens * blocks / 2048));
+  // sixteens of rows of a workgroup, so that all workgroups have a place at once
+  const int64_t places = 256 * up_occupancy(YT, BF, FORM);
+  const int run = (int)std::max<int64_t>(1, std::min<int64_t>(64, (sixteens * blocks + places - 1) / places));
   const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>((sixteens + run - 1) / run, 65535));
-  T5K_LAUNCH((adapter_up_kernel<YT, BF, STEPS, false>), grid, dim3(64 * UP_WAVES), 0, s, a, 1, run);
+  T5K_LAUNCH((adapter_up_kernel<YT, BF, FORM>), grid, dim3(64 * UP_WAVES), 0, s, a, 1, run);
   return hipGetLastError();
 }
 template <int YT, bool BF>
 hipError_t launch_up(const AdapterArgs& a, const Plan& q, int blocks, hipStream_t s) {
   if (q.few) {
     const dim3 grid((unsigned)blocks, (unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)std::min(ROWS, a.T));
-    T5K_LAUNCH((adapter_up_kernel<YT, BF, 1, true>), grid, dim3(64 * UP_WAVES), 0, s, a, q.splits, 1);
+    T5K_LAUNCH((adapter_up_kernel<YT, BF, JOIN>), grid, dim3(64 * UP_WAVES), 0, s, a, q.splits, 1);
     return hipGetLastError();
   }
-  if (a.R <= 32) return launch_up_steps<YT, BF, 1>(a, blocks, s);
-  if (a.R <= 64) return launch_up_steps<YT, BF, 2>(a, blocks, s);
-  return launch_up_steps<YT, BF, 4>(a, blocks, s);
+  if (a.R <= 16) return launch_up_form<YT, BF, SHORT>(a, blocks, s);
+  if (a.R <= 32) return launch_up_form<YT, BF, 1>(a, blocks, s);
+  if (a.R <= 64) return launch_up_form<YT, BF, 2>(a, blocks, s);
+  return launch_up_form<YT, BF, 4>(a, blocks, s);
 }
 template <bool BF>
 hipError_t launch(const AdapterArgs& a, hipStream_t s) {
@@ -672,7 +745,8 @@ hipError_t launch(const AdapterArgs& a, hipStream_t s) {
 namespace t5k {
 size_t adapter_work_bytes(int T, int K, int SR) {
   const Plan q = plan_of(T, K, SR);
-  return (size_t)T * SR * (q.few ? 4 * (size_t)q.splits : 6);
+  if (q.few) return (size_t)q.splits * T * SR * 4;
+  return ((size_t)T + ROWS - 1) / ROWS * ROWS * SR * 6;  // three parts of 16 bits, whole sixteens of rows
 }
 
 hipError_t launch_adapter(const AdapterArgs& a, hipStream_t s) {
