@@ -354,8 +354,8 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
  * (within 2^-17 of it for bf16 adapters under 16-bit results, 2^-22 otherwise); results are rounded once.
  * Adapters are finite; an infinity or NaN in a row stays in that row.
  * K is a multiple of 16 up to 2^21, R one of 8 up to 128, columns of a slice one of 16 up to 2^24; T up to
- * 2^30, G up to 2^24.  Rows of x, y and out start on multiples of 16 bytes and are up to 2^24 values apart; a,
- * b and the workspace start on 16 bytes.  Device buffers lie on the current device; the call is enqueued on `stream`
+ * 2^30 (codes: their scales below 2^31 bytes), G up to 2^24.  Rows of x, y and out start on multiples of 16 bytes and are up to 2^24 values apart; a,
+ * b, the scales of codes and the workspace start on 16 bytes.  Device buffers lie on the current device; the call is enqueued on `stream`
  * (a hipStream_t; NULL = the default stream) and returns without waiting.  It allocates nothing and keeps no
  * state: intermediate sums live in d_work, of at least t5h_adapter_workspace's bytes, which serves one call
  * (or replay of a graph that holds one) at a time. */

@@ -40,7 +40,7 @@ def _call(x=P, xt=1, xs=None, ldx=128, T=5, K=128, ids=P, G=3, a=P, b=P, wt=1, r
     (dict(wt=2, xt=1), "type"), (dict(yt=3), "type of results"), (dict(yt=-1), "type of results"), (dict(cols=None, slices=1), "NULL columns"),
     (dict(cols=(64, 24)), "columns"), (dict(cols=(0,)), "columns"), (dict(cols=(-16, 64)), "columns"), (dict(cols=((1 << 24) + 16,)), "columns"),
     (dict(x=None), "NULL x"), (dict(y=None), "NULL y"), (dict(out=None), "NULL out"), (dict(ids=None), "NULL ids"), (dict(a=None), "NULL a"),
-    (dict(b=None), "NULL b"), (dict(work=None), "NULL workspace"), (dict(xt=3), "NULL scales"), (dict(x=P + 8), "x is not aligned"),
+    (dict(b=None), "NULL b"), (dict(work=None), "NULL workspace"), (dict(xt=3), "NULL scales"), (dict(xt=3, xs=P + 8), "scales of x is not aligned"), (dict(xt=3, xs=P, T=1 << 30, K=256), "2^31"), (dict(x=P + 8), "x is not aligned"),
     (dict(y=P + FAR + 4), "y is not aligned"), (dict(out=P + 2), "out is not aligned"), (dict(a=P + 8), "a is not aligned"),
     (dict(b=P + 8), "b is not aligned"), (dict(ids=P + 2), "ids is not aligned"), (dict(ranks=P + 1), "ranks is not aligned"),
     (dict(scales=P + 2), "scales is not aligned"), (dict(work=P + 4), "workspace is not aligned"), (dict(ldx=120), "x's rows"),

@@ -34,6 +34,8 @@ int check_shape(int32_t x_type, int32_t T, int32_t K, int32_t G, int32_t w_type,
   if (w_type != T5H_TYPE_F16 && w_type != T5H_TYPE_BF16) return bad("adapters must be f16 or bf16");
   if (x_type != w_type && x_type != T5H_TYPE_E4M3) return bad("rows must be of the adapters' type, or e4m3 codes");
   if (!known_type(y_type)) return bad("unknown type of results");
+  if (x_type == T5H_TYPE_E4M3 && (((uint64_t)K + t5k::FP8_BLOCK - 1) / t5k::FP8_BLOCK * t5k::fp8_scale_rows(T)) >> 31)
+    return bad("scales of x of 2^31 bytes or more");
   if (!cols) return bad("NULL columns");
   N = 0;
   for (int32_t i = 0; i < slices; i++) {
@@ -81,7 +83,7 @@ int t5h_adapter_add_device(const void* d_x, int32_t x_type, const uint8_t* d_x_s
   TRY(check_rows(y, ldy, N));
   TRY(check_rows(out, ldo, N));
   if (!(y.at == out.at && y.stride == out.stride) && overlap(y, out, T)) return bad("out overlaps y without being y");
-  if (x_type == T5H_TYPE_E4M3) TRY(check_buffer(d_x_scales, "scales of x", 1));
+  if (x_type == T5H_TYPE_E4M3) TRY(check_buffer(d_x_scales, "scales of x", 16));
   TRY(check_buffer(d_ids, "ids", 4));
   if (G) {
     TRY(check_buffer(d_a, "a", 16));

@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "fp8.hpp"
+#include "lds_copy.hpp"
 
 namespace {
 using namespace t5k;
@@ -28,8 +29,7 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int ROWS = 16;        // of a matrix instruction
-constexpr int STEP = 128;       // K values of a step of the first product
-constexpr int FEW_STEP = 64;    // of the one for few rows
+constexpr int FEW_STEP = 64;    // K values of a step of the first product for few rows
 constexpr int FEW_WAVES = 8;    // its waves, at most
 constexpr int COLS = 64;        // columns of a wave in the second product
 constexpr int UP_WAVES = 4;     // its waves, on columns beside each other
@@ -200,83 +200,104 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(Adapte
 }
 
 // ---- h = scale x A^T, many rows: 64 rows x 16 RT ranks per workgroup --------------------------------
-// 4 KG waves: four of sixteen rows each, KG times over, on steps of 128 K in turn.  A goes through LDS, loaded in whole
-// rows by the four waves that share it and read in the operand's order; a row's sixteen 16-byte chunks are stored
-// rotated (xor) by its number, so that sixteen rows at once spread over all banks.  x goes straight to registers,
-// where the lanes of a load lie in sixteen rows: that costs the address unit a quarter of its rate, which x alone can
-// bear.  The next step's loads are on their way while one is multiplied.  The KG sums meet in LDS and are added in order.
+// Steps of 128 bytes of x's rows (64 values, or 128 codes) through a ring of STAGES in LDS: copies in whole rows, eight
+// of 128 bytes to an instruction, straight from memory.  A row's eight 16-byte chunks are stored rotated (xor) by its
+// number, so that eight rows' same chunk, which a read takes at a time, lie in different banks.  Four waves of sixteen
+// rows each read x once and A between them; with KG = 2 four more take every other step, and the sums meet in LDS.
+// A wait and a barrier per step: stage n has been requested STAGES - 1 steps ahead.  Chunks past K, and steps past
+// the last, are copied from outside the descriptors' range, as zeros.
+template <bool CODES, int RT>
+struct Ring {
+  static constexpr int ROW_BYTES = 4 * ROWS * 128, HALVES = CODES ? 2 : 1;  // of x; pieces of 128 bytes of A's rows
+  static constexpr int A_BYTES = HALVES * RT * ROWS * 128, A_COPIES = A_BYTES / 1024;  // copies of four waves
+  // behind them the scales of codes, one copy a wave, or room for the copies of waves that have none of A's
+  static constexpr int REST = CODES ? 4 * 256 : (A_COPIES % 4 ? 1024 : 0);
+  static constexpr int STAGE = ROW_BYTES + A_BYTES + REST;
+  static constexpr int STAGES = STAGE <= 16384 ? 4 : 3;
+  static constexpr int COPIES = 2 + (A_COPIES + 3) / 4 + (CODES ? 1 : 0);  // of a wave, the same for all
+};
 template <bool CODES, bool BF, int RT, int KG>
-__global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : 3) void adapter_down_kernel(AdapterArgs p, int parts) {
-  constexpr int BUFFER = RT * ROWS * STEP * 2;  // bytes of A's ranks of a step
-  extern __shared__ char lds[];                 // [KG][2][BUFFER]; the sums: [KG][4][RT][64] f4, no more
+__global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p, int parts) {
+  typedef Ring<CODES, RT> Lds;
+  __shared__ __attribute__((aligned(1024))) char lds[KG * Lds::STAGES * Lds::STAGE];  // the sums: [4][RT][64] f4, no more
+  constexpr int SIZE = CODES ? 1 : 2, K_STEP = 128 / SIZE, STAGES = Lds::STAGES;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int rw = wave & 3, kg = wave >> 2, tid = threadIdx.x & 255;
-  const int SR = p.S * p.R, steps = (p.K + STEP - 1) / STEP, group = (int)blockIdx.y;
+  const int rw = wave & 3, kg = wave >> 2;
+  const int SR = p.S * p.R, steps = (p.K + K_STEP - 1) / K_STEP, turns = (steps + KG - 1) / KG, group = (int)blockIdx.y;
   const size_t m16 = fp8_scale_rows(p.T);
   const int64_t tiles = ((int64_t)p.T + 4 * ROWS - 1) / (4 * ROWS);
-  char* mine = lds + kg * 2 * BUFFER;
-  const u4 zero = u4{0, 0, 0, 0};
+  const uint32_t lds0 = lds_offset(lds) + (uint32_t)(kg * STAGES * Lds::STAGE);
+  char* mine = lds + kg * STAGES * Lds::STAGE;
+  const int cr = lane >> 3, cc = (lane & 7) ^ cr;  // the row of eight and the chunk that the lane copies
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t row0 = tile * 4 * ROWS;
+    const int rows = (int)min((int64_t)4 * ROWS, p.T - row0);
     Adapters<4> ad(p, row0);
     for (unsigned seen = 0; ad.next(); seen++) {
       if (seen % gridDim.z != blockIdx.z) continue;
       const float scale = p.scales ? p.scales[ad.current] : 1.f;
+      const int given = given_rank(p, ad.current);
       const int id = rw == 0 ? ad.id[0] : (rw == 1 ? ad.id[1] : (rw == 2 ? ad.id[2] : ad.id[3]));
       const int64_t row = row0 + ROWS * rw + r;
-      const int64_t at = id == ad.current ? row : ad.row;  // of rows whose result nothing keeps, one that is read anyway
-      const uint16_t* a = (const uint16_t*)p.a + (size_t)ad.current * SR * p.K;
-      struct Step {
-        u4 a[RT], x[CODES ? 2 : 4];
-        uint32_t scale;
-      };
-      // loads are unconditional, past the rows' end from their start: a branch around each would cost registers
-      const auto load = [&](Step& v, int n) {
+      // this wave's copies: rows 16 rw + 8 i + cr of x (in the place of those whose result nothing keeps, one that is
+      // copied anyway), eights of A's ranks
+      const i4v x_at = buffer_at((const char*)p.x + row0 * p.ldx * SIZE, (uint32_t)((rows - 1) * p.ldx + p.K) * SIZE);
+      uint32_t x_off[2];
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-          const int c = tid + 256 * i, k = n * STEP + 8 * (c & 15);
-          v.a[i] = *(const u4*)(a + (size_t)min(ROWS * RT * group + c / 16, SR - 1) * p.K + (k < p.K ? k : 0));
-        }
+      for (int i = 0; i < 2; i++) {
+        const int other = __builtin_amdgcn_ds_bpermute(4 * (8 * i + cr), id);
+        const int from = other == ad.current ? ROWS * rw + 8 * i + cr : (int)(ad.row - row0);
+        x_off[i] = (uint32_t)(from * p.ldx * SIZE) + 16 * cc;
+      }
+      const int j0 = ROWS * RT * group, ranks = min(ROWS * RT, SR - j0);
+      const i4v a_at = buffer_at((const uint16_t*)p.a + ((size_t)ad.current * SR + j0) * p.K, (uint32_t)ranks * p.K * 2);
+      const i4v s_at = buffer_at(CODES ? (const void*)p.x_scales : p.x, CODES ? (uint32_t)(steps * m16) : 0u);
+      const auto copy = [&](int turn) {
+        const int n = turn * KG + kg;
+        const uint32_t stage = lds0 + (uint32_t)(turn % STAGES) * Lds::STAGE;
+        const bool ok = n * K_STEP + cc * (16 / SIZE) < p.K;
 #pragma unroll
-        for (int e = 0; e < (CODES ? 2 : 4); e++) {
-          const int k = n * STEP + (CODES ? 16 * (g + 4 * e) : 8 * (g + 4 * e));
-          v.x[e] = *(const u4*)((const char*)p.x + (at * p.ldx + (k < p.K ? k : 0)) * (CODES ? 1 : 2));
+        for (int i = 0; i < 2; i++) lds_copy16(x_at, ok ? x_off[i] + (uint32_t)n * 128 : kOutside, 0, stage + (2 * rw + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < Lds::A_COPIES; i += 4) {
+          // piece c: eight ranks, codes: of one half of a step; a wave without one copies zeros behind the last
+          const int c = i + rw, half = c / (2 * RT), j = c % (2 * RT) * 8 + cr, k = (n * Lds::HALVES + half) * 64 + 8 * cc;
+          const bool is = c < Lds::A_COPIES && j < ranks && k < p.K;
+          lds_copy16(a_at, is ? (uint32_t)(j * p.K + k) * 2 : kOutside, 0, stage + Lds::ROW_BYTES + min(c, (int)Lds::A_COPIES) * 1024);
         }
-        if constexpr (CODES) v.scale = p.x_scales[(size_t)min(n, steps - 1) * m16 + at];
+        if constexpr (CODES)
+          lds_copy4(s_at, lane < 4 && n < steps ? (uint32_t)(n * m16 + row0 + ROWS * rw + 4 * lane) : kOutside, 0,
+                    stage + Lds::ROW_BYTES + Lds::A_BYTES + rw * 256);
       };
       f4 acc[RT];
 #pragma unroll
       for (int q = 0; q < RT; q++) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
-      Step u;
-      load(u, kg);
-      const int given = given_rank(p, ad.current);
-#pragma unroll 2
-      for (int i = 0; i * KG < steps; i++) {
-        const int n = i * KG + kg;
-        char* buffer = mine + (i & 1) * BUFFER;
 #pragma unroll
-        for (int k = 0; k < RT; k++) {
-          const int c = tid + 256 * k, j = c / 16;
-          *(u4*)(buffer + j * 256 + ((c ^ j) & 15) * 16) = u.a[k];
-        }
-        Step v;
-        load(v, n + KG);
-        __syncthreads();  // the buffer is whole; it is written again past the next one's barrier
-        u4 x[4];
+      for (int i = 0; i < STAGES - 1; i++) copy(i);
+#pragma unroll 1
+      for (int turn = 0; turn < turns; turn++) {
+        // this turn's stage is whole, and the last one's has been read by all
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * Lds::COPIES) : "memory");
+        copy(turn + STAGES - 1);
+        const char* stage = mine + turn % STAGES * Lds::STAGE;
+        const char* xs = stage + (ROWS * rw + r) * 128;
+        const char* as = stage + Lds::ROW_BYTES + r * 128;
+        u4 x[CODES ? 4 : 2];
 #pragma unroll
-        for (int e = 0; e < (CODES ? 2 : 4); e++) {
-          const u4 c = n * STEP + (CODES ? 16 * (g + 4 * e) : 8 * (g + 4 * e)) < p.K ? u.x[e] : zero;
+        for (int e = 0; e < 2; e++) {
+          const u4 c = *(const u4*)(xs + (((g + 4 * e) ^ r) & 7) * 16);
           if constexpr (CODES) x[2 * e] = widen8<BF>(c[0], c[1]), x[2 * e + 1] = widen8<BF>(c[2], c[3]);
           else x[e] = c;
         }
-        const float f = CODES ? e8m0_value(u.scale) : 1.f;
+        const float f = CODES ? e8m0_value((uint8_t)stage[Lds::ROW_BYTES + Lds::A_BYTES + rw * 256 + r]) : 1.f;
 #pragma unroll
         for (int q = 0; q < RT; q++) {
           f4 t = CODES ? f4{0.f, 0.f, 0.f, 0.f} : acc[q];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int c = CODES ? 2 * (g + 4 * (e / 2)) + e % 2 : g + 4 * e;  // the chunk with the same K values
-            t = mfma<BF>(*(const u4*)(buffer + (ROWS * q + r) * 256 + ((c ^ r) & 15) * 16), x[e], t);
+          for (int e = 0; e < (CODES ? 4 : 2); e++) {
+            // the chunk with the same K values, of which codes have two in one of x's
+            const int c = CODES ? 2 * g + e % 2 : g + 4 * e, half = CODES ? e / 2 : 0;
+            t = mfma<BF>(*(const u4*)(as + (half * RT + q) * ROWS * 128 + ((c ^ r) & 7) * 16), x[e], t);
           }
           if constexpr (CODES) {
 #pragma unroll
@@ -285,28 +306,25 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : 3) void adapter_down_kernel
             acc[q] = t;
           }
         }
-        u = v;
       }
-      __syncthreads();  // the buffers are free
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the ring is free
       if constexpr (KG > 1) {
+        if (kg > 0) {
 #pragma unroll
-        for (int q = 0; q < RT; q++) ((f4*)lds)[(wave * RT + q) * 64 + lane] = acc[q];
+          for (int q = 0; q < RT; q++) ((f4*)lds)[(rw * RT + q) * 64 + lane] = acc[q];
+        }
         __syncthreads();
       }
       const int rank = whole_rank(p, given);
       int gg = g;
-      asm volatile("" : "+v"(gg));  // the addresses of results are left to be computed here
-      if (id == ad.current) {       // -1 behind the last row
+      asm volatile("" : "+v"(gg));           // the addresses of results are left to be computed here
+      if (id == ad.current && kg == 0) {  // -1 behind the last row
 #pragma unroll
         for (int q = 0; q < RT; q++) {
-          const int j = ROWS * (group * RT + q) + 4 * gg;
-          if (q % KG != kg || j >= SR) continue;
+          const int j = j0 + ROWS * q + 4 * gg;
+          if (j >= SR) continue;
           f4 v = acc[q];
-          if constexpr (KG > 1) {
-            v = ((f4*)lds)[(rw * RT + q) * 64 + lane];
-#pragma unroll
-            for (int k = 1; k < KG; k++) v += ((f4*)lds)[((4 * k + rw) * RT + q) * 64 + lane];
-          }
+          if constexpr (KG > 1) v += ((f4*)lds)[(rw * RT + q) * 64 + lane];
           const int slice = j / p.R, at_rank = j - slice * p.R;
           float rest[4];  // values past the adapter's rank may come from anything
 #pragma unroll
@@ -663,10 +681,9 @@ Plan plan_of(int T, int K, int SR) {
     q.ranks = 1;
     return q;
   }
-  const int steps = (K + STEP - 1) / STEP;
   q.ranks = tiles <= 4 ? tiles : (tiles % 3 == 0 ? 3 : 4);
   const int64_t blocks = ((int64_t)T + 4 * ROWS - 1) / (4 * ROWS) * ((tiles + q.ranks - 1) / q.ranks);
-  q.waves = blocks >= 768 || steps < 2 ? 1 : (blocks >= 192 || steps < 4 ? 2 : 4);
+  q.waves = blocks >= 512 ? 1 : 2;
   return q;
 }
 
@@ -676,8 +693,7 @@ hipError_t launch_down(const AdapterArgs& a, hipStream_t s) {
   const int64_t rows = ((int64_t)a.T + 4 * ROWS - 1) / (4 * ROWS);
   // a tile with the rows of several short requests would take as many turns: workgroups share them while there is room
   const dim3 grid((unsigned)std::min<int64_t>(rows, 1 << 20), (unsigned)groups, rows * groups < 768 ? 4 : 1);
-  const size_t lds = (size_t)KG * 2 * RT * ROWS * STEP * 2;
-  T5K_LAUNCH((adapter_down_kernel<CODES, BF, RT, KG>), grid, dim3(256 * KG), lds, s, a, a.y_type == FP8_IO_F32 ? 3 : 2);
+  T5K_LAUNCH((adapter_down_kernel<CODES, BF, RT, KG>), grid, dim3(256 * KG), 0, s, a, a.y_type == FP8_IO_F32 ? 3 : 2);
   return hipGetLastError();
 }
 template <bool CODES, bool BF, int KG>
@@ -697,11 +713,7 @@ hipError_t launch_down_plan(const AdapterArgs& a, const Plan& q, hipStream_t s) 
     T5K_LAUNCH((adapter_down_few_kernel<CODES, BF>), grid, dim3(64 * q.waves), 0, s, a, q.splits);
     return hipGetLastError();
   }
-  switch (q.waves) {
-    case 1: return launch_down_ranks<CODES, BF, 1>(a, q, s);
-    case 2: return launch_down_ranks<CODES, BF, 2>(a, q, s);
-  }
-  return launch_down_ranks<CODES, BF, 4>(a, q, s);
+  return q.waves == 1 ? launch_down_ranks<CODES, BF, 1>(a, q, s) : launch_down_ranks<CODES, BF, 2>(a, q, s);
 }
 
 template <int YT, bool BF, int FORM>
