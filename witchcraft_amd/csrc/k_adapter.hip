@@ -206,19 +206,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(Adapte
 // rows each read x once and A between them; with KG = 2 four more take every other step, and the sums meet in LDS.
 // A wait and a barrier per step: stage n has been requested STAGES - 1 steps ahead.  Chunks past K, and steps past
 // the last, are copied from outside the descriptors' range, as zeros.
-template <bool CODES, int RT>
+template <bool CODES, int RT, int KG>
 struct Ring {
   static constexpr int ROW_BYTES = 4 * ROWS * 128, HALVES = CODES ? 2 : 1;  // of x; pieces of 128 bytes of A's rows
   static constexpr int A_BYTES = HALVES * RT * ROWS * 128, A_COPIES = A_BYTES / 1024;  // copies of four waves
   // behind them the scales of codes, one copy a wave, or room for the copies of waves that have none of A's
   static constexpr int REST = CODES ? 4 * 256 : (A_COPIES % 4 ? 1024 : 0);
   static constexpr int STAGE = ROW_BYTES + A_BYTES + REST;
-  static constexpr int STAGES = STAGE <= 16384 ? 4 : 3;
+  static constexpr int STAGES = KG * STAGE <= 16384 ? 3 : 2;               // two workgroups on a compute unit
   static constexpr int COPIES = 2 + (A_COPIES + 3) / 4 + (CODES ? 1 : 0);  // of a wave, the same for all
 };
 template <bool CODES, bool BF, int RT, int KG>
 __global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p, int parts) {
-  typedef Ring<CODES, RT> Lds;
+  typedef Ring<CODES, RT, KG> Lds;
   __shared__ __attribute__((aligned(1024))) char lds[KG * Lds::STAGES * Lds::STAGE];  // the sums: [4][RT][64] f4, no more
   constexpr int SIZE = CODES ? 1 : 2, K_STEP = 128 / SIZE, STAGES = Lds::STAGES;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
@@ -239,35 +239,44 @@ __global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p
       const int given = given_rank(p, ad.current);
       const int id = rw == 0 ? ad.id[0] : (rw == 1 ? ad.id[1] : (rw == 2 ? ad.id[2] : ad.id[3]));
       const int64_t row = row0 + ROWS * rw + r;
-      // this wave's copies: rows 16 rw + 8 i + cr of x (in the place of those whose result nothing keeps, one that is
-      // copied anyway), eights of A's ranks
+      // This wave's copies: rows 16 rw + 8 i + cr of x (in the place of those whose result nothing keeps, one that is
+      // copied anyway), and pieces i + rw of A: eight ranks, codes: of one half of a step.  A wave without one copies zeros
+      // behind the last.
       const i4v x_at = buffer_at((const char*)p.x + row0 * p.ldx * SIZE, (uint32_t)((rows - 1) * p.ldx + p.K) * SIZE);
-      uint32_t x_off[2];
+      const int j0 = ROWS * RT * group, ranks = min(ROWS * RT, SR - j0);
+      const i4v a_at = buffer_at((const uint16_t*)p.a + ((size_t)ad.current * SR + j0) * p.K, (uint32_t)ranks * p.K * 2);
+      const i4v s_at = buffer_at(CODES ? (const void*)p.x_scales : p.x, CODES ? (uint32_t)(steps * m16) : 0u);
+      uint32_t x_off[2], a_off[(Lds::A_COPIES + 3) / 4];
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int other = __builtin_amdgcn_ds_bpermute(4 * (8 * i + cr), id);
         const int from = other == ad.current ? ROWS * rw + 8 * i + cr : (int)(ad.row - row0);
         x_off[i] = (uint32_t)(from * p.ldx * SIZE) + 16 * cc;
       }
-      const int j0 = ROWS * RT * group, ranks = min(ROWS * RT, SR - j0);
-      const i4v a_at = buffer_at((const uint16_t*)p.a + ((size_t)ad.current * SR + j0) * p.K, (uint32_t)ranks * p.K * 2);
-      const i4v s_at = buffer_at(CODES ? (const void*)p.x_scales : p.x, CODES ? (uint32_t)(steps * m16) : 0u);
+#pragma unroll
+      for (int i = 0; i < (Lds::A_COPIES + 3) / 4; i++) {
+        const int c = 4 * i + rw, half = c / (2 * RT), j = c % (2 * RT) * 8 + cr;
+        a_off[i] = c < Lds::A_COPIES && j < ranks ? (uint32_t)(j * p.K + 64 * half + 8 * cc) * 2 : kOutside;
+      }
+      const uint32_t s_off = lane < 4 ? (uint32_t)(row0 + ROWS * rw + 4 * lane) : kOutside;
+      // Workgroups begin at different steps: with all at the same one the 32 compute units of an XCD, whose workgroups are
+      // every eighth, want the same few lines of A at a time.
+      const int shift = (int)((tile / 8) % steps);
       const auto copy = [&](int turn) {
-        const int n = turn * KG + kg;
+        const int at = turn * KG + kg, n = at + shift - (at + shift >= steps ? steps : 0);
         const uint32_t stage = lds0 + (uint32_t)(turn % STAGES) * Lds::STAGE;
-        const bool ok = n * K_STEP + cc * (16 / SIZE) < p.K;
+        const int left = at < steps ? p.K - n * K_STEP : 0;  // values of this step
+        const uint32_t soff = (uint32_t)n * 128;
 #pragma unroll
-        for (int i = 0; i < 2; i++) lds_copy16(x_at, ok ? x_off[i] + (uint32_t)n * 128 : kOutside, 0, stage + (2 * rw + i) * 1024);
+        for (int i = 0; i < 2; i++)
+          lds_copy16(x_at, cc * (16 / SIZE) < left ? x_off[i] : kOutside, soff, stage + (2 * rw + i) * 1024);
 #pragma unroll
-        for (int i = 0; i < Lds::A_COPIES; i += 4) {
-          // piece c: eight ranks, codes: of one half of a step; a wave without one copies zeros behind the last
-          const int c = i + rw, half = c / (2 * RT), j = c % (2 * RT) * 8 + cr, k = (n * Lds::HALVES + half) * 64 + 8 * cc;
-          const bool is = c < Lds::A_COPIES && j < ranks && k < p.K;
-          lds_copy16(a_at, is ? (uint32_t)(j * p.K + k) * 2 : kOutside, 0, stage + Lds::ROW_BYTES + min(c, (int)Lds::A_COPIES) * 1024);
+        for (int i = 0; i < (Lds::A_COPIES + 3) / 4; i++) {
+          const int c = 4 * i + rw, half = c / (2 * RT);
+          lds_copy16(a_at, 64 * half + 8 * cc < left ? a_off[i] : kOutside, soff * Lds::HALVES,
+                     stage + Lds::ROW_BYTES + min(c, (int)Lds::A_COPIES) * 1024);
         }
-        if constexpr (CODES)
-          lds_copy4(s_at, lane < 4 && n < steps ? (uint32_t)(n * m16 + row0 + ROWS * rw + 4 * lane) : kOutside, 0,
-                    stage + Lds::ROW_BYTES + Lds::A_BYTES + rw * 256);
+        if constexpr (CODES) lds_copy4(s_at, left > 0 ? s_off : kOutside, (uint32_t)(n * m16), stage + Lds::ROW_BYTES + Lds::A_BYTES + rw * 256);
       };
       f4 acc[RT];
 #pragma unroll
@@ -683,7 +692,7 @@ Plan plan_of(int T, int K, int SR) {
   }
   q.ranks = tiles <= 4 ? tiles : (tiles % 3 == 0 ? 3 : 4);
   const int64_t blocks = ((int64_t)T + 4 * ROWS - 1) / (4 * ROWS) * ((tiles + q.ranks - 1) / q.ranks);
-  q.waves = blocks >= 512 ? 1 : 2;
+  q.waves = blocks > 512 ? 1 : 2;
   return q;
 }
 
