@@ -31,7 +31,6 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int ROWS = 16;        // of a matrix instruction
 constexpr int FEW_STEP = 64;    // K values of a step of the first product for few rows
 constexpr int FEW_WAVES = 8;    // its waves, at most
-constexpr int COLS = 64;        // columns of a wave in the second product
 constexpr int UP_WAVES = 4;     // its waves, on columns beside each other
 
 template <bool BF>
@@ -352,11 +351,10 @@ __global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p
   }
 }
 
-// ---- out = y + h B^T: 16 rows x 256 columns of one slice per workgroup and turn, 64 columns a wave -------
-// A wave loads and stores y in whole lines, eight rows of 128 bytes or four of 256 to an instruction, lane after lane:
-// with lanes in the matrix units' order, sixteen rows in turn, the address unit takes four times as long.  The
-// products therefore change lanes, through LDS: rows of 64 f32, 16 bytes apart in their banks.
-constexpr int PITCH = 64 + 4;
+// ---- out = y + h B^T: 16 rows x 64 columns (32 for ranks past 64) of one slice per wave and turn, four waves side by side --
+// A wave loads and stores y in whole rows, eight of 128 bytes or four of 256 to an instruction, lane after lane: with
+// lanes in the matrix units' order, sixteen rows in turn, the address unit takes four times as long.  The products
+// therefore change lanes, through LDS: rows of f32, 16 bytes apart in their banks.
 // raw (16 bytes of y) += v (as many values as it has), rounded once.
 template <int YT>
 __device__ __forceinline__ u4 add_to(const u4& raw, const f4& v0, const f4& v1) {
@@ -412,23 +410,23 @@ __device__ __forceinline__ void join8(const float* from, int splits, size_t stri
 }
 
 // Three forms: SHORT, ranks up to 16, where the matrix unit's 32 hold a row's parts one after the other; otherwise STEPS
-// times 32 ranks for each part (f16 weights kept as their two parts where registers hold them); JOIN, few rows, one
-// sixteen and one of its adapters.  Except there, a wave walks sixteens of rows, the next one or two on their way
+// times 32 ranks for each part; JOIN, few rows, one sixteen and one of its adapters.  Except there, a wave walks sixteens of rows, the next one or two on their way
 // while one is taken, and loads weights where the adapter changes.
 enum UpForm : int { SHORT = 0, JOIN = -1 };  // else STEPS
+constexpr int up_columns(int YT, bool BF, int FORM) { return FORM == 4 && !BF ? 32 : 64; }  // of a wave
 constexpr int up_occupancy(int YT, bool BF, int FORM) {  // waves a SIMD
-  if (FORM == 4 && !BF) return 1;
-  if (YT == FP8_IO_F32) return FORM <= 0 || (FORM == 1 && BF) ? 3 : 2;
+  if (YT == FP8_IO_F32) return FORM <= 0 || (FORM == 1 && BF) || (FORM == 4 && !BF) ? 3 : 2;
   return FORM == JOIN || (FORM == SHORT && BF) ? 4 : (FORM <= 1 || BF ? 3 : 2);
 }
 template <int YT, bool BF, int FORM>
 __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void adapter_up_kernel(AdapterArgs p, int splits, int run) {
   constexpr int PARTS = YT == FP8_IO_F32 ? 3 : 2, SIZE = YT == FP8_IO_F32 ? 4 : 2;
-  constexpr int PIECES = YT == FP8_IO_F32 ? 4 : 2, COUNT = 16 / SIZE, LANES = COLS / COUNT, STRIDE = 64 / LANES;
+  constexpr int COLS = up_columns(YT, BF, FORM), NJ = COLS / 16, PITCH = COLS + 4;
+  constexpr int COUNT = 16 / SIZE, LANES = COLS / COUNT, STRIDE = 64 / LANES, PIECES = ROWS / STRIDE;
   constexpr int STEPS = FORM > 0 ? FORM : 1;
   constexpr int TURNS = YT == FP8_IO_F32 ? 2 : 1;  // SHORT: of four eights of ranks
-  constexpr int EARLY = FORM == SHORT ? TURNS : (FORM == 1 || FORM == 2 ? FORM * PARTS : 0);  // pieces of h that come with y
-  constexpr bool APART = !BF && FORM >= 0 && FORM < 4;                                        // f16 weights are kept as their parts
+  constexpr int EARLY = FORM == SHORT ? TURNS : (FORM == 1 || FORM == 2 || (NJ == 2 && PARTS == 2) ? FORM * PARTS : 0);  // pieces of h that come with y
+  constexpr bool APART = !BF && FORM >= 0;                                                    // f16 weights are kept as their parts
   constexpr int AHEAD = FORM == SHORT && YT != FP8_IO_F32 ? 2 : 1;                            // sixteens on their way
   __shared__ f4 stage_all[UP_WAVES][ROWS * PITCH / 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
@@ -488,33 +486,33 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
     for (int k = 0; k < PIECES; k++)
       if (row_id(id, k) == -1) store(tile, k, x.y[k]);
   };
-  const auto weights = [&](u4 (&v)[4], int current, int at) {  // of ranks at .. + 7
+  const auto weights = [&](u4 (&v)[NJ], int current, int at) {  // of ranks at .. + 7
     int first = n0 + r;
     asm volatile("" : "+v"(first));  // no address is held from before
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < NJ; j++) {
       const int n = min(first + 16 * j, end - 1);
       v[j] = *(const u4*)((const uint16_t*)p.b + ((size_t)current * p.N + n) * p.R + (at < p.R ? at : 0));
     }
   };
-  const auto apart = [&](const u4 (&f)[4], u4 (&hi)[4], u4 (&low)[4]) {
+  const auto apart = [&](const u4 (&f)[NJ], u4 (&hi)[NJ], u4 (&low)[NJ]) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < NJ; j++) {
       if constexpr (BF) hi[j] = f[j];
       else split8(f[j], hi[j], low[j]);
     }
   };
-  const auto multiply = [&](f4 (&acc)[4], const u4 (&hi)[4], const u4 (&low)[4], const u4& v) {
+  const auto multiply = [&](f4 (&acc)[NJ], const u4 (&hi)[NJ], const u4 (&low)[NJ], const u4& v) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < NJ; j++) {
       acc[j] = mfma<true>(hi[j], v, acc[j]);
       if constexpr (!BF) acc[j] = mfma<true>(low[j], v, acc[j]);
     }
   };
   // y and the products, in the order of memory, and the rows of adapter `current`
-  const auto finish = [&](const f4 (&acc)[4], const Tile& x, int64_t tile, int id, int current) {
+  const auto finish = [&](const f4 (&acc)[NJ], const Tile& x, int64_t tile, int id, int current) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) *(f4*)(stage + r * PITCH + 16 * j + 4 * g) = acc[j];
+    for (int j = 0; j < NJ; j++) *(f4*)(stage + r * PITCH + 16 * j + 4 * g) = acc[j];
     // the wave's own region: its lanes' writes come before its reads, and these before the next writes
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -541,17 +539,17 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
     if (!ad.next()) return;
     const int rank = whole_rank(p, given_rank(p, ad.current));
     const int64_t row = ad.source(0);
-    f4 acc[4];
+    f4 acc[NJ];
 #pragma unroll
-    for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NJ; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int t = 0; 32 * t < p.R; t++) {
       const int at = 32 * t + 8 * g;
-      u4 w[4], v[PARTS], hi[4], low[4];
+      u4 w[NJ], v[PARTS], hi[NJ], low[NJ];
       weights(w, ad.current, at);
       join8<PARTS>((const float*)p.h + (size_t)row * p.S * p.R + s * p.R + (at < p.R ? at : 0), splits, (size_t)p.T * p.S * p.R, v);
 #pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = at < rank ? w[j] : zero;
+      for (int j = 0; j < NJ; j++) w[j] = at < rank ? w[j] : zero;
       apart(w, hi, low);
 #pragma unroll
       for (int k = 0; k < PARTS; k++) multiply(acc, hi, low, at < rank ? v[k] : zero);
@@ -574,7 +572,7 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
       while (tile < stop) {
         const int current = waiting(left);
         int rank = 0;
-        u4 w[STEPS][4], lo[APART ? STEPS : 1][4];
+        u4 w[STEPS][NJ], lo[APART ? STEPS : 1][NJ];
         if (current >= 0) {
 #pragma unroll
           for (int t = 0; t < STEPS; t++) weights(w[t], current, FORM == SHORT ? short_at : 32 * t + 8 * g);
@@ -582,7 +580,7 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
 #pragma unroll
           for (int t = 0; t < STEPS; t++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < NJ; j++) {
               w[t][j] = (FORM == SHORT ? short_at : 32 * t + 8 * g) < rank ? w[t][j] : zero;
               if constexpr (APART) {
                 const u4 f = w[t][j];
@@ -598,9 +596,9 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
           load(later, min(tile + AHEAD, stop - 1));
           if (!in_place && fresh) store_none(now, tile, id);
           if (current >= 0) {
-            f4 acc[4];
+            f4 acc[NJ];
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < NJ; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
             if constexpr (FORM == SHORT) {
 #pragma unroll
               for (int t = 0; t < TURNS; t++)
@@ -609,20 +607,17 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
 #pragma unroll
               for (int t = 0; t < STEPS; t++) {
                 const int at = 32 * t + 8 * g;
-                u4 v[PARTS], hi[4], low[4];
+                u4 v[PARTS];
                 const char* from = (const char*)p.h + 2 * h_index(tile * ROWS, s, 0, 0, p.S, PARTS, p.R);
 #pragma unroll
                 for (int k = 0; k < PARTS; k++)
                   v[k] = EARLY ? now.v[EARLY ? PARTS * t + k : 0]
                                : *(const u4*)(from + (uint32_t)(((at < p.R ? at : 0) + k * p.R) * ROWS + r * 8) * 2);
-                if constexpr (!APART) apart(w[t], hi, low);
 #pragma unroll
                 for (int k = 0; k < PARTS; k++) {
                   const u4 u = at < rank ? v[k] : zero;
-                  if constexpr (APART) multiply(acc, w[t], lo[t], u);
-                  else multiply(acc, hi, low, u);
+                  multiply(acc, w[t], lo[APART ? t : 0], u);
                 }
-                if constexpr (STEPS == 4) __builtin_amdgcn_sched_barrier(0);  // all steps' operands at once are too many
               }
             }
             finish(acc, now, tile, id, current);
@@ -681,7 +676,7 @@ struct Plan {
 Plan plan_of(int T, int K, int SR) {
   Plan q{};
   const int tiles = (SR + ROWS - 1) / ROWS;
-  q.few = T <= 256;
+  q.few = T <= 512;
   q.splits = 1;
   if (q.few) {
     const int steps = (K + FEW_STEP - 1) / FEW_STEP;
@@ -690,8 +685,9 @@ Plan plan_of(int T, int K, int SR) {
     q.ranks = 1;
     return q;
   }
-  q.ranks = tiles <= 4 ? tiles : (tiles % 3 == 0 ? 3 : 4);
-  const int64_t blocks = ((int64_t)T + 4 * ROWS - 1) / (4 * ROWS) * ((tiles + q.ranks - 1) / q.ranks);
+  const int groups = (tiles + 3) / 4;
+  q.ranks = (tiles + groups - 1) / groups;
+  const int64_t blocks = ((int64_t)T + 4 * ROWS - 1) / (4 * ROWS) * groups;
   q.waves = blocks > 512 ? 1 : 2;
   return q;
 }
@@ -725,8 +721,15 @@ hipError_t launch_down_plan(const AdapterArgs& a, const Plan& q, hipStream_t s) 
   return q.waves == 1 ? launch_down_ranks<CODES, BF, 1>(a, q, s) : launch_down_ranks<CODES, BF, 2>(a, q, s);
 }
 
+// Workgroups side by side.
+int up_blocks(const AdapterArgs& a, int columns) {
+  int blocks = 0;
+  for (int i = 0; i < a.S; i++) blocks += (a.cols[i] + UP_WAVES * columns - 1) / (UP_WAVES * columns);
+  return blocks;
+}
 template <int YT, bool BF, int FORM>
-hipError_t launch_up_form(const AdapterArgs& a, int blocks, hipStream_t s) {
+hipError_t launch_up_form(const AdapterArgs& a, hipStream_t s) {
+  const int blocks = up_blocks(a, up_columns(YT, BF, FORM));
   const int64_t sixteens = ((int64_t)a.T + ROWS - 1) / ROWS;
   // sixteens of rows of a workgroup, so that all workgroups have a place at once
   const int64_t places = 256 * up_occupancy(YT, BF, FORM);
@@ -736,28 +739,26 @@ hipError_t launch_up_form(const AdapterArgs& a, int blocks, hipStream_t s) {
   return hipGetLastError();
 }
 template <int YT, bool BF>
-hipError_t launch_up(const AdapterArgs& a, const Plan& q, int blocks, hipStream_t s) {
+hipError_t launch_up(const AdapterArgs& a, const Plan& q, hipStream_t s) {
   if (q.few) {
-    const dim3 grid((unsigned)blocks, (unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)std::min(ROWS, a.T));
+    const dim3 grid((unsigned)up_blocks(a, up_columns(YT, BF, JOIN)), (unsigned)((a.T + ROWS - 1) / ROWS), (unsigned)std::min(ROWS, a.T));
     T5K_LAUNCH((adapter_up_kernel<YT, BF, JOIN>), grid, dim3(64 * UP_WAVES), 0, s, a, q.splits, 1);
     return hipGetLastError();
   }
-  if (a.R <= 16) return launch_up_form<YT, BF, SHORT>(a, blocks, s);
-  if (a.R <= 32) return launch_up_form<YT, BF, 1>(a, blocks, s);
-  if (a.R <= 64) return launch_up_form<YT, BF, 2>(a, blocks, s);
-  return launch_up_form<YT, BF, 4>(a, blocks, s);
+  if (a.R <= 16) return launch_up_form<YT, BF, SHORT>(a, s);
+  if (a.R <= 32) return launch_up_form<YT, BF, 1>(a, s);
+  if (a.R <= 64) return launch_up_form<YT, BF, 2>(a, s);
+  return launch_up_form<YT, BF, 4>(a, s);
 }
 template <bool BF>
 hipError_t launch(const AdapterArgs& a, hipStream_t s) {
-  int blocks = 0;
-  for (int i = 0; i < a.S; i++) blocks += (a.cols[i] + UP_WAVES * COLS - 1) / (UP_WAVES * COLS);
   const Plan q = plan_of(a.T, a.K, a.S * a.R);
   const hipError_t e = a.x_type == ADAPTER_E4M3 ? launch_down_plan<true, BF>(a, q, s) : launch_down_plan<false, BF>(a, q, s);
   if (e != hipSuccess) return e;
   switch (a.y_type) {
-    case FP8_IO_F32: return launch_up<FP8_IO_F32, BF>(a, q, blocks, s);
-    case FP8_IO_F16: return launch_up<FP8_IO_F16, BF>(a, q, blocks, s);
-    case FP8_IO_BF16: return launch_up<FP8_IO_BF16, BF>(a, q, blocks, s);
+    case FP8_IO_F32: return launch_up<FP8_IO_F32, BF>(a, q, s);
+    case FP8_IO_F16: return launch_up<FP8_IO_F16, BF>(a, q, s);
+    case FP8_IO_BF16: return launch_up<FP8_IO_BF16, BF>(a, q, s);
   }
   return hipErrorInvalidValue;
 }
