@@ -339,9 +339,9 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
  * to requests of which each has an adapter of its own, or none; the shared product y = x W^T (t5h_fp8_matmul
  * or any other) is the same for all, and these calls add what the adapters say, for all of them at once:
  *   out[t][n] = y[t][n] + scale_g sum_r (sum_k x[t][k] A_g[s R + r][k]) B_g[n][r],    g = ids[t]
- * ids[t] outside 0 .. G - 1 (-1, say): the row has no adapter, out[t] is y[t], bit for bit.  Rows of one adapter are fastest
- * where they follow each other.  Columns come in `slices` (1 .. 4, as q, k and v of a fused projection), each
- * with its own A: column n of slice s takes ranks s R .. s R + R - 1 of A.
+ * ids[t] outside 0 .. G - 1 (-1, say): the row has no adapter, out[t] is y[t], bit for bit.  Rows of one
+ * adapter are fastest where they follow each other.  Columns come in `slices` (1 .. 4, as q, k and v of a fused
+ * projection), each with its own A: column n of slice s takes ranks s R .. s R + R - 1 of A.
  *   x: [T] rows of K values, ldx from row to row, of the adapters' type, or e4m3 codes (T5H_TYPE_E4M3) with
  *      scales as t5h_fp8_quantize and t5h_fp8_rmsnorm write them (what the shared product takes).
  *   a: [G][slices][R][K], b: [G][N][R], f16 or bf16, N = the sum of cols[slices] (a HOST array).
@@ -350,15 +350,16 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
  *   scales: [G] f32, or NULL (all 1).
  *   y, out: [T] rows of N values in f32, f16 or bf16; out may be y itself with its row length, or share no
  *      byte with it.  Rows without an adapter are then not touched.
- * Sums are f32, and so is the inner product, which goes to the matrix units in two or three 16-bit parts
- * (within 2^-17 of it for bf16 adapters under 16-bit results, 2^-22 otherwise); results are rounded once.
+ * Sums are f32, and so is the inner product, which goes to the matrix units in bf16 parts: three, which hold all
+ * of it, where y is f32, and otherwise two (within 2^-16 of it).  Results are rounded once.
  * Adapters are finite; an infinity or NaN in a row stays in that row.
  * K is a multiple of 16 up to 2^21, R one of 8 up to 128, columns of a slice one of 16 up to 2^24; T up to
- * 2^30 (codes: their scales below 2^31 bytes), G up to 2^24.  Rows of x, y and out start on multiples of 16 bytes and are up to 2^24 values apart; a,
- * b, the scales of codes and the workspace start on 16 bytes.  Device buffers lie on the current device; the call is enqueued on `stream`
- * (a hipStream_t; NULL = the default stream) and returns without waiting.  It allocates nothing and keeps no
+ * 2^30 (codes: their scales below 2^31 bytes), G up to 2^24.  Rows of x, y and out start on multiples of 16 bytes
+ * and are up to 2^24 values apart; a, b, the scales of codes and the workspace start on 16 bytes.  Device buffers
+ * lie on the current device; the call is enqueued on `stream` (a hipStream_t; NULL = the default stream) and returns
+ * without waiting.  It allocates nothing and keeps no
  * state: intermediate sums live in d_work, of at least t5h_adapter_workspace's bytes, which serves one call
- * (or replay of a graph that holds one) at a time. */
+ * (or replay of a graph that holds one) at a time.  A workspace for T rows serves fewer rows too. */
 #define T5H_TYPE_E4M3 3
 int t5h_adapter_workspace(int32_t T, int32_t K, int32_t slices, int32_t R, size_t* bytes);
 int t5h_adapter_add_device(const void* d_x, int32_t x_type, const uint8_t* d_x_scales, int64_t ldx, int32_t T, int32_t K,

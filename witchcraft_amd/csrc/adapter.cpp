@@ -64,7 +64,7 @@ extern "C" {
 int t5h_adapter_workspace(int32_t T, int32_t K, int32_t slices, int32_t R, size_t* bytes) {
   TRY(check_inner(T, K, slices, R));
   if (!bytes) return bad("NULL bytes");
-  *bytes = t5k::adapter_work_bytes(T, K, slices * R);
+  *bytes = t5k::adapter_work_bytes(T, K, slices, R);
   return T5H_OK;
 }
 
@@ -92,7 +92,7 @@ int t5h_adapter_add_device(const void* d_x, int32_t x_type, const uint8_t* d_x_s
   if (d_ranks) TRY(check_buffer(d_ranks, "ranks", 4));
   if (d_scales) TRY(check_buffer(d_scales, "scales", 4));
   TRY(check_buffer(d_work, "workspace", 16));
-  if (work_bytes < t5k::adapter_work_bytes(T, K, slices * R)) return bad("the workspace is smaller than t5h_adapter_workspace says");
+  if (work_bytes < t5k::adapter_work_bytes(T, K, slices, R)) return bad("the workspace is smaller than t5h_adapter_workspace says");
   t5k::AdapterArgs p{};
   p.x = d_x, p.x_scales = d_x_scales, p.ldx = ldx, p.x_type = x_type, p.T = T, p.K = K;
   p.ids = d_ids, p.G = G, p.a = d_a, p.b = d_b, p.w_type = w_type, p.ranks = d_ranks, p.scales = d_scales;
@@ -115,7 +115,7 @@ int t5h_adapter_add(int32_t hip_device, const void* x, int32_t x_type, const uin
   HostCall d;
   const size_t xb = (size_t)T * K * x_bytes(x_type), yb = (size_t)T * N * type_bytes(y_type);
   const size_t sb = x_type == T5H_TYPE_E4M3 ? ((size_t)K + t5k::FP8_BLOCK - 1) / t5k::FP8_BLOCK * t5k::fp8_scale_rows(T) : 0;
-  const size_t ab = (size_t)G * slices * R * K * 2, bb = (size_t)G * N * R * 2, wb = t5k::adapter_work_bytes(T, K, slices * R);
+  const size_t ab = (size_t)G * slices * R * K * 2, bb = (size_t)G * N * R * 2, wb = t5k::adapter_work_bytes(T, K, slices, R);
   const size_t dx = d.part(xb), ds = d.part(sb), di = d.part((size_t)T * 4), da = d.part(ab), db = d.part(bb);
   const size_t dr = d.part((size_t)G * 4), df = d.part((size_t)G * 4), dy = d.part(yb), dw = d.part(wb);
   TRY(d.open(hip_device));

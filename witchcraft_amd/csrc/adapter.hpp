@@ -27,6 +27,6 @@ struct AdapterArgs {
   int y_type;
   void* h;  // bf16 parts in operand order, or for few rows f32 [splits][T][S R]: the kernels' own
 };
-size_t adapter_work_bytes(int T, int K, int SR);
+size_t adapter_work_bytes(int T, int K, int S, int R);
 hipError_t launch_adapter(const AdapterArgs& a, hipStream_t s);
 }  // namespace t5k

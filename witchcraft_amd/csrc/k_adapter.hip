@@ -12,7 +12,7 @@
 //
 // h is f32 and stays so: it is stored as a sum of bf16 parts, all of which multiply the same weights in the second
 // product, as if there were so many times the ranks.  Three parts hold all 24 bits (results in f32), two the upper 16
-// (within 2^-17 of h, where the results' own rounding is 2^-9 or 2^-12).  bf16 has f32's range, which f16 has not; f16
+// (within 2^-16 of h, where the results' own rounding is 2^-8 or 2^-11).  bf16 has f32's range, which f16 has not; f16
 // weights go in as two bf16 parts, which hold their 11 bits.
 #include "adapter.hpp"
 
@@ -198,98 +198,104 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(Adapte
   *(f4*)((float*)p.h + ((size_t)split * p.T + row0 + r) * SR + j) = acc;
 }
 
-// ---- h = scale x A^T, many rows: 64 rows x 16 RT ranks per workgroup --------------------------------
-// Steps of 128 bytes of x's rows (64 values, or 128 codes) through a ring of STAGES in LDS: copies in whole rows, eight
-// of 128 bytes to an instruction, straight from memory.  A row's eight 16-byte chunks are stored rotated (xor) by its
-// number, so that eight rows' same chunk, which a read takes at a time, lie in different banks.  Four waves of sixteen
-// rows each read x once and A between them; with KG = 2 four more take every other step, and the sums meet in LDS.
-// A wait and a barrier per step: stage n has been requested STAGES - 1 steps ahead.  Chunks past K, and steps past
-// the last, are copied from outside the descriptors' range, as zeros.
-template <bool CODES, int RT, int KG>
+// ---- h = scale x A^T, many rows: 16 RG rows x 16 RT ranks per workgroup ------------------------------
+// Steps of 128 bytes of x's rows (64 values, or 128 codes) go through a ring of STAGES in LDS: copies in whole rows,
+// eight of 128 bytes to an instruction, straight from memory.  A row's eight 16-byte chunks are stored rotated (xor) by
+// its number, so that eight rows' same chunk, which a read takes at a time, lie in different banks.  Four waves: RG
+// sixteens of rows, the ranks in 4 / RG parts.  A wait and a barrier per step: step n has been requested STAGES - 1 ahead.
+// Chunks past K, and steps past the last, are copied from outside the descriptors' range, as zeros.  Bound by the way
+// through LDS and the wait for a step where rows are few (4,616 of 768: 8.7 us), by memory where they are many
+// (16,391 of 4,096 against 64 ranks: 51 us, 2.6 TB/s; 74,640 of 768 codes: 39).
+template <bool CODES, int RT, int RG>
 struct Ring {
-  static constexpr int ROW_BYTES = 4 * ROWS * 128, HALVES = CODES ? 2 : 1;  // of x; pieces of 128 bytes of A's rows
-  static constexpr int A_BYTES = HALVES * RT * ROWS * 128, A_COPIES = A_BYTES / 1024;  // copies of four waves
+  static constexpr int ROW_COPIES = RG / 2, HALVES = CODES ? 2 : 1;  // of a wave; pieces of 128 bytes of A's rows
+  static constexpr int ROW_BYTES = RG * ROWS * 128, A_BYTES = HALVES * RT * ROWS * 128, A_COPIES = A_BYTES / 1024;  // of four waves
   // behind them the scales of codes, one copy a wave, or room for the copies of waves that have none of A's
   static constexpr int REST = CODES ? 4 * 256 : (A_COPIES % 4 ? 1024 : 0);
   static constexpr int STAGE = ROW_BYTES + A_BYTES + REST;
-  static constexpr int STAGES = KG * STAGE <= 16384 ? 3 : 2;               // two workgroups on a compute unit
-  static constexpr int COPIES = 2 + (A_COPIES + 3) / 4 + (CODES ? 1 : 0);  // of a wave, the same for all
+  // three where they leave room for two workgroups on a compute unit and more: 4,096 rows of 64 ranks 66 us, with two
+  // stages 86; larger ones take 145 us with three, 122 with two (three slices' codes)
+  static constexpr int STAGES = STAGE <= 16384 ? 3 : 2;
+  static constexpr int COPIES = ROW_COPIES + (A_COPIES + 3) / 4 + (CODES ? 1 : 0);  // of a wave, the same for all
 };
-template <bool CODES, bool BF, int RT, int KG>
-__global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p, int parts) {
-  typedef Ring<CODES, RT, KG> Lds;
-  __shared__ __attribute__((aligned(1024))) char lds[KG * Lds::STAGES * Lds::STAGE];  // the sums: [4][RT][64] f4, no more
-  constexpr int SIZE = CODES ? 1 : 2, K_STEP = 128 / SIZE, STAGES = Lds::STAGES;
+template <bool CODES, bool BF, int RT, int RG>
+__global__ __launch_bounds__(256, 2) void adapter_down_kernel(AdapterArgs p, int parts) {
+  typedef Ring<CODES, RT, RG> Lds;
+  __shared__ __attribute__((aligned(1024))) char lds[Lds::STAGES * Lds::STAGE];
+  constexpr int SIZE = CODES ? 1 : 2, K_STEP = 128 / SIZE, STAGES = Lds::STAGES, RQ = RT * RG / 4;  // RQ: sixteens of ranks of a wave
+  static_assert(RG == 4 || (RG == 2 && RT % 2 == 0), "whole sixteens of ranks for each wave");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int rw = wave & 3, kg = wave >> 2;
-  const int SR = p.S * p.R, steps = (p.K + K_STEP - 1) / K_STEP, turns = (steps + KG - 1) / KG, group = (int)blockIdx.y;
+  const int rw = wave % RG, q0 = wave / RG * RQ;
+  const int SR = p.S * p.R, steps = (p.K + K_STEP - 1) / K_STEP, group = (int)blockIdx.y;
   const size_t m16 = fp8_scale_rows(p.T);
-  const int64_t tiles = ((int64_t)p.T + 4 * ROWS - 1) / (4 * ROWS);
-  const uint32_t lds0 = lds_offset(lds) + (uint32_t)(kg * STAGES * Lds::STAGE);
-  char* mine = lds + kg * STAGES * Lds::STAGE;
+  const int64_t tiles = ((int64_t)p.T + RG * ROWS - 1) / (RG * ROWS);
+  const uint32_t lds0 = lds_offset(lds);
   const int cr = lane >> 3, cc = (lane & 7) ^ cr;  // the row of eight and the chunk that the lane copies
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t row0 = tile * 4 * ROWS;
-    const int rows = (int)min((int64_t)4 * ROWS, p.T - row0);
-    Adapters<4> ad(p, row0);
+    const int64_t row0 = tile * RG * ROWS;
+    const int rows = (int)min((int64_t)RG * ROWS, p.T - row0);
+    Adapters<RG> ad(p, row0);
     for (unsigned seen = 0; ad.next(); seen++) {
       if (seen % gridDim.z != blockIdx.z) continue;
       const float scale = p.scales ? p.scales[ad.current] : 1.f;
       const int given = given_rank(p, ad.current);
-      const int id = rw == 0 ? ad.id[0] : (rw == 1 ? ad.id[1] : (rw == 2 ? ad.id[2] : ad.id[3]));
+      const int id0 = ad.id[0], id1 = ad.id[1], id2 = ad.id[RG - 2], id3 = ad.id[RG - 1];
+      const auto id_of = [&](int i) { return i == 0 ? id0 : (i == 1 ? id1 : (i == 2 ? id2 : id3)); };  // of the i-th sixteen
+      const int id = id_of(rw);
       const int64_t row = row0 + ROWS * rw + r;
-      // This wave's copies: rows 16 rw + 8 i + cr of x (in the place of those whose result nothing keeps, one that is
-      // copied anyway), and pieces i + rw of A: eight ranks, codes: of one half of a step.  A wave without one copies zeros
+      // This wave's copies: eights of rows of x (in the place of those whose result nothing keeps, one that is
+      // copied anyway), and pieces 4 i + wave of A: eight ranks, codes: of one half of a step.  A wave without one copies zeros
       // behind the last.
       const i4v x_at = buffer_at((const char*)p.x + row0 * p.ldx * SIZE, (uint32_t)((rows - 1) * p.ldx + p.K) * SIZE);
       const int j0 = ROWS * RT * group, ranks = min(ROWS * RT, SR - j0);
       const i4v a_at = buffer_at((const uint16_t*)p.a + ((size_t)ad.current * SR + j0) * p.K, (uint32_t)ranks * p.K * 2);
       const i4v s_at = buffer_at(CODES ? (const void*)p.x_scales : p.x, CODES ? (uint32_t)(steps * m16) : 0u);
-      uint32_t x_off[2], a_off[(Lds::A_COPIES + 3) / 4];
+      uint32_t x_off[Lds::ROW_COPIES], a_off[(Lds::A_COPIES + 3) / 4];
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int other = __builtin_amdgcn_ds_bpermute(4 * (8 * i + cr), id);
-        const int from = other == ad.current ? ROWS * rw + 8 * i + cr : (int)(ad.row - row0);
+      for (int i = 0; i < Lds::ROW_COPIES; i++) {
+        const int eight = Lds::ROW_COPIES * wave + i, at = 8 * eight + cr;
+        const int other = __builtin_amdgcn_ds_bpermute(4 * (at % ROWS), id_of(eight / 2));
+        const int from = other == ad.current ? at : (int)(ad.row - row0);
         x_off[i] = (uint32_t)(from * p.ldx * SIZE) + 16 * cc;
       }
 #pragma unroll
       for (int i = 0; i < (Lds::A_COPIES + 3) / 4; i++) {
-        const int c = 4 * i + rw, half = c / (2 * RT), j = c % (2 * RT) * 8 + cr;
+        const int c = 4 * i + wave, half = c / (2 * RT), j = c % (2 * RT) * 8 + cr;
         a_off[i] = c < Lds::A_COPIES && j < ranks ? (uint32_t)(j * p.K + 64 * half + 8 * cc) * 2 : kOutside;
       }
-      const uint32_t s_off = lane < 4 ? (uint32_t)(row0 + ROWS * rw + 4 * lane) : kOutside;
+      const uint32_t s_off = lane < 4 ? (uint32_t)(row0 + ROWS * wave + 4 * lane) : kOutside;
       // Workgroups begin at different steps: with all at the same one the 32 compute units of an XCD, whose workgroups are
-      // every eighth, want the same few lines of A at a time.
+      // every eighth, want the same few lines of A at a time (16,391 rows of 4,096: 169 us for both products, 165 so).
       const int shift = (int)((tile / 8) % steps);
-      const auto copy = [&](int turn) {
-        const int at = turn * KG + kg, n = at + shift - (at + shift >= steps ? steps : 0);
-        const uint32_t stage = lds0 + (uint32_t)(turn % STAGES) * Lds::STAGE;
+      const auto copy = [&](int at) {
+        const int n = at + shift - (at + shift >= steps ? steps : 0);
+        const uint32_t stage = lds0 + (uint32_t)(at % STAGES) * Lds::STAGE;
         const int left = at < steps ? p.K - n * K_STEP : 0;  // values of this step
         const uint32_t soff = (uint32_t)n * 128;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-          lds_copy16(x_at, cc * (16 / SIZE) < left ? x_off[i] : kOutside, soff, stage + (2 * rw + i) * 1024);
+        for (int i = 0; i < Lds::ROW_COPIES; i++)
+          lds_copy16(x_at, cc * (16 / SIZE) < left ? x_off[i] : kOutside, soff, stage + (Lds::ROW_COPIES * wave + i) * 1024);
 #pragma unroll
         for (int i = 0; i < (Lds::A_COPIES + 3) / 4; i++) {
-          const int c = 4 * i + rw, half = c / (2 * RT);
+          const int c = 4 * i + wave, half = c / (2 * RT);
           lds_copy16(a_at, 64 * half + 8 * cc < left ? a_off[i] : kOutside, soff * Lds::HALVES,
                      stage + Lds::ROW_BYTES + min(c, (int)Lds::A_COPIES) * 1024);
         }
-        if constexpr (CODES) lds_copy4(s_at, left > 0 ? s_off : kOutside, (uint32_t)(n * m16), stage + Lds::ROW_BYTES + Lds::A_BYTES + rw * 256);
+        if constexpr (CODES) lds_copy4(s_at, left > 0 ? s_off : kOutside, (uint32_t)(n * m16), stage + Lds::ROW_BYTES + Lds::A_BYTES + wave * 256);
       };
-      f4 acc[RT];
+      f4 acc[RQ];
 #pragma unroll
-      for (int q = 0; q < RT; q++) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int q = 0; q < RQ; q++) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < STAGES - 1; i++) copy(i);
 #pragma unroll 1
-      for (int turn = 0; turn < turns; turn++) {
-        // this turn's stage is whole, and the last one's has been read by all
+      for (int n = 0; n < steps; n++) {
+        // this step's stage is whole, and the last one's has been read by all
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * Lds::COPIES) : "memory");
-        copy(turn + STAGES - 1);
-        const char* stage = mine + turn % STAGES * Lds::STAGE;
+        copy(n + STAGES - 1);
+        const char* stage = lds + n % STAGES * Lds::STAGE;
         const char* xs = stage + (ROWS * rw + r) * 128;
-        const char* as = stage + Lds::ROW_BYTES + r * 128;
+        const char* as = stage + Lds::ROW_BYTES + (ROWS * q0 + r) * 128;
         u4 x[CODES ? 4 : 2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -299,7 +305,7 @@ __global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p
         }
         const float f = CODES ? e8m0_value((uint8_t)stage[Lds::ROW_BYTES + Lds::A_BYTES + rw * 256 + r]) : 1.f;
 #pragma unroll
-        for (int q = 0; q < RT; q++) {
+        for (int q = 0; q < RQ; q++) {
           f4 t = CODES ? f4{0.f, 0.f, 0.f, 0.f} : acc[q];
 #pragma unroll
           for (int e = 0; e < (CODES ? 4 : 2); e++) {
@@ -316,23 +322,15 @@ __global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p
         }
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the ring is free
-      if constexpr (KG > 1) {
-        if (kg > 0) {
-#pragma unroll
-          for (int q = 0; q < RT; q++) ((f4*)lds)[(rw * RT + q) * 64 + lane] = acc[q];
-        }
-        __syncthreads();
-      }
       const int rank = whole_rank(p, given);
       int gg = g;
       asm volatile("" : "+v"(gg));           // the addresses of results are left to be computed here
-      if (id == ad.current && kg == 0) {  // -1 behind the last row
+      if (id == ad.current) {  // -1 behind the last row
 #pragma unroll
-        for (int q = 0; q < RT; q++) {
-          const int j = j0 + ROWS * q + 4 * gg;
+        for (int q = 0; q < RQ; q++) {
+          const int j = j0 + ROWS * (q0 + q) + 4 * gg;
           if (j >= SR) continue;
-          f4 v = acc[q];
-          if constexpr (KG > 1) v += ((f4*)lds)[(rw * RT + q) * 64 + lane];
+          const f4 v = acc[q];
           const int slice = j / p.R, at_rank = j - slice * p.R;
           float rest[4];  // values past the adapter's rank may come from anything
 #pragma unroll
@@ -346,12 +344,11 @@ __global__ __launch_bounds__(256 * KG, 2) void adapter_down_kernel(AdapterArgs p
           }
         }
       }
-      if constexpr (KG > 1) __syncthreads();  // the sums are read
     }
   }
 }
 
-// ---- out = y + h B^T: 16 rows x 64 columns (32 for ranks past 64) of one slice per wave and turn, four waves side by side --
+// ---- out = y + h B^T: 16 rows x 64 columns of one slice per wave and turn, four waves side by side --------
 // A wave loads and stores y in whole rows, eight of 128 bytes or four of 256 to an instruction, lane after lane: with
 // lanes in the matrix units' order, sixteen rows in turn, the address unit takes four times as long.  The products
 // therefore change lanes, through LDS: rows of f32, 16 bytes apart in their banks.
@@ -410,12 +407,15 @@ __device__ __forceinline__ void join8(const float* from, int splits, size_t stri
 }
 
 // Three forms: SHORT, ranks up to 16, where the matrix unit's 32 hold a row's parts one after the other; otherwise STEPS
-// times 32 ranks for each part; JOIN, few rows, one sixteen and one of its adapters.  Except there, a wave walks sixteens of rows, the next one or two on their way
-// while one is taken, and loads weights where the adapter changes.
+// times 32 ranks for each part; JOIN, few rows, one sixteen and one of its adapters.  Except there, a wave walks sixteens
+// of rows, the next one on its way while one is taken (two gain nothing), and loads weights where the adapter changes.
+// Bound by the reads and writes of y: 74,640 rows of 2,304 columns
+// 152 us (4.5 TB/s), 16,391 of 8,192 121 us (4.4 TB/s); 4,616 rows 15.3 us (2.8 TB/s), of which launch and ends are 5.
 enum UpForm : int { SHORT = 0, JOIN = -1 };  // else STEPS
-constexpr int up_columns(int YT, bool BF, int FORM) { return FORM == 4 && !BF ? 32 : 64; }  // of a wave
+// 64 columns are a whole line of y; f32 results from f16 weights of more than 64 ranks have registers for 32
+constexpr int up_columns(int YT, bool BF, int FORM) { return FORM == 4 && !BF && YT == FP8_IO_F32 ? 32 : 64; }  // of a wave
 constexpr int up_occupancy(int YT, bool BF, int FORM) {  // waves a SIMD
-  if (YT == FP8_IO_F32) return FORM <= 0 || (FORM == 1 && BF) || (FORM == 4 && !BF) ? 3 : 2;
+  if (YT == FP8_IO_F32) return FORM <= 0 || (FORM == 1 && BF) || up_columns(YT, BF, FORM) == 32 ? 3 : 2;
   return FORM == JOIN || (FORM == SHORT && BF) ? 4 : (FORM <= 1 || BF ? 3 : 2);
 }
 template <int YT, bool BF, int FORM>
@@ -425,9 +425,8 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
   constexpr int COUNT = 16 / SIZE, LANES = COLS / COUNT, STRIDE = 64 / LANES, PIECES = ROWS / STRIDE;
   constexpr int STEPS = FORM > 0 ? FORM : 1;
   constexpr int TURNS = YT == FP8_IO_F32 ? 2 : 1;  // SHORT: of four eights of ranks
-  constexpr int EARLY = FORM == SHORT ? TURNS : (FORM == 1 || FORM == 2 || (NJ == 2 && PARTS == 2) ? FORM * PARTS : 0);  // pieces of h that come with y
-  constexpr bool APART = !BF && FORM >= 0;                                                    // f16 weights are kept as their parts
-  constexpr int AHEAD = FORM == SHORT && YT != FP8_IO_F32 ? 2 : 1;                            // sixteens on their way
+  constexpr int EARLY = FORM == SHORT ? TURNS : (FORM == 1 || FORM == 2 ? FORM * PARTS : 0);  // pieces of h that come with y
+  constexpr bool APART = !BF && FORM >= 0;  // f16 weights are kept as their parts
   __shared__ f4 stage_all[UP_WAVES][ROWS * PITCH / 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   float* stage = (float*)stage_all[wave];
@@ -563,11 +562,10 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
         const uint64_t m = __ballot(id >= 0);
         return m ? __builtin_amdgcn_readlane(id, __builtin_ctzll(m)) : -1;
       };
-      Tile x, x1, x2;
+      Tile x, x1;
       int64_t tile = first;
       int id = id_of(tile), left = id, next_id = id_of(min(tile + 1, stop - 1));  // left: of rows not yet taken
       load(x, tile);
-      if constexpr (AHEAD == 2) load(x1, min(tile + 1, stop - 1));
       bool fresh = true;  // rows without an adapter are yet to come
       while (tile < stop) {
         const int current = waiting(left);
@@ -593,7 +591,7 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
         bool same = false;
         const auto take = [&](const Tile& now, Tile& later) {
           const int later_id = id_of(min(tile + 2, stop - 1));
-          load(later, min(tile + AHEAD, stop - 1));
+          load(later, min(tile + 1, stop - 1));
           if (!in_place && fresh) store_none(now, tile, id);
           if (current >= 0) {
             f4 acc[NJ];
@@ -636,29 +634,13 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
         };
         // the sixteens' registers take turns: moved from one to the next, they would have to have arrived
         while (true) {
-          if constexpr (AHEAD == 2) {
-            if (!take(x, x2)) {
-              if (!same) x = x1, x1 = x2;
-              break;
-            }
-            if (!take(x1, x)) {
-              if (same) x = x1, x1 = x2;
-              else x1 = x, x = x2;
-              break;
-            }
-            if (!take(x2, x1)) {
-              if (same) x1 = x, x = x2;
-              break;
-            }
-          } else {
-            if (!take(x, x1)) {
-              if (!same) x = x1;
-              break;
-            }
-            if (!take(x1, x)) {
-              if (same) x = x1;
-              break;
-            }
+          if (!take(x, x1)) {
+            if (!same) x = x1;
+            break;
+          }
+          if (!take(x1, x)) {
+            if (same) x = x1;
+            break;
           }
         }
       }
@@ -670,13 +652,19 @@ __global__ __launch_bounds__(64 * UP_WAVES, up_occupancy(YT, BF, FORM)) void ada
 struct Plan {
   bool few;     // rows: one of a sixteen's adapters to a workgroup, K split over workgroups
   int splits;   // their parts of K
-  int waves;    // of a workgroup, on parts of K: few rows; times four otherwise
+  int waves;    // few rows: of a workgroup, on parts of K
+  int sixteens; // many rows: of a workgroup
   int ranks;    // sixteens of ranks of a workgroup
 };
-Plan plan_of(int T, int K, int SR) {
+// The few rows' form reads A once for each sixteen of rows and adapter, and its second product splits h for each 64
+// columns, so it is taken for fewer rows where ranks are many: 512 rows of rank 16 take 11.9 us in it (16 requests, three
+// slices; 46.5 with 64 adapters mixed) and 12.6 (77) in the other, 700 rows 15.9 and 13.9; of rank 64 256 rows take 30.5
+// and 28.7 (8,192 columns) or 15.4 and 21.9 (768), 512 rows 50.8 and 30.8 or 22.0 and 22.7.
+int few_rows(int R) { return std::min(512, 24576 / R); }
+Plan plan_of(int T, int K, int S, int R) {
   Plan q{};
-  const int tiles = (SR + ROWS - 1) / ROWS;
-  q.few = T <= 512;
+  const int SR = S * R, tiles = (SR + ROWS - 1) / ROWS;
+  q.few = T <= few_rows(R);
   q.splits = 1;
   if (q.few) {
     const int steps = (K + FEW_STEP - 1) / FEW_STEP;
@@ -685,30 +673,28 @@ Plan plan_of(int T, int K, int SR) {
     q.ranks = 1;
     return q;
   }
+  // Up to 64 ranks to a workgroup.  With 128 bf16 adapters of rank 128 take 1% less (16,391 rows), codes 70% more.
   const int groups = (tiles + 3) / 4;
   q.ranks = (tiles + groups - 1) / groups;
   const int64_t blocks = ((int64_t)T + 4 * ROWS - 1) / (4 * ROWS) * groups;
-  q.waves = blocks > 512 ? 1 : 2;
+  // Halves of tiles while those are fewer than compute units, which read A twice as often but LDS less: 4,616 rows of
+  // 2,048 against 64 ranks 29.0 us (both products), in whole tiles 31.1; past that it is the same or less (18,464 rows: 63.9 and 61.7).
+  q.sixteens = q.ranks > 1 && blocks <= 256 ? 2 : 4;
+  if (q.sixteens == 2) q.ranks = (q.ranks + 1) & ~1;
   return q;
 }
 
-template <bool CODES, bool BF, int RT, int KG>
+template <bool CODES, bool BF, int RT, int RG>
 hipError_t launch_down(const AdapterArgs& a, hipStream_t s) {
   const int tiles = (a.S * a.R + ROWS - 1) / ROWS, groups = (tiles + RT - 1) / RT;
-  const int64_t rows = ((int64_t)a.T + 4 * ROWS - 1) / (4 * ROWS);
-  // a tile with the rows of several short requests would take as many turns: workgroups share them while there is room
-  const dim3 grid((unsigned)std::min<int64_t>(rows, 1 << 20), (unsigned)groups, rows * groups < 768 ? 4 : 1);
-  T5K_LAUNCH((adapter_down_kernel<CODES, BF, RT, KG>), grid, dim3(256 * KG), 0, s, a, a.y_type == FP8_IO_F32 ? 3 : 2);
+  const int64_t rows = ((int64_t)a.T + RG * ROWS - 1) / (RG * ROWS);
+  // A tile with the rows of several short requests takes as many turns; up to 16 workgroups share them while the grid
+  // stays within 2,048: 1,000 rows of 64 adapters, mixed, take 83 us so and 193 with 4, 4,616 rows of 32 requests 23.5 and
+  // 32 with one to a tile.  Past that the ones without a turn cost more: 9,232 rows 37.2 us, with twice as many 40.5.
+  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(ROWS, 2048 / (rows * groups)));
+  const dim3 grid((unsigned)std::min<int64_t>(rows, 1 << 20), (unsigned)groups, (unsigned)share);
+  T5K_LAUNCH((adapter_down_kernel<CODES, BF, RT, RG>), grid, dim3(256), 0, s, a, a.y_type == FP8_IO_F32 ? 3 : 2);
   return hipGetLastError();
-}
-template <bool CODES, bool BF, int KG>
-hipError_t launch_down_ranks(const AdapterArgs& a, const Plan& q, hipStream_t s) {
-  switch (q.ranks) {
-    case 1: return launch_down<CODES, BF, 1, KG>(a, s);
-    case 2: return launch_down<CODES, BF, 2, KG>(a, s);
-    case 3: return launch_down<CODES, BF, 3, KG>(a, s);
-  }
-  return launch_down<CODES, BF, 4, KG>(a, s);
 }
 template <bool CODES, bool BF>
 hipError_t launch_down_plan(const AdapterArgs& a, const Plan& q, hipStream_t s) {
@@ -718,7 +704,13 @@ hipError_t launch_down_plan(const AdapterArgs& a, const Plan& q, hipStream_t s) 
     T5K_LAUNCH((adapter_down_few_kernel<CODES, BF>), grid, dim3(64 * q.waves), 0, s, a, q.splits);
     return hipGetLastError();
   }
-  return q.waves == 1 ? launch_down_ranks<CODES, BF, 1>(a, q, s) : launch_down_ranks<CODES, BF, 2>(a, q, s);
+  if (q.sixteens == 2) return q.ranks == 2 ? launch_down<CODES, BF, 2, 2>(a, s) : launch_down<CODES, BF, 4, 2>(a, s);
+  switch (q.ranks) {
+    case 1: return launch_down<CODES, BF, 1, 4>(a, s);
+    case 2: return launch_down<CODES, BF, 2, 4>(a, s);
+    case 3: return launch_down<CODES, BF, 3, 4>(a, s);
+  }
+  return launch_down<CODES, BF, 4, 4>(a, s);
 }
 
 // Workgroups side by side.
@@ -731,7 +723,8 @@ template <int YT, bool BF, int FORM>
 hipError_t launch_up_form(const AdapterArgs& a, hipStream_t s) {
   const int blocks = up_blocks(a, up_columns(YT, BF, FORM));
   const int64_t sixteens = ((int64_t)a.T + ROWS - 1) / ROWS;
-  // sixteens of rows of a workgroup, so that all workgroups have a place at once
+  // sixteens of rows of a workgroup, so that all workgroups have a place at once: 16,391 rows of 8,192 columns 165 us, with
+  // one each 297
   const int64_t places = 256 * up_occupancy(YT, BF, FORM);
   const int run = (int)std::max<int64_t>(1, std::min<int64_t>(64, (sixteens * blocks + places - 1) / places));
   const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>((sixteens + run - 1) / run, 65535));
@@ -752,7 +745,7 @@ hipError_t launch_up(const AdapterArgs& a, const Plan& q, hipStream_t s) {
 }
 template <bool BF>
 hipError_t launch(const AdapterArgs& a, hipStream_t s) {
-  const Plan q = plan_of(a.T, a.K, a.S * a.R);
+  const Plan q = plan_of(a.T, a.K, a.S, a.R);
   const hipError_t e = a.x_type == ADAPTER_E4M3 ? launch_down_plan<true, BF>(a, q, s) : launch_down_plan<false, BF>(a, q, s);
   if (e != hipSuccess) return e;
   switch (a.y_type) {
@@ -765,10 +758,12 @@ hipError_t launch(const AdapterArgs& a, hipStream_t s) {
 }  // namespace
 
 namespace t5k {
-size_t adapter_work_bytes(int T, int K, int SR) {
-  const Plan q = plan_of(T, K, SR);
-  if (q.few) return (size_t)q.splits * T * SR * 4;
-  return ((size_t)T + ROWS - 1) / ROWS * ROWS * SR * 6;  // three parts of 16 bits, whole sixteens of rows
+size_t adapter_work_bytes(int T, int K, int S, int R) {
+  // no less than for fewer rows
+  const int few = std::min(T, few_rows(R));
+  const size_t sums = (size_t)plan_of(few, K, S, R).splits * few * S * R * 4;
+  if (few == T) return sums;
+  return std::max(sums, ((size_t)T + ROWS - 1) / ROWS * ROWS * S * R * 6);  // three parts of 16 bits, whole sixteens of rows
 }
 
 hipError_t launch_adapter(const AdapterArgs& a, hipStream_t s) {
