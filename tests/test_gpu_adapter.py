@@ -401,3 +401,39 @@ def test_a_workspace_serves_fewer_rows(adapters, R, K):
         c.work = work
         c.check(c.run(adapters, work=work))
         assert bool((work[-256:] == 255).all())
+
+
+@pytest.mark.parametrize("K", [16, 32, 112, 128, 144, 496, 768, 2064, 4096])
+@pytest.mark.parametrize("x,w", [("f16", "f16"), ("bf16", "bf16"), ("e4m3", "f16"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("T,R", [(600, 64), (5003, 16), (2100, 128), (17000, 48)])
+def test_depths_of_many_rows(adapters, K, x, w, T, R):
+    """Depths that end inside a step of the first product, whose tiles begin at different ones."""
+    ids = (torch.arange(T) // 37) % 4 - 1
+    _go(adapters, T, K, (48,), R, 3, x=x, w=w, y="f32" if K % 3 else "f16", ids=ids, seed=K + T)
+
+
+@pytest.mark.parametrize("R", [8, 24, 48, 56, 72, 104, 128])
+@pytest.mark.parametrize("S", [1, 2, 4])
+@pytest.mark.parametrize("T", [520, 4500, 9000])
+@pytest.mark.parametrize("x,y", [("f16", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+def test_ranks_of_many_rows(adapters, R, S, T, x, y):
+    """Whole and half tiles of the first product and every number of its ranks, every form of the second."""
+    ids = (torch.arange(T) // 50) % 5 - 1
+    _go(adapters, T, 128, (80, 16, 256, 32)[:S], R, 4, x=x, w=x, y=y, ids=ids, ranks=[R, R // 2, 5, R - 1], seed=R + S + T)
+
+
+@pytest.mark.parametrize("x", ["f16", "e4m3"])
+@pytest.mark.parametrize("R", [8, 64])
+def test_tiles_of_far_rows(adapters, x, R):
+    """Many rows as far apart as may be: a tile of 64 spans 2^31 bytes of x, a sixteen 2^29 of y."""
+    T, K, n, ld = 600, 176, 32, 1 << 24
+    c = Case(T, K, (n,), R, 2, x=x, ids=[0, 1, -1, 1, 0] * (T // 5))
+    far = torch.empty((T - 1) * ld + K, dtype=c.x.dtype, device=DEV)
+    big = torch.empty((T - 1) * ld + n, dtype=c.y.dtype, device=DEV)
+    for t in range(T):
+        far[t * ld:t * ld + K], big[t * ld:t * ld + n] = c.x[t, :K], c.y[t, :n]
+    work = torch.empty(adapters.workspace_bytes(T, K, 1, R), dtype=torch.uint8, device=DEV)
+    adapters.add_device(far.data_ptr(), CODE[x], 0 if c.xs is None else c.xs.data_ptr(), ld, T, K, c.ids.data_ptr(), 2, c.a.data_ptr(),
+                        c.b.data_ptr(), 1, 0, c.scales.data_ptr(), R, (n,), big.data_ptr(), ld, big.data_ptr(), ld, 1,
+                        work.data_ptr(), work.numel(), _stream())
+    c.check(torch.stack([big[t * ld:t * ld + n] for t in range(T)]))
