@@ -137,3 +137,33 @@ def test_captured_run_equals_eager(fp8, T):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(run.qkv.view(torch.int16), want.view(torch.int16)), i
+
+
+def test_failed_calls_leave_no_error(fp8):
+    """Host forms whose buffers no card holds (2 TB, of which nothing is read here), and a device that is not there:
+    the next call on the thread succeeds."""
+    import ctypes as C
+
+    import numpy as np
+
+    from witchcraft_amd import _lib, adapters, rotary
+    buf, lib, cols = np.zeros(4096, np.uint8).ctypes.data, _lib.lib, (C.c_int32 * 1)(64)
+    table = rotary.table(rotary.frequencies(8))
+    x = np.ones((3, 2, 8), np.float16)
+    a, b = np.ones((1, 1, 8, 16), np.float16), np.ones((1, 16, 8), np.float16)
+
+    def good():
+        q, _ = rotary.rotate(x, x, np.zeros(3, np.int32), table)
+        assert (q == 1).all()
+        y = adapters.add(np.ones((3, 16), np.float16), [0, -1, 0], a, b, np.zeros((3, 16), np.float32))
+        assert (y == np.array([128, 0, 128])[:, None]).all()
+        assert int(torch.ones(5, device=DEV).sum()) == 5
+
+    good()
+    for call in (lambda dev: lib.t5h_adapter_add(dev, buf, 1, None, 1 << 20, 1 << 20, buf, 1, buf, buf, 1, None, None, 8, C.addressof(cols), 1,
+                                                 buf, buf, 1),
+                 lambda dev: lib.t5h_rotary(dev, buf, 64, buf, 64, 0, 1 << 24, 512, None, None, 1e-6, buf, 512, 0, buf, 1, buf, buf)):
+        assert call(0) == _lib.T5H_ERR_NOMEM
+        good()
+        assert call(4096) not in (0, _lib.T5H_ERR_NOMEM)
+        good()
