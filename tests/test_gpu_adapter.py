@@ -437,3 +437,59 @@ def test_tiles_of_far_rows(adapters, x, R):
                         c.b.data_ptr(), 1, 0, c.scales.data_ptr(), R, (n,), big.data_ptr(), ld, big.data_ptr(), ld, 1,
                         work.data_ptr(), work.numel(), _stream())
     c.check(torch.stack([big[t * ld:t * ld + n] for t in range(T)]))
+
+
+@pytest.mark.parametrize("w", ["f16", "bf16"])
+@pytest.mark.parametrize("T", [40, 600, 17000])
+def test_codes_that_are_no_numbers(adapters, w, T):
+    """A NaN code and the scale byte that stands for none make their rows NaN, and no others; every other code and the
+    smallest and largest scales count as they are."""
+    c = Case(T, 144, (64,), 8, 3, x="e4m3", w=w, y="f32", ids=[0, 1, 2, 1] * (T // 4))
+    c.b[c.b == 0] = 1
+    good = c.run(adapters).clone()
+    c.x[5, 3], c.x[T - 2, 143] = 0x7f, 0xff
+    c.xs[0, 6], c.xs[1, T - 5] = 255, 255
+    got = c.run(adapters)
+    torch.cuda.synchronize()
+    bad = [5, 6, T - 5, T - 2]
+    assert bool(got[bad, :64].isnan().all())
+    keep = torch.ones(T, dtype=torch.bool, device=DEV)
+    keep[bad] = False
+    assert torch.equal(got[:T, :64][keep], good[:T, :64][keep])
+
+
+@pytest.mark.parametrize("w", ["f16", "bf16"])
+@pytest.mark.parametrize("T", [16, 640])
+def test_every_code(adapters, w, T):
+    """One code and one weight of one to a row: results are the code's value, bit for bit, times each power of two."""
+    codes = torch.tensor([i for i in range(256) if i & 0x7f != 0x7f], dtype=torch.uint8, device=DEV)
+    c = Case(T, 128, (16,), 8, 1, x="e4m3", w=w, y="f32", ids=[0] * T, scales=False)
+    c.y.zero_(), c.a.zero_(), c.b.zero_()
+    c.a[0, 0, 0, 17], c.b[0, :, 0] = 1, 1
+    for i in range(0, 254, T):
+        part = codes[i:i + T]
+        n = len(part)
+        c.x.zero_()
+        c.x[:n, 17] = part
+        for byte in (1, 100, 127, 200, 244):
+            c.xs.fill_(byte)
+            want = part.view(torch.float8_e4m3fn).double() * 2.0 ** (byte - 127)
+            got = c.run(adapters)[:n, :16]
+            # a power of two below f32's normal numbers may be taken as zero
+            fine = (want.abs() >= 2.0 ** -126) | (want == 0)
+            assert torch.equal(got[fine], want.float()[fine, None].expand(-1, 16)), byte
+
+
+@pytest.mark.parametrize("w", ["f16", "bf16"])
+@pytest.mark.parametrize("T", [40, 5000])
+def test_infinite_rows(adapters, w, T):
+    """An infinite inner product makes its row infinite (or NaN, f16 adapters), never finite, and only that row."""
+    c = Case(T, 64, (64,), 8, 1, x=w, w=w, y="f32", ids=[0] * T, scales=False)
+    c.a[:, :, :, 3], c.b[:] = 1, c.b.abs() + 1
+    good = c.run(adapters).clone()
+    c.x[5, 3], c.x[T - 1, 3] = float("inf"), float("-inf")
+    got = c.run(adapters)
+    assert torch.equal(got[[i for i in range(T) if i not in (5, T - 1)], :64], good[[i for i in range(T) if i not in (5, T - 1)], :64])
+    if w == "bf16":
+        assert bool((got[5, :64] == float("inf")).all()) and bool((got[T - 1, :64] == float("-inf")).all())
+    assert not bool(got[[5, T - 1], :64].isfinite().any())
