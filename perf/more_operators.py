@@ -281,13 +281,15 @@ def _own_adapter(s):
 
     case = s["case"]
     n = case["cols"] * case["slices"]
+    # a 32-bit stream takes the sums in place, here as in the plain form
+    out = s["y"] if case["y"] == "f32" else s["out"]
     adapters.add_device(s["x"].data_ptr(), CODE[case["x"]], 0 if s["x_scales"] is None else s["x_scales"].data_ptr(),
                         case["depth"], case["tokens"], case["depth"], s["ids"].data_ptr(), case["adapters"],
                         s["a"].data_ptr(), s["b"].data_ptr(), CODE[case["w"]], s["ranks"].data_ptr(),
                         s["scales"].data_ptr(), case["rank"], (case["cols"],) * case["slices"], s["y"].data_ptr(), n,
-                        s["out"].data_ptr(), n, CODE[case["y"]], s["work"].data_ptr(), s["work"].numel(),
+                        out.data_ptr(), n, CODE[case["y"]], s["work"].data_ptr(), s["work"].numel(),
                         torch.cuda.current_stream().cuda_stream)
-    return {"out": s["out"]}
+    return {"out": out}
 
 
 def _own_rotate(s):
