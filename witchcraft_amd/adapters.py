@@ -44,8 +44,8 @@ def workspace_bytes(t: int, k: int, slices: int, rank: int) -> int:
 
 def add(x, ids, a: np.ndarray, b: np.ndarray, y: np.ndarray, scales=None, ranks=None, cols=None,
         hip_device: int = 0) -> np.ndarray:
-    """y [T, N] (f32 or f16) + scales[ids] * (x a[ids]^T) b[ids]^T: x [T, K] f16 or (codes, scales); a, b f16; cols: the
-    slices' columns (None: all alike)."""
+    """y [T, N] (f32 or f16) + scales[ids] * (x a[ids]^T) b[ids]^T: x [T, K] f16 or (codes, scales); a, b f16; ranks: whole
+    numbers [G] (None: all R; outside 0 .. R the nearer of both); cols: the slices' columns (None: all alike)."""
     if isinstance(x, tuple):
         codes, xs = (np.ascontiguousarray(v) for v in x)
         if codes.ndim != 2 or codes.dtype != np.uint8 or xs.dtype != np.uint8:
@@ -78,7 +78,10 @@ def add(x, ids, a: np.ndarray, b: np.ndarray, y: np.ndarray, scales=None, ranks=
         raise ValueError(f"ids must be whole numbers, one for each of {t} rows, got {given.dtype} {given.shape}")
     which = np.ascontiguousarray(np.where((given < 0) | (given >= g), -1, given), np.int32)
     sp = None if scales is None else np.ascontiguousarray(scales, np.float32)
-    rp = None if ranks is None else np.ascontiguousarray(np.clip(ranks, 0, r), np.int32)
+    own = None if ranks is None else np.asarray(ranks)
+    if own is not None and not np.issubdtype(own.dtype, np.integer):
+        raise ValueError(f"ranks must be whole numbers, got {own.dtype} {own.shape}")
+    rp = None if own is None else np.ascontiguousarray(np.where(own < 0, 0, np.where(own > r, r, own)), np.int32)
     for name, v in (("scales", sp), ("ranks", rp)):
         if v is not None and v.shape != (g,):
             raise ValueError(f"{name} are {v.shape}, there are {g} adapters")
