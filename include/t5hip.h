@@ -345,8 +345,9 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
  *   x: [T] rows of K values, ldx from row to row, of the adapters' type, or e4m3 codes (T5H_TYPE_E4M3) with
  *      scales as t5h_fp8_quantize and t5h_fp8_rmsnorm write them (what the shared product takes).
  *   a: [G][slices][R][K], b: [G][N][R], f16 or bf16, N = the sum of cols[slices] (a HOST array).
- *   ranks: [G] or NULL (all R): adapter g has ranks[g] <= R ranks; past those, up to a multiple of 8, its a
- *      and b hold zeros, and what lies behind is not read.  Values outside 0 .. R count as the nearer of both.
+ *   ranks: [G] or NULL (all R): adapter g has ranks[g] <= R ranks, and what its a and b hold past those does not
+ *      count.  The memory is there all the same, for all of R may be read, and b is finite up to the next multiple
+ *      of 8.  Values outside 0 .. R count as the nearer of both.
  *   scales: [G] f32, or NULL (all 1).
  *   y, out: [T] rows of N values in f32, f16 or bf16; out may be y itself with its row length, or share no
  *      byte with it.  Rows without an adapter are then not touched.

@@ -45,7 +45,8 @@ def workspace_bytes(t: int, k: int, slices: int, rank: int) -> int:
 def add(x, ids, a: np.ndarray, b: np.ndarray, y: np.ndarray, scales=None, ranks=None, cols=None,
         hip_device: int = 0) -> np.ndarray:
     """y [T, N] (f32 or f16) + scales[ids] * (x a[ids]^T) b[ids]^T: x [T, K] f16 or (codes, scales); a, b f16; ranks: whole
-    numbers [G] (None: all R; outside 0 .. R the nearer of both); cols: the slices' columns (None: all alike)."""
+    numbers [G], how many of each adapter's R count (None: all; outside 0 .. R the nearer of both), where b is finite up to
+    the next multiple of 8; cols: the slices' columns (None: all alike)."""
     if isinstance(x, tuple):
         codes, xs = (np.ascontiguousarray(v) for v in x)
         if codes.ndim != 2 or codes.dtype != np.uint8 or xs.dtype != np.uint8:

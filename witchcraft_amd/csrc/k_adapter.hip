@@ -103,7 +103,8 @@ struct Adapters {
   }
 };
 
-// The adapter's rank as it is given, and (the same in all lanes) rounded up to whole eights: what of its weights counts.
+// The adapter's rank as it is given: inner products past it are zeros.  And (the same in all lanes) rounded up to whole
+// eights: what the second product takes of them and of B.
 __device__ __forceinline__ int given_rank(const AdapterArgs& p, int g) { return p.ranks ? p.ranks[g] : p.R; }
 __device__ __forceinline__ int whole_rank(const AdapterArgs& p, int given) {
   const int r = __builtin_amdgcn_readfirstlane(given);
@@ -193,9 +194,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapter_down_few_kernel(Adapte
   const int j = j0 + 4 * g;
   if (wave != 0 || ad.id[0] != ad.current || j >= SR) return;
   for (int k = 1; k < waves; k++) acc += red[k][lane];
-  const int rank = whole_rank(p, given);  // values past it may come from anything
+  // values past the adapter's rank may come from anything
 #pragma unroll
-  for (int e = 0; e < 4; e++) acc[e] = j % p.R < rank ? acc[e] * scale : 0.f;
+  for (int e = 0; e < 4; e++) acc[e] = j % p.R + e < given ? acc[e] * scale : 0.f;
   *(f4*)((float*)p.h + ((size_t)split * p.T + row0 + r) * SR + j) = acc;
 }
 
@@ -323,7 +324,6 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(AdapterArgs p, int
         }
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the ring is free
-      const int rank = whole_rank(p, given);
       int gg = g;
       asm volatile("" : "+v"(gg));           // the addresses of results are left to be computed here
       if (id == ad.current) {  // -1 behind the last row
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(AdapterArgs p, int
           const int slice = j / p.R, at_rank = j - slice * p.R;
           float rest[4];  // values past the adapter's rank may come from anything
 #pragma unroll
-          for (int e = 0; e < 4; e++) rest[e] = at_rank < rank ? v[e] * scale : 0.f;
+          for (int e = 0; e < 4; e++) rest[e] = at_rank + e < given ? v[e] * scale : 0.f;
           uint16_t* to = (uint16_t*)p.h + h_index(row, slice, 0, at_rank, p.S, parts, p.R);
           for (int k = 0; k < parts; k++) {
             uint32_t w[4];
