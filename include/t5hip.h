@@ -352,7 +352,8 @@ int t5h_fp8_gated_gelu_device(const uint8_t* d_a, const uint8_t* d_a_scales, int
  *   y, out: [T] rows of N values in f32, f16 or bf16; out may be y itself with its row length, or share no
  *      byte with it.  Rows without an adapter are then not touched.
  * Sums are f32, and so is the inner product, which goes to the matrix units in bf16 parts: three, which hold all
- * of it, where y is f32, and otherwise two (within 2^-16 of it).  Results are rounded once.
+ * of it, where y is f32, and otherwise two (within 2^-16 of it).  Results are rounded once; a 16-bit one that is
+ * small because y cancels what the adapter adds is off by up to 2^-16 of that, which may be more than its half step.
  * Adapters are finite; an infinity or NaN in a row of x stays in that row, whose results may be NaN where the sums
  * above would be infinite (f16 adapters: a weight's second part may be zero).
  * K is a multiple of 16 up to 2^21, R one of 8 up to 128, columns of a slice one of 16 up to 2^24; T up to

@@ -3,7 +3,9 @@
 Rows hold digits and A's rows the digits' places (a few powers of two each, elsewhere zeros), so that an inner product
 is a whole number of 23 or 24 bits, whose lowest ones lie below what two bf16 parts hold; every partial sum is a whole
 number below 2^24, so f32 sums are exact in any order.  B has one power of two a column, scales are powers of two.
-  * f32 results are then the definition's, bit for bit, which takes all three parts of the inner product.
+  * f32 results are then the definition's, bit for bit, which takes all three parts of the inner product;
+  * 16-bit results may be off by 2^-16 of the inner product's share, and half a step of their type: where y cancels the
+    adapter's share this is more than half a step of what is left.
 """
 import pytest
 
@@ -24,7 +26,7 @@ def _two_parts(h):
 
 
 class Digits(Case):
-    def __init__(self, T, cols, R, x, w, y, seed):
+    def __init__(self, T, cols, R, x, w, y, seed, factor=1.0):
         K, G = 272, 4
         super().__init__(T, K, cols, R, G, x=x, w=w, y=y, seed=seed)
         g = torch.Generator().manual_seed(seed)
@@ -55,7 +57,7 @@ class Digits(Case):
         self.rank = rank[:, :, 0].to(DEV)
         b.scatter_(2, rank, 2.0 ** torch.randint(-2, 3, rank.shape, generator=g).float() * (torch.randint(0, 2, rank.shape, generator=g) * 2 - 1))
         self.b = b.to(TYPE[w]).to(DEV)
-        self.scales = (2.0 ** torch.randint(-1, 3, (G,), generator=g).float()).to(DEV)
+        self.scales = (factor * 2.0 ** torch.randint(-1, 3, (G,), generator=g).float()).to(DEV)
         self.y.zero_()
 
     def inner(self):
@@ -88,3 +90,25 @@ def test_f32_results_take_the_whole_inner_product(adapters, T, R, x, w):  # noqa
     torch.cuda.synchronize()
     assert torch.equal(out[:T, :c.N], (h * b).float())
     c.around(out)
+
+
+@pytest.mark.parametrize("w,y", [("f16", "f16"), ("bf16", "bf16"), ("f16", "bf16"), ("bf16", "f16")])
+@pytest.mark.parametrize("R", [8, 16, 32, 64, 128])
+@pytest.mark.parametrize("T", [40, 700])
+def test_results_that_cancel(adapters, T, R, w, y):  # noqa: F811
+    """y is what the adapter adds, rounded and negative: what is left is that rounding.  Scales take the inner products
+    to some 2^10, within f16's range."""
+    c = Digits(T, (48, 272), R, w, w, y, seed=R + T, factor=2.0 ** -13)
+    h, b = c.inner()
+    add = h * b
+    c.y[:T, :c.N] = (-add).to(c.y.dtype)
+    want = c.y[:T, :c.N].double() + add
+    out = c.run(adapters)[:T, :c.N].double()
+    half = torch.finfo(c.y.dtype).eps / 2
+    left = add.abs() * 2.0 ** -16 + (c.y[:T, :c.N].double().abs() + add.abs()) * 2.0 ** -23  # two parts; f32's own sum
+    least = 2.0 ** -25 if y == "f16" else 0.0
+    tol = left + (want.abs() + left) * half + least
+    assert bool(((out - want).abs() <= tol).all()), float(((out - want).abs() - tol).max())
+    # and y does cancel: what is left is a step of its type
+    mine = c.ids >= 0
+    assert float(want[mine].abs().mean()) < 2 * half * float(add[mine].abs().mean())

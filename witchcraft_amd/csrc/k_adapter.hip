@@ -12,8 +12,11 @@
 //
 // h is f32 and stays so: it is stored as a sum of bf16 parts, all of which multiply the same weights in the second
 // product, as if there were so many times the ranks.  Three parts hold all 24 bits (results in f32), two the upper 16
-// (within 2^-16 of h, where the results' own rounding is 2^-8 or 2^-11).  bf16 has f32's range, which f16 has not; f16
-// weights go in as two bf16 parts, which hold their 11 bits; where the second is zero, an infinite h makes NaN of it.
+// (within 2^-16 of h, where the results' own rounding is 2^-8 or 2^-11).  The third would show where y cancels the
+// adapter's share, and in one of 50 f16 results elsewhere by a step; it costs 1 to 4% with up to 32 ranks (74,640 rows of
+// codes 186 and 193 us) and 8 to 16% with more (16,391 x 4,096 -> 8,192, rank 64, bf16: 167 and 193), so 16-bit results go
+// without.  bf16 has f32's range, which f16 has not; f16 weights go in as two bf16 parts, which hold their 11 bits; where
+// the second is zero, an infinite h makes NaN of it.
 #include "adapter.hpp"
 
 #include <algorithm>
