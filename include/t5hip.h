@@ -388,8 +388,10 @@ int t5h_adapter_add(int32_t hip_device, const void* x, int32_t x_type, const uin
 #define T5H_ROTARY_HALVES 0
 #define T5H_ROTARY_NEIGHBOURS 1
 /* Host only: the table of `pairs` frequencies, in radians per step, finite; axis[i] in 0 .. 7, or axis NULL:
- * all 0.  An entry is the frequency in turns modulo 1, in 61 bits, and the axis in 3, so that angles stay
- * within 2^-29 radians of position * frequency for every 32-bit position. */
+ * all 0.  An entry is the frequency in turns modulo 1, in 61 bits, and the axis in 3, so that angles (ahead of
+ * their rounding to f32) stay within 2^-27 radians of position * frequency for every 32-bit position, where the
+ * frequency is up to one turn (2 pi) a step.  Each further turn a step adds up to 2^-28 at the farthest position:
+ * at 10^12 radians a step, say, far angles mean nothing. */
 int t5h_rotary_table(const double* frequency, const int32_t* axis, int32_t pairs, uint64_t* table);
 /* d_q: T rows of q_heads heads of D values each, ldq values from row to row; d_k likewise; so q and k may
  * be columns of one projection's rows, of which nothing else is read.  Results go to d_q_out and d_k_out,

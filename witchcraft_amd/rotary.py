@@ -37,7 +37,8 @@ def frequencies(rot: int, theta: float = 10000.0) -> np.ndarray:
 
 
 def table(freqs, axes=None) -> np.ndarray:
-    """The table of pairs' frequencies (radians per step) and axes (0 .. 7; None: all 0)."""
+    """The table of pairs' frequencies (radians per step) and axes (0 .. 7; None: all 0).  Angles are within 2^-27 of
+    position * frequency; each turn (2 pi) a step past the first adds up to 2^-28 at positions of 2^31."""
     freqs = np.ascontiguousarray(freqs, np.float64)
     if freqs.ndim != 1:
         raise ValueError(f"frequencies must be 1-D, got shape {freqs.shape}")
