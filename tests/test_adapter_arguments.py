@@ -1,4 +1,4 @@
-"""What witchcraft_amd.adapters takes for ranks, ahead of any device work (no GPU needed).
+"""What witchcraft_amd.adapters takes for ids and ranks, and .rotary for positions, ahead of any device work (no GPU needed).
 
 The library's call is replaced by one that keeps what it is given.
 """
@@ -7,7 +7,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from witchcraft_amd import adapters
+from witchcraft_amd import adapters, rotary
 
 
 def _taken(monkeypatch, module, name, at, n):
@@ -42,3 +42,19 @@ def test_ranks_that_are_whole(monkeypatch, ranks, want):
     seen = _taken(monkeypatch, adapters, "t5h_adapter_add", 11, 2)
     adapters.add(*_inputs(), ranks=ranks)
     assert seen == want
+
+
+def test_no_rows_and_no_adapters():
+    """Empty lists, which numpy takes for floats, are no fractions."""
+    x, ids, a, b, y = _inputs(t=0)
+    assert adapters.add(x, [], a, b, y).shape == (0, 32)
+    assert adapters.add(x, ids, a[:0], b[:0], y, ranks=[], scales=[]).shape == (0, 32)
+
+
+def test_no_positions():
+    q, tab = np.zeros((0, 2, 64), np.float32), rotary.table(rotary.frequencies(64))
+    for none in ([], [[], []], np.zeros((3, 0))):
+        a, b = rotary.rotate(q, q, none, tab)
+        assert a.shape == b.shape == (0, 2, 64)
+    with pytest.raises(ValueError, match="positions"):
+        rotary.rotate(q, q, [0.5], tab)

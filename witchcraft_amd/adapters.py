@@ -75,12 +75,12 @@ def add(x, ids, a: np.ndarray, b: np.ndarray, y: np.ndarray, scales=None, ranks=
     if len(cols) != slices or sum(cols) != b.shape[1]:
         raise ValueError(f"slices of {tuple(cols)} columns, a has {slices}, b {b.shape[1]} columns")
     given = np.asarray(ids)
-    if given.shape != (t,) or not np.issubdtype(given.dtype, np.integer):
+    if given.shape != (t,) or not np.issubdtype(given.dtype, np.integer) and given.size:
         raise ValueError(f"ids must be whole numbers, one for each of {t} rows, got {given.dtype} {given.shape}")
     which = np.ascontiguousarray(np.where((given < 0) | (given >= g), -1, given), np.int32)
     sp = None if scales is None else np.ascontiguousarray(scales, np.float32)
     own = None if ranks is None else np.asarray(ranks)
-    if own is not None and not np.issubdtype(own.dtype, np.integer):
+    if own is not None and not np.issubdtype(own.dtype, np.integer) and own.size:
         raise ValueError(f"ranks must be whole numbers, got {own.dtype} {own.shape}")
     rp = None if own is None else np.ascontiguousarray(np.where(own < 0, 0, np.where(own > r, r, own)), np.int32)
     for name, v in (("scales", sp), ("ranks", rp)):

@@ -85,7 +85,7 @@ def rotate(q: np.ndarray, k: np.ndarray, positions, table: np.ndarray, q_gamma=N
     rows, qh, d = q.shape
     given = np.asarray(positions)
     given = given[None] if given.ndim == 1 else given
-    if given.ndim != 2 or given.shape[1] != rows or not np.issubdtype(given.dtype, np.integer):
+    if given.ndim != 2 or given.shape[1] != rows or not np.issubdtype(given.dtype, np.integer) and given.size:
         raise ValueError(f"positions must be whole numbers [T] or [axes, T], got {given.dtype} {given.shape}")
     if given.size and (given.min() < -2 ** 31 or given.max() >= 2 ** 31):
         raise ValueError("positions must fit 32 bits")
