@@ -264,7 +264,7 @@ hipError_t launch(const RotaryArgs& a, int pairing, hipStream_t s) {
   const Shared u{1.f / (float)a.D, a.rot ? (unsigned)((1 << 20) + a.rot / 2 - 1) / (unsigned)(a.rot / 2) : 0u};
   const dim3 grid(q.blocks + k.blocks);
   const size_t lds = (size_t)std::max(q.tokens, k.tokens) * a.rot * 4;
-  if constexpr (L == 4) {
+  if constexpr (L == 4 && (T == FP8_IO_F32 || V == 8)) {  // of 16-bit values, four to a load never are a whole such head
     if (a.D == 8 * V && a.rot == a.D) {
       if (pairing == ROTARY_HALVES) T5K_LAUNCH((rotary_kernel<T, V, L, true, true>), grid, dim3(256), lds, s, a, u, q, k);
       else T5K_LAUNCH((rotary_kernel<T, V, L, false, true>), grid, dim3(256), lds, s, a, u, q, k);
@@ -282,7 +282,9 @@ hipError_t launch_lanes(const RotaryArgs& a, int pairing, hipStream_t s) {
   if (units <= 8) return launch<T, V, 8>(a, pairing, s);
   if (units <= 16) return launch<T, V, 16>(a, pairing, s);
   if (units <= 32) return launch<T, V, 32>(a, pairing, s);
-  if (units <= 64) return launch<T, V, 64>(a, pairing, s);
+  if constexpr (ROTARY_MAX_DIM > 64 * V) {
+    if (units <= 64) return launch<T, V, 64>(a, pairing, s);
+  }
   return hipErrorInvalidValue;
 }
 }  // namespace
