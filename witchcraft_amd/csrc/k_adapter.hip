@@ -662,9 +662,12 @@ struct Plan {
   int ranks;    // sixteens of ranks of a workgroup
 };
 // The few rows' form reads A once for each sixteen of rows and adapter, and its second product splits h for each 64
-// columns, so it is taken for fewer rows where ranks are many: 512 rows of rank 16 take 11.9 us in it (16 requests, three
-// slices; 46.5 with 64 adapters mixed) and 12.6 (77) in the other, 700 rows 15.9 and 13.9; of rank 64 256 rows take 30.5
-// and 28.7 (8,192 columns) or 15.4 and 21.9 (768), 512 rows 50.8 and 30.8 or 22.0 and 22.7.
+// columns, so it is taken for fewer rows where ranks are many.  Rank 16, K -> columns, 16 requests, this form and the
+// other: 512 rows of 768 codes -> 3 x 768 14.1 and 14.1 us, 4,096 -> 4,096 21.3 and 25.5 (64 adapters mixed 46 and 77); 700
+// rows 17.5 and 15.3, 24.1 and 25.2.  Rank 64, two requests: 256 rows of 4,096 -> 8,192 28.9 and 28.7, of 2,048 -> 768 13.8
+// and 20.0; 512 rows 49.3 and 30.4, 19.3 and 20.8.  It goes by rows and ranks alone, though the other form walks all of K in
+// one workgroup: where K is 8,192, 700 rows of rank 16 -> 4,096 would take 26 us in this form and take 38, and 256 rows of
+// rank 64 -> 8,192 take 32 and would take 44.
 int few_rows(int R) { return std::min(512, 24576 / R); }
 Plan plan_of(int T, int K, int S, int R) {
   Plan q{};
