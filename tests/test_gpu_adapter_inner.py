@@ -15,8 +15,8 @@ torch = pytest.importorskip("torch")
 
 from test_gpu_adapter import DEV, TYPE, Case, adapters  # noqa: E402,F401
 
-# bits of a digit, digits, and where the first and second half of them may lie (codes: in blocks of scales of their own)
-DIGITS = {"f16": (11, 12, 2), "bf16": (8, 8, 3), "e4m3": (4, 4, 6)}  # (bits, places from digit to digit, digits)
+# Bits of a digit, places from digit to digit, digits.  Codes: three each in two blocks with scales of their own.
+DIGITS = {"f16": (11, 12, 2), "bf16": (8, 8, 3), "e4m3": (4, 4, 6)}
 
 
 def _two_parts(h):
